@@ -256,6 +256,60 @@ typedef struct {
 int mlxs_moe_profile_enable(mlxs_moe *h, int on);
 int mlxs_moe_profile_read(mlxs_moe *h, mlxs_moe_profile *out);
 
+/* ---- products over 16-bit weights that the caller keeps in device memory (no counterpart in the reference, whose banks are all
+ * quantised): grouped by expert, and the low-rank adapters of many requests.  Any handle of the device serves them: they take
+ * their own weights, run on `stream`, allocate nothing, keep nothing from call to call and hold no workspace of the handle but
+ * its status word, so calls on several streams, or several captured graphs, may be in flight at once. ---- */
+enum { MLXS_DTYPE_BF16 = 0, MLXS_DTYPE_F16 = 1, MLXS_DTYPE_F32 = 2 };
+/* weight matrices row-major as [outputs, inputs] or [inputs, outputs] */
+enum { MLXS_LAYOUT_OUT_IN = 0, MLXS_LAYOUT_IN_OUT = 1 };
+enum { MLXS_GROUPED_PLAIN = 0, MLXS_GROUPED_SWIGLU = 1 };
+enum { MLXS_ROWS_GATHER = 1, MLXS_ROWS_SCATTER = 2 };
+typedef struct {
+    uint32_t struct_size;         /* sizeof(mlxs_grouped_desc) */
+    uint32_t dtype;               /* of x and w: MLXS_DTYPE_BF16 or _F16 */
+    uint32_t out_dtype;           /* of y: the same type or MLXS_DTYPE_F32 */
+    uint32_t layout;
+    uint32_t act;
+    float act_limit;              /* SWIGLU: > 0 cuts the gate from above and the up row from both sides; 0: no limit */
+    uint32_t n_groups;            /* 1..1024 */
+    uint32_t n_in, n_out;         /* multiples of 8, up to 262,144; SWIGLU: a group's matrix has 2 n_out outputs, the gate's first */
+    uint32_t rows;                /* sorted positions of the call, up to 2^22; offsets_dev[n_groups] <= rows */
+    uint32_t row_flags;           /* MLXS_ROWS_* */
+    uint32_t x_div;               /* GATHER: position p reads row order_dev[p] / x_div of x (top_k: an assignment's token; 1: itself) */
+    uint32_t x_rows, y_rows;      /* rows that x and y have */
+    uint64_t ld_x, ld_y;          /* elements from row to row, multiples of 8 (0: dense) */
+    uint64_t ld_w, w_stride;      /* elements from row to row of a group's matrix and from group to group, multiples of 8 (0: dense) */
+} mlxs_grouped_desc;
+/* y[p] = W_g x[p], or silu(gate_g x[p]) * (up_g x[p]), for the sorted positions offsets_dev[g] <= p < offsets_dev[g + 1]
+ * (u32 [n_groups + 1], as mlxs_moe_sort_rows writes it).  Sums in f32, one rounding to y's type.  Positions of no group, and the
+ * rows of y that no position writes, are left as they were; a group may be empty.  Without GATHER position p reads row p of x,
+ * without SCATTER it writes row p of y; with SCATTER row order_dev[p] (u32 [rows], as mlxs_moe_sort_rows writes it; positions
+ * of one call write different rows).  y overlaps neither x nor w.  An index out of range skips its position, offsets that descend or pass
+ * `rows` are cut to it; both set the status word. */
+int mlxs_moe_grouped(mlxs_moe *h, const mlxs_grouped_desc *desc, const void *x_dev, const void *w_dev,
+                     const uint32_t *offsets_dev, const uint32_t *order_dev, void *y_dev, void *stream);
+
+typedef struct {
+    uint32_t struct_size;         /* sizeof(mlxs_adapters_desc) */
+    uint32_t dtype;               /* of x, a and b: MLXS_DTYPE_BF16 or _F16 */
+    uint32_t out_dtype;           /* of base and y: the same type or MLXS_DTYPE_F32 */
+    uint32_t n_in, n_out;         /* multiples of 8, up to 262,144 */
+    uint32_t rank;                /* rows of an adapter's a, 8..256, a multiple of 8 */
+    uint32_t n_adapters;
+    uint32_t tokens;              /* up to 2^22 */
+    uint64_t ld_x, ld_base, ld_y; /* elements from row to row, multiples of 8 (0: dense) */
+    uint64_t a_stride, b_stride;  /* elements from adapter to adapter, multiples of 8 (0: dense) */
+} mlxs_adapters_desc;
+/* y[t] = base[t] + scale_a (x[t] A_a^T) B_a^T with a = ids_dev[t]; a token with a negative id has no adapter: y[t] = base[t].
+ * a_dev [n_adapters, rank, n_in], b_dev [n_adapters, n_out, rank]; scales_dev f32 [n_adapters] or NULL (1); ranks_dev
+ * i32 [n_adapters] or NULL: how many of an adapter's rank rows count (the others are not looked at).  base_dev NULL: zeros; base_dev == y_dev with
+ * the same row stride: in place.  The inner product is kept in f32 and as two 16-bit parts (16 bits of precision or more) between
+ * the two factors; one rounding to y's type.  An id >= n_adapters counts as none and sets the status word. */
+int mlxs_moe_adapters(mlxs_moe *h, const mlxs_adapters_desc *desc, const void *x_dev, const void *a_dev, const void *b_dev,
+                      const int32_t *ids_dev, const float *scales_dev, const int32_t *ranks_dev, const void *base_dev,
+                      void *y_dev, void *stream);
+
 /* ---- expert parallel (no counterpart in the reference: it pages experts from SSD on one GPU; here they are HBM
  * resident and sharded, with a dispatch and a combine all-to-all per layer) ---- */
 /* 128-byte NCCL unique id made on rank 0 and handed to every rank by the host */

@@ -20,6 +20,10 @@ BANK_EXL3_K3_MUL1, BANK_MXFP4, BANK_NVFP4, BANK_EXL3_K2_MUL1 = 0, 1, 2, 3
 SCORE_SQRTSOFTPLUS, SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1, 2
 ACT_SWIGLU, ACT_SWIGLU_CLAMPED = 0, 1
 COMBINE_F32, COMBINE_CHAIN = 0, 1
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+LAYOUT_OUT_IN, LAYOUT_IN_OUT = 0, 1
+GROUPED_PLAIN, GROUPED_SWIGLU = 0, 1
+ROWS_GATHER, ROWS_SCATTER = 1, 2
 # return codes (include/mlxs_moe.h)
 (E_ARG, E_CONFIG, E_CUDA, E_BANK, E_NOT_LOADED, E_TOO_MANY_TOKENS, E_DEVICE_STATUS, E_MANIFEST, E_EP) = range(-1, -10, -1)
 
@@ -34,6 +38,7 @@ EXPORTS = [
     "mlxs_moe_ep_window_bytes", "mlxs_moe_ep_overloaded_rank",
     "mlxs_moe_status_clear", "mlxs_moe_sort_rows", "mlxs_moe_debug_wait", "mlxs_moe_exl3_decode_rate", "mlxs_moe_fp4_native_probe", "mlxs_moe_mma_rate",
     "mlxs_moe_bank_verify", "mlxs_moe_usage_enable", "mlxs_moe_usage_add", "mlxs_moe_usage_read", "mlxs_moe_usage_reset", "mlxs_moe_plan_placement",
+    "mlxs_moe_grouped", "mlxs_moe_adapters",
 ]
 
 
@@ -69,6 +74,19 @@ class BankInfo(C.Structure):
 class Fp4NativeResult(C.Structure):
     _fields_ = [("rel_l2_hi_lo", C.c_double), ("rel_l2_hi_only", C.c_double), ("tflops_f16", C.c_double),
                 ("tflops_mxf8f6f4", C.c_double), ("tflops_hi_lo_effective", C.c_double)]
+
+
+class GroupedDesc(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("dtype", C.c_uint32), ("out_dtype", C.c_uint32), ("layout", C.c_uint32), ("act", C.c_uint32),
+                ("act_limit", C.c_float), ("n_groups", C.c_uint32), ("n_in", C.c_uint32), ("n_out", C.c_uint32), ("rows", C.c_uint32),
+                ("row_flags", C.c_uint32), ("x_div", C.c_uint32), ("x_rows", C.c_uint32), ("y_rows", C.c_uint32), ("ld_x", C.c_uint64),
+                ("ld_y", C.c_uint64), ("ld_w", C.c_uint64), ("w_stride", C.c_uint64)]
+
+
+class AdaptersDesc(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("dtype", C.c_uint32), ("out_dtype", C.c_uint32), ("n_in", C.c_uint32), ("n_out", C.c_uint32),
+                ("rank", C.c_uint32), ("n_adapters", C.c_uint32), ("tokens", C.c_uint32), ("ld_x", C.c_uint64), ("ld_base", C.c_uint64),
+                ("ld_y", C.c_uint64), ("a_stride", C.c_uint64), ("b_stride", C.c_uint64)]
 
 
 class MlxsError(RuntimeError):
@@ -139,6 +157,8 @@ def lib():
         L.mlxs_moe_status_clear.argtypes = [C.c_void_p]
         L.mlxs_moe_sort_rows.argtypes = [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]
         L.mlxs_moe_debug_wait.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32]
+        L.mlxs_moe_grouped.argtypes = [C.c_void_p, C.POINTER(GroupedDesc)] + [C.c_void_p] * 6
+        L.mlxs_moe_adapters.argtypes = [C.c_void_p, C.POINTER(AdaptersDesc)] + [C.c_void_p] * 9
         if L.mlxs_moe_abi() != ABI:
             raise RuntimeError(f"libmlxs_moe.so ABI {L.mlxs_moe_abi()} != binding ABI {ABI}")
         _lib = L
@@ -321,6 +341,25 @@ class MoE:
     def sort_rows(self, slot, n, n_slots, order, offsets, stream=None):
         """The dispatch permutation alone: slot ids -> order (sorted position -> row) and per-slot offsets."""
         _check(lib().mlxs_moe_sort_rows(self._h, slot, n, n_slots, order, offsets, stream))
+
+    def grouped(self, x, w, offsets, y, rows, n_groups, n_in, n_out, dtype=DTYPE_BF16, out_dtype=None, layout=LAYOUT_OUT_IN,
+                act=GROUPED_PLAIN, act_limit=0.0, order=None, gather=False, scatter=False, x_div=1, x_rows=None, y_rows=None,
+                ld_x=0, ld_y=0, ld_w=0, w_stride=0, stream=None):
+        """Products grouped by expert over 16-bit weights: y[p] = W_g x[p] (or SwiGLU of gate and up) for offsets[g] <= p < offsets[g + 1].
+        order, offsets: as sort_rows writes them; gather reads row order[p] // x_div of x, scatter writes row order[p] of y.
+        y has the type of x unless out_dtype names another."""
+        d = GroupedDesc(C.sizeof(GroupedDesc), dtype, dtype if out_dtype is None else out_dtype, layout, act, act_limit, n_groups, n_in,
+                        n_out, rows, (ROWS_GATHER if gather else 0) | (ROWS_SCATTER if scatter else 0), x_div,
+                        rows if x_rows is None else x_rows, rows if y_rows is None else y_rows, ld_x, ld_y, ld_w, w_stride)
+        _check(lib().mlxs_moe_grouped(self._h, C.byref(d), x, w, offsets, order, y, stream))
+
+    def adapters(self, x, T, a, b, ids, y, n_in, n_out, rank, n_adapters, dtype=DTYPE_BF16, out_dtype=None, base=None, scales=None,
+                 ranks=None, ld_x=0, ld_base=0, ld_y=0, a_stride=0, b_stride=0, stream=None):
+        """Low-rank adapters of many requests: y[t] = base[t] + scale_a B_a (A_a x[t]), a = ids[t]; a negative id: y[t] = base[t].
+        base None: zeros; base == y: in place."""
+        d = AdaptersDesc(C.sizeof(AdaptersDesc), dtype, dtype if out_dtype is None else out_dtype, n_in, n_out, rank, n_adapters, T,
+                         ld_x, ld_base, ld_y, a_stride, b_stride)
+        _check(lib().mlxs_moe_adapters(self._h, C.byref(d), x, a, b, ids, scales, ranks, base, y, stream))
 
     def debug_wait(self, poll_limit=0, withhold_stage=0):
         """Self-test hook of the bounded waits: a short poll limit and one withheld ring stage."""

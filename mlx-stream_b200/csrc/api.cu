@@ -889,6 +889,9 @@ static int read_status(mlxs_moe* h, cudaStream_t st) {
                        : s == ST_WORKLIST_OVERFLOW ? "work list overflow"
                        : s == ST_EP_OVERFLOW ? "expert parallel: a rank received more rows than the workspace holds"
                        : s == ST_EP_TIMEOUT ? "expert parallel: a peer's signal did not arrive within the bound"
+                       : s == ST_BAD_ROW ? "grouped: a gathered or scattered row out of range"
+                       : s == ST_BAD_OFFSETS ? "grouped: group offsets that descend or pass the call's rows"
+                       : s == ST_BAD_ADAPTER ? "adapters: an adapter id out of range"
                                             : "a bounded wait ran out");
     return MLXS_OK;
 }

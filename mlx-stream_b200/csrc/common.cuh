@@ -16,7 +16,10 @@ enum : uint32_t {
     ST_WORKLIST_OVERFLOW = 4,
     ST_NOT_LOADED = 5,       // a routed expert has no resident record
     ST_EP_OVERFLOW = 6,      // expert parallel: a rank received more rows than its workspace holds
-    ST_EP_TIMEOUT = 7        // expert parallel: a peer's epoch word did not arrive within the bound
+    ST_EP_TIMEOUT = 7,       // expert parallel: a peer's epoch word did not arrive within the bound
+    ST_BAD_ROW = 8,          // grouped product: a gathered or scattered row outside its buffer
+    ST_BAD_OFFSETS = 9,      // grouped product: group offsets that descend or pass the call's rows
+    ST_BAD_ADAPTER = 10      // adapters: an id outside [.., n_adapters)
 };
 
 constexpr uint32_t SCALE_BITS = 0x3DB504F3u;  // 128^-0.5 (src/arch/deepseek_v41/experts.zig:428-429)

@@ -286,4 +286,39 @@ cudaError_t launch_dense_logits(const __nv_bfloat16* x, const void* w_tiled, uin
 cudaError_t launch_combine(const void* ro, int ro_bf16, const float* weights, const float* shared, uint32_t T,
                            uint32_t K, uint32_t H, int chain, __nv_bfloat16* y, cudaStream_t st);
 
+// ---- products over 16-bit weights of the caller (grouped.cu) ----
+enum { DT_BF16 = 0, DT_F16 = 1, DT_F32 = 2 };
+struct GroupedArgs {
+    const void* x;
+    const void* w;
+    void* y;
+    const uint32_t* offsets;     // [G + 1]
+    const uint32_t* order;       // [rows] or null
+    uint32_t G, K, N, rows;      // N outputs of y; a group's matrix has n_w() of them
+    uint32_t x_div, x_rows, y_rows;
+    bool gather, scatter, in_out, swiglu;
+    int dtype, out_dtype;
+    float limit;
+    size_t ld_x, ld_y, ld_w, w_stride;
+    uint32_t* status;
+    int sm_count;
+    __host__ __device__ uint32_t n_w() const { return swiglu ? 2 * N : N; }
+};
+cudaError_t launch_grouped(const GroupedArgs& a, cudaStream_t st);
+
+// ---- low-rank adapters (adapters.cu) ----
+struct AdaptersArgs {
+    const void *x, *a, *b, *base;
+    void* y;
+    const int32_t* ids;
+    const float* scales;         // or null
+    const int32_t* ranks;        // or null
+    uint32_t K, N, R, n_adapters, T;
+    int dtype, out_dtype;
+    size_t ld_x, ld_base, ld_y, a_stride, b_stride;
+    uint32_t* status;
+    int sm_count;
+};
+cudaError_t launch_adapters(const AdaptersArgs& a, cudaStream_t st);
+
 }  // namespace mlxs

@@ -123,6 +123,49 @@ pub extern fn mlxs_moe_usage_reset(h: *Moe) c_int;
 pub extern fn mlxs_moe_plan_placement(counts: [*]const u64, n_experts: u32, world: u32, rank_of_expert: [*]u16) c_int;
 pub extern fn mlxs_moe_set_placement(h: *Moe, layer: u32, rank_of_expert: [*]const u16) c_int;
 
+pub const Dtype = enum(u32) { bf16 = 0, f16 = 1, f32 = 2 };
+pub const Layout = enum(u32) { out_in = 0, in_out = 1 };
+pub const GroupedAct = enum(u32) { plain = 0, swiglu = 1 };
+pub const rows_gather: u32 = 1;
+pub const rows_scatter: u32 = 2;
+pub const GroupedDesc = extern struct {
+    struct_size: u32 = @sizeOf(GroupedDesc),
+    dtype: u32,
+    out_dtype: u32,
+    layout: u32,
+    act: u32,
+    act_limit: f32 = 0,
+    n_groups: u32,
+    n_in: u32,
+    n_out: u32,
+    rows: u32,
+    row_flags: u32 = 0,
+    x_div: u32 = 1,
+    x_rows: u32,
+    y_rows: u32,
+    ld_x: u64 = 0,
+    ld_y: u64 = 0,
+    ld_w: u64 = 0,
+    w_stride: u64 = 0,
+};
+pub extern fn mlxs_moe_grouped(h: *Moe, desc: *const GroupedDesc, x_dev: ?*const anyopaque, w_dev: ?*const anyopaque, offsets_dev: ?[*]const u32, order_dev: ?[*]const u32, y_dev: ?*anyopaque, stream: ?*anyopaque) c_int;
+pub const AdaptersDesc = extern struct {
+    struct_size: u32 = @sizeOf(AdaptersDesc),
+    dtype: u32,
+    out_dtype: u32,
+    n_in: u32,
+    n_out: u32,
+    rank: u32,
+    n_adapters: u32,
+    tokens: u32,
+    ld_x: u64 = 0,
+    ld_base: u64 = 0,
+    ld_y: u64 = 0,
+    a_stride: u64 = 0,
+    b_stride: u64 = 0,
+};
+pub extern fn mlxs_moe_adapters(h: *Moe, desc: *const AdaptersDesc, x_dev: ?*const anyopaque, a_dev: ?*const anyopaque, b_dev: ?*const anyopaque, ids_dev: ?[*]const i32, scales_dev: ?[*]const f32, ranks_dev: ?[*]const i32, base_dev: ?*const anyopaque, y_dev: ?*anyopaque, stream: ?*anyopaque) c_int;
+
 pub const Error = error{ Arg, Config, Cuda, Bank, NotLoaded, TooManyTokens, DeviceStatus, Manifest, Ep };
 
 /// rc -> Zig error, the message left at mlxs_moe_last_error() (the reference's Diag carries the same kind of text,
