@@ -6,18 +6,16 @@
 
 namespace mlxs {
 
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ void from_f32(float v, __nv_bfloat16* o) { *o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_f32(float v, __half* o) { *o = __float2half_rn(v); }
-__device__ __forceinline__ void from_f32(float v, float* o) { *o = v; }
 
+// EXACT: the exponential's own function (f32 outputs); without it the product with log2(e) rounds once more, 2^-24 of the exponent,
+// far inside a 16-bit output's half step
+template <bool EXACT>
 __device__ __forceinline__ float gp_swiglu(float g, float u, float limit) {
     if (limit > 0.f) {   // comparisons keep a NaN
         g = g > limit ? limit : g;
         u = u > limit ? limit : (u < -limit ? -limit : u);
     }
-    return __fdividef(g, 1.f + expf(-g)) * u;
+    return __fdividef(g, 1.f + (EXACT ? expf(-g) : __expf(-g))) * u;
 }
 
 // The rows [r0, r1) of group g, cut to the call's rows; false where the offsets had to be cut
@@ -32,27 +30,33 @@ __device__ __forceinline__ bool gp_range(const GroupedArgs& a, uint32_t g, uint3
 // tensor-core tiles
 // ------------------------------------------------------------------------------------------------------------
 constexpr uint32_t GT_KS = 64;                                   // inputs per stage: 128 bytes, one swizzle row
-constexpr uint32_t GT_NT = 256;                                  // most rows of a tile (MMA N)
-constexpr uint32_t GT_STAGES = 6;
-constexpr uint32_t GT_A_BYTES = 128 * GT_KS * 2;                 // a CTA's 128 outputs of a stage
+constexpr uint32_t GT_STAGES = 4;
+constexpr uint32_t GT_A_HALF = 128 * GT_KS * 2;                  // 128 outputs of a stage
+constexpr uint32_t GT_A_BYTES = 2 * GT_A_HALF;                   // a CTA's outputs of a stage: one half per accumulator
 constexpr uint32_t GT_B_BYTES = 128 * GT_KS * 2;                 // at most: a CTA's half of 256 rows
 constexpr uint32_t GT_STAGE = GT_A_BYTES + GT_B_BYTES;
-constexpr uint32_t GT_SWAP_BYTES = 2 * 4 * 2 * 8 * 32 * 4;       // gate / up swap: [buffer][warp pair][side][8 rows][32 outputs] f32
-constexpr uint32_t GT_SMEM = GT_STAGES * GT_STAGE + GT_SWAP_BYTES + 1024;
 constexpr uint32_t GT_MAX_G = 1024;
-constexpr uint32_t GT_EPI_WARPS = 8;
+constexpr uint32_t GT_EPI_WARPS = 8, GT_GATHER_WARPS = 4;
+constexpr uint32_t GT_THREADS = 64 + (GT_EPI_WARPS + GT_GATHER_WARPS + 1) * 32;
+constexpr uint32_t GT_TURN = 8 * 32 * 4;                         // an epilogue warp's turn of 16 rows x 32 outputs, two rows to a word
+constexpr uint32_t GT_SMEM = GT_STAGES * GT_STAGE + GT_EPI_WARPS * 2 * GT_TURN + 1024;
+
+constexpr uint32_t GT_BOXES = 5;
+__host__ __device__ constexpr uint32_t gt_box_rows(uint32_t i) { return i < 3 ? 16u << i : 32 * i; }   // 16 32 64 96 128
 
 struct TileParams {
-    CUtensorMap w, x;
+    CUtensorMap w, x[GT_BOXES];   // x by box height
     GroupedArgs a;
-    uint32_t n_ft, n_ks;     // output tiles of a row tile, stages
-    uint32_t fmt, poll_limit;
+    uint32_t n_ft, n_ks;          // output tiles of a row tile, stages
+    uint32_t cap;                 // most rows of a tile: 128 or 256
+    uint32_t w_loads;             // copies that a stage of weights takes: 1, or 2 x 2 halves
+    uint32_t fmt;
 };
 
 struct GtItem { uint32_t g, p0, rows, n; };   // group, first position, rows, MMA N (a multiple of 32)
 // walks the call's row tiles: tile number -> group and rows.  A group's rows are cut into as few tiles as hold them, all alike.
 struct GtWalk {
-    const uint32_t *off, *tiles;   // [G + 1] positions, [G + 1] first row tile
+    const uint32_t *off, *tiles;   // [G][first, end], [G + 1] first row tile
     uint32_t g = 0;
     __device__ GtItem at(uint32_t tile) {
         while (tiles[g + 1] <= tile) ++g;
@@ -73,31 +77,44 @@ __device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&v)[1
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// true where all 64 threads of a named barrier say so
-__device__ __forceinline__ bool both_warps(uint32_t id, bool ok) {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.u32 p, %2, 0;\n\tbar.red.and.pred r, %1, 64, p;\n\tselp.u32 %0, 1, 0, r;\n\t}" : "=r"(r) : "r"(id), "r"((uint32_t)ok) : "memory");
-    return r != 0;
+// 16 bytes, or zeros where there is nothing to read
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
+}
+// one arrival of this thread on `bar` once all its copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void st_shared4(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 template <bool SWIGLU, class O>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + GT_EPI_WARPS * 32, 1) grouped_tile_kernel(const __grid_constant__ TileParams P) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __grid_constant__ TileParams P) {
     extern __shared__ uint8_t smem_any[];
-    __shared__ __align__(8) uint64_t full_bar[GT_STAGES], empty_bar[GT_STAGES], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) uint64_t full_bar[GT_STAGES], empty_bar[GT_STAGES], acc_full[2], acc_empty[2], row_bar[GT_STAGES];
     __shared__ uint32_t s_tmem, s_off[2 * GT_MAX_G], s_tiles[GT_MAX_G + 1];
     __shared__ volatile int s_abort;
     const GroupedArgs& a = P.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, rank = cluster_rank();
     const uint32_t ring = (smem_u32(smem_any) + 1023u) & ~1023u;
-    float* swap = reinterpret_cast<float*>(smem_any + (ring - smem_u32(smem_any)) + GT_STAGES * GT_STAGE);
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < GT_STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        for (uint32_t s = 0; s < GT_STAGES; ++s) { mbar_init(&full_bar[s], a.gather ? 3 : 1); mbar_init(&empty_bar[s], 1); mbar_init(&row_bar[s], GT_GATHER_WARPS * 32); }
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * GT_EPI_WARPS); }
         s_abort = 0;
         mbar_fence_init();
         tma_prefetch_map(&P.w);
-        tma_prefetch_map(&P.x);
     }
     // the groups' positions and row tiles
     for (uint32_t g = threadIdx.x; g < a.G; g += blockDim.x) {
@@ -109,11 +126,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + GT_EPI_WARPS * 
     if (warp == 0) {
         const uint32_t per = (a.G + 31) / 32, g0 = min(lane * per, a.G), g1 = min(g0 + per, a.G);
         uint32_t mine = 0;
-        for (uint32_t g = g0; g < g1; ++g) mine += (s_off[2 * g + 1] - s_off[2 * g] + GT_NT - 1) / GT_NT;
+        for (uint32_t g = g0; g < g1; ++g) mine += (s_off[2 * g + 1] - s_off[2 * g] + P.cap - 1) / P.cap;
         uint32_t sum = mine;
         for (uint32_t o = 1; o < 32; o <<= 1) { const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, sum, o); if (lane >= o) sum += v; }
         uint32_t at = sum - mine;
-        for (uint32_t g = g0; g < g1; ++g) { s_tiles[g] = at; at += (s_off[2 * g + 1] - s_off[2 * g] + GT_NT - 1) / GT_NT; }
+        for (uint32_t g = g0; g < g1; ++g) { s_tiles[g] = at; at += (s_off[2 * g + 1] - s_off[2 * g] + P.cap - 1) / P.cap; }
         if (lane == 31) s_tiles[a.G] = sum;
     } else if (warp == 1) {
         tmem_alloc_pair(&s_tmem, 512);
@@ -122,48 +139,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + GT_EPI_WARPS * 
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = s_tmem, n_items = s_tiles[a.G] * P.n_ft, n_pairs = gridDim.x / 2, pair = blockIdx.x / 2;
-    constexpr uint32_t FT = SWIGLU ? 128 : 256;                  // outputs of an item
+    constexpr uint32_t FT = SWIGLU ? 256 : 512;                  // outputs of an item: half of them this CTA's
+    // tensor memory: buffers of two accumulators of `cap` columns
+    const uint32_t n_buf = 256 / P.cap;
     auto give_up = [&](uint32_t code) { if (!s_abort) atomicMax(a.status, code); s_abort = 1; };
     GtWalk walk{s_off, s_tiles};
 
     if (warp == 0) {
-        // ---------------- producer: this CTA's half of A's rows and of B's ----------------
+        // ---------------- producer: this CTA's outputs' weights, and its half of the tile's rows where they lie in order ----------------
         const bool gather = a.gather;
         uint32_t s = 0, ph = 0;
         bool ok = true;
         for (uint32_t i = pair; i < n_items && ok; i += n_pairs) {
             const GtItem it = walk.at(i / P.n_ft);
-            const uint32_t f0 = (i % P.n_ft) * FT + rank * (FT / 2), hb = it.n / 2, b0 = it.p0 + rank * hb;
-            const uint32_t nb = (hb + 31) / 32, b_bytes = gather ? hb * GT_KS * 2 : nb * 32 * GT_KS * 2;
-            const uint32_t both = 2 * (GT_A_BYTES + b_bytes);
-            // rows of W behind this CTA's two halves of 64 outputs: one after the other, or the gate's and the up's
-            const uint32_t o0 = f0, o1 = SWIGLU ? a.N + f0 : f0 + 64;
-            int32_t r[4] = {0, 0, 0, 0};
-            if (gather && lane < hb / 4)
-                for (int j = 0; j < 4; ++j) {
-                    // a position behind the tile's last repeats it, an index out of range reads row 0: neither is stored
-                    const uint32_t p = min(b0 + lane * 4 + j, it.p0 + it.rows - 1), xr = a.order[p] / a.x_div;
-                    r[j] = xr < a.x_rows ? (int32_t)xr : 0;
-                }
+            const int32_t f0 = (int32_t)((i % P.n_ft) * FT + rank * (FT / 2)), g = (int32_t)it.g;
+            const uint32_t hb = it.n / 2, b0 = it.p0 + rank * hb, bi = hb <= 16 ? 0 : hb <= 32 ? 1 : (hb + 31) / 32;
+            const uint32_t bytes = 2 * (GT_A_BYTES + (gather ? 0 : gt_box_rows(bi) * GT_KS * 2));   // both CTAs' copies
             for (uint32_t ks = 0; ks < P.n_ks; ++ks) {
                 if (!mbar_wait_warp_at(smem_u32(&empty_bar[s]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
-                const uint32_t full = map_to_rank(smem_u32(&full_bar[s]), 0), sa = ring + s * GT_STAGE, sb = sa + GT_A_BYTES;
-                const int32_t k = (int32_t)(ks * GT_KS);
                 if (lane == 0) {
-                    if (rank == 0) mbar_expect_tx(&full_bar[s], both);
-                    if (a.in_out) {
-                        tma_load_3d(sa, &P.w, (int32_t)o0, k, (int32_t)it.g, full);
-                        tma_load_3d(sa + GT_A_BYTES / 2, &P.w, (int32_t)o1, k, (int32_t)it.g, full);
+                    const uint32_t full = map_to_rank(smem_u32(&full_bar[s]), 0), sa = ring + s * GT_STAGE;
+                    const int32_t k = (int32_t)(ks * GT_KS);
+                    if (rank == 0) mbar_expect_tx(&full_bar[s], bytes);
+                    if (!a.in_out) {
+                        tma_load_4d(sa, &P.w, k, f0, 0, g, full);
+                    } else if (SWIGLU) {
+                        // 64 outputs, 64 inputs, gate and up: the halves of one accumulator's tile lie 16 KB apart in the box's order
+                        tma_load_4d(sa, &P.w, f0, k, 0, g, full);
+                        tma_load_4d(sa + GT_A_HALF, &P.w, f0 + 64, k, 0, g, full);
+                    } else if (P.w_loads == 1) {
+                        tma_load_4d(sa, &P.w, 0, k, f0 / 64, g, full);
                     } else {
-                        tma_load_3d(sa, &P.w, k, (int32_t)o0, (int32_t)it.g, full);
-                        tma_load_3d(sa + GT_A_BYTES / 2, &P.w, k, (int32_t)o1, (int32_t)it.g, full);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) tma_load_4d(sa + j * (GT_A_HALF / 2), &P.w, f0 + j * 64, k, 0, g, full);
                     }
+                    if (!gather) tma_load_2d(sa + GT_A_BYTES, &P.x[bi], k, (int32_t)b0, full);
                 }
-                if (gather) {
-                    if (lane < hb / 4) tma_gather4(sb + lane * 4 * 128, &P.x, k, r[0], r[1], r[2], r[3], full);
-                } else if (lane < nb) {
-                    tma_load_2d(sb + lane * 32 * 128, &P.x, k, (int32_t)(b0 + lane * 32), full);
-                }
+                __syncwarp();
                 if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
             }
         }
@@ -173,52 +185,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + GT_EPI_WARPS * 
         if (rank == 0) {
             uint32_t s = 0, ph = 0, n_done = 0;
             bool ok = true;
+            // K-major: 16 inputs are 32 bytes of every row; M-major: 16 rows of 128 bytes.  M-major 64-output tiles of one accumulator:
+            // 8 KB apart, but for the activation's boxes (gate and up of 64 outputs) 16 KB
+            const uint32_t a_step = a.in_out ? 2048u : 32u, a_lbo = !a.in_out ? 16u : SWIGLU ? GT_A_HALF : GT_A_HALF / 2;
+            const uint32_t a_next = a.in_out && SWIGLU ? GT_A_HALF / 2 : GT_A_HALF;   // to the second accumulator's tile
             for (uint32_t i = pair; i < n_items && ok; i += n_pairs) {
                 const GtItem it = walk.at(i / P.n_ft);
-                const uint32_t idesc = umma_idesc_pair(P.fmt, it.n, a.in_out), buf = n_done & 1u, acc = tmem + buf * 256;
-                if (!mbar_wait_cluster(smem_u32(&acc_empty[buf]), (n_done >> 1 & 1u) ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; }
-                ok = __all_sync(0xFFFFFFFFu, ok);
-                if (!ok) break;
+                const uint32_t idesc = umma_idesc_pair(P.fmt, it.n, a.in_out), buf = n_done % n_buf, acc = tmem + buf * 2 * P.cap;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_empty[buf]), (n_done / n_buf & 1u) ^ 1u, &s_abort));
+                if (!ok) { give_up(ST_WAIT_EMPTY); break; }
                 tc_fence_after();
                 for (uint32_t ks = 0; ks < P.n_ks; ++ks) {
-                    if (!mbar_wait_cluster(smem_u32(&full_bar[s]), ph, &s_abort)) { give_up(ST_WAIT_FULL); ok = false; }
-                    ok = __all_sync(0xFFFFFFFFu, ok);
-                    if (!ok) break;
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&full_bar[s]), ph, &s_abort));
+                    if (!ok) { give_up(ST_WAIT_FULL); break; }
                     tc_fence_after();
                     const uint32_t sa = ring + s * GT_STAGE, sb = sa + GT_A_BYTES;
-                    // K-major: 16 inputs are 32 bytes of every row; M-major: 16 rows of 128 bytes
-                    const uint32_t a_step = a.in_out ? 2048u : 32u;
                     if (elect_one()) {
 #pragma unroll
-                        for (uint32_t j = 0; j < GT_KS / 16; ++j)
-                            umma_f16_pair(acc, umma_desc_sw128(sa + j * a_step, a.in_out ? GT_A_BYTES / 2 : 16, 1024),
-                                          umma_desc_sw128(sb + j * 32, 16, 1024), idesc, ks | j ? 1u : 0u);
+                        for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                            for (uint32_t j = 0; j < GT_KS / 16; ++j)
+                                umma_f16_pair(acc + h * P.cap, umma_desc_sw128(sa + h * a_next + j * a_step, a_lbo, 1024),
+                                              umma_desc_sw128(sb + j * 32, 16, 1024), idesc, ks | j ? 1u : 0u);
                         umma_commit_pair(smem_u32(&empty_bar[s]), 3);
                     }
                     __syncwarp();
                     if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
                 }
-                if (ok && elect_one()) umma_commit_pair(smem_u32(&acc_full[buf]), 3);
+                if (!ok) break;
+                if (elect_one()) umma_commit_pair(smem_u32(&acc_full[buf]), 3);
                 __syncwarp();
                 ++n_done;
             }
         }
-    } else {
-        // ---------------- epilogue: a thread owns one lane (output) of the accumulator; a warp half of the tile's rows ----------------
+    } else if (warp < 2 + GT_EPI_WARPS) {
+        // ---------------- epilogue: a thread owns a lane (output) of both accumulators; a warp every other 16 rows of the tile ----------------
         const uint32_t q = warp & 3u, half = (warp - 2) >> 2;
-        uint32_t n_done = 0, swaps = 0;
+        uint32_t n_done = 0;
         O* y = static_cast<O*>(a.y);
+        const uint32_t turn = ring + GT_STAGES * GT_STAGE + (warp - 2) * 2 * GT_TURN;
         for (uint32_t i = pair; i < n_items; i += n_pairs) {
             const GtItem it = walk.at(i / P.n_ft);
-            const uint32_t buf = n_done & 1u, f0 = (i % P.n_ft) * FT + rank * (FT / 2);
-            bool got = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_full[buf]), n_done >> 1 & 1u, &s_abort));
-            if (SWIGLU) got = both_warps(1 + half * 2 + (q & 1u), got);   // the two warps of a swap go on, or give up, together
-            if (!got) { give_up(ST_WAIT_FULL); break; }
+            const uint32_t buf = n_done % n_buf, f = (i % P.n_ft) * FT + rank * (FT / 2) + q * 32 + lane;
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_full[buf]), n_done / n_buf & 1u, &s_abort))) { give_up(ST_WAIT_FULL); break; }
             tc_fence_after();
-            const uint32_t f = f0 + (SWIGLU ? (q & 1u) * 32 : q * 32) + lane;
-            for (uint32_t c = half * 16; c < it.n; c += 32) {
-                uint32_t v[16];
-                tmem_ld16_nowait(tmem + buf * 256 + c + ((q * 32u) << 16), v);
+            for (uint32_t c = half * 16; c < it.rows; c += 32) {
+                uint32_t v0[16], v1[16];
+                tmem_ld16_nowait(tmem + buf * 2 * P.cap + c + ((q * 32u) << 16), v0);
+                tmem_ld16_nowait(tmem + buf * 2 * P.cap + P.cap + c + ((q * 32u) << 16), v1);
                 // lane j < 16: where row c + j of the tile goes
                 uint32_t yr = 0xFFFFFFFFu;
                 if (lane < 16 && c + lane < it.rows) {
@@ -227,27 +241,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + GT_EPI_WARPS * 
                     if ((a.gather && o / a.x_div >= a.x_rows) || yr >= a.y_rows) { yr = 0xFFFFFFFFu; atomicMax(a.status, ST_BAD_ROW); }
                 }
                 tmem_wait_ld();
-                if (SWIGLU) {
-                    // Warps q and q + 2 hold gate and up of the same outputs: the first takes rows 0 .. 7 of the chunk, the second
-                    // 8 .. 15, and each gives the other what it needs.
-                    const uint32_t pr = half * 2 + (q & 1u), up = q >> 1;
-                    float* b = swap + ((swaps & 1u) * 4 + pr) * 512;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) b[(up * 8 + j) * 32 + lane] = __uint_as_float(up ? v[j] : v[8 + j]);
-                    asm volatile("bar.sync %0, 64;" ::"r"(1 + pr) : "memory");
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float other = b[((up ^ 1u) * 8 + j) * 32 + lane], mine = __uint_as_float(up ? v[8 + j] : v[j]);
-                        const uint32_t row = __shfl_sync(0xFFFFFFFFu, yr, up * 8 + j);
-                        const float z = up ? gp_swiglu(other, mine, a.limit) : gp_swiglu(mine, other, a.limit);
-                        if (row != 0xFFFFFFFFu && f < a.N) from_f32(z, y + (size_t)row * a.ld_y + f);
-                    }
-                    ++swaps;
-                } else {
+                if constexpr (sizeof(O) == 4) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const uint32_t row = __shfl_sync(0xFFFFFFFFu, yr, j);
-                        if (row != 0xFFFFFFFFu && f < a.N) from_f32(__uint_as_float(v[j]), y + (size_t)row * a.ld_y + f);
+                        if (row == 0xFFFFFFFFu) continue;
+                        float* o = reinterpret_cast<float*>(y) + (size_t)row * a.ld_y + f;
+                        if (SWIGLU) {
+                            if (f < a.N) *o = gp_swiglu<true>(__uint_as_float(v0[j]), __uint_as_float(v1[j]), a.limit);
+                        } else {
+                            if (f < a.N) *o = __uint_as_float(v0[j]);
+                            if (f + 128 < a.N) o[128] = __uint_as_float(v1[j]);
+                        }
+                    }
+                } else {
+                    // two rows to a word, turned through shared memory: a lane then stores four outputs (8 bytes) of a row, a warp
+                    // instruction four rows
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float x0 = __uint_as_float(v0[2 * k]), x1 = __uint_as_float(v0[2 * k + 1]);
+                        const float z0 = __uint_as_float(v1[2 * k]), z1 = __uint_as_float(v1[2 * k + 1]);
+                        if (SWIGLU) {
+                            st_shared4(turn + (k * 32 + lane) * 4, pack2(gp_swiglu<false>(x0, z0, a.limit), gp_swiglu<false>(x1, z1, a.limit), O()));
+                        } else {
+                            st_shared4(turn + (k * 32 + lane) * 4, pack2(x0, x1, O()));
+                            st_shared4(turn + GT_TURN + (k * 32 + lane) * 4, pack2(z0, z1, O()));
+                        }
+                    }
+                    __syncwarp();
+                    const uint32_t fq = f - lane + (lane & 7u) * 4;
+#pragma unroll
+                    for (uint32_t i2 = 0; i2 < 2; ++i2) {
+                        const uint32_t k = (lane >> 3) + 4 * i2;
+                        const uint32_t ra = __shfl_sync(0xFFFFFFFFu, yr, 2 * k), rb = __shfl_sync(0xFFFFFFFFu, yr, 2 * k + 1);
+                        O *oa = y + (size_t)ra * a.ld_y + fq, *ob = y + (size_t)rb * a.ld_y + fq;
+#pragma unroll
+                        for (uint32_t h = 0; h < (SWIGLU ? 1u : 2u); ++h) {
+                            const uint4 w = ld_shared16(turn + h * GT_TURN + k * 128 + (lane & 7u) * 16);
+                            if (fq + h * 128 < a.N) {
+                                if (ra != 0xFFFFFFFFu) *reinterpret_cast<uint2*>(oa + h * 128) = make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.z, w.w, 0x5410));
+                                if (rb != 0xFFFFFFFFu) *reinterpret_cast<uint2*>(ob + h * 128) = make_uint2(__byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x7632));
+                            }
+                        }
                     }
                 }
             }
@@ -256,6 +292,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + GT_EPI_WARPS * 
             if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[buf]), 0));
             ++n_done;
         }
+    } else if (a.gather && warp < 2 + GT_EPI_WARPS + GT_GATHER_WARPS) {
+        // ---------------- gathered rows: eight lanes copy 128 bytes of a row, a warp 32 rows of a stage ----------------
+        const uint32_t r_in = (warp - 2 - GT_EPI_WARPS) * 32 + (lane >> 3), chunk = lane & 7u;
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        for (uint32_t i = pair; i < n_items && ok; i += n_pairs) {
+            const GtItem it = walk.at(i / P.n_ft);
+            const uint32_t hb = it.n / 2, t0 = rank * hb;         // this CTA's rows of the tile: t0 .. t0 + hb
+            const uint16_t* src[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) {
+                // rows behind the tile's last are not copied (what their columns hold is not stored), an index out of range reads row 0
+                const uint32_t r = r_in + j * 4;
+                src[j] = nullptr;
+                if (r < hb && t0 + r < it.rows) {
+                    const uint32_t xr = a.order[it.p0 + t0 + r] / a.x_div;
+                    src[j] = static_cast<const uint16_t*>(a.x) + (size_t)(xr < a.x_rows ? xr : 0) * a.ld_x + chunk * 8;
+                }
+            }
+            for (uint32_t ks = 0; ks < P.n_ks; ++ks) {
+                if (!mbar_wait_warp_at(smem_u32(&empty_bar[s]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
+                const uint32_t sb = ring + s * GT_STAGE + GT_A_BYTES, k = ks * GT_KS;
+                const bool there = k + chunk * 8 < a.K;           // K is a multiple of 8
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    const uint32_t r = r_in + j * 4;
+                    if (src[j]) cp_async16(sb + r * 128 + ((chunk ^ (r & 7u)) << 4), src[j] + (there ? k : 0u), there);
+                }
+                cp_async_arrive(smem_u32(&row_bar[s]));
+                if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (a.gather) {
+        // ---------------- a stage's gathered rows have landed: make them the tensor core's to read, and say so to the even CTA's issuer ----------------
+        // (a warp of its own, so that the copying warps run ahead as far as the ring lets them)
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        for (uint32_t i = pair; i < n_items && ok; i += n_pairs)
+            for (uint32_t ks = 0; ks < P.n_ks; ++ks) {
+                if (!mbar_wait_warp_at(smem_u32(&row_bar[s]), ph, &s_abort)) { give_up(ST_WAIT_FULL); ok = false; break; }
+                if (lane == 0) {
+                    fence_async_smem();
+                    mbar_arrive_cluster(map_to_rank(smem_u32(&full_bar[s]), 0));
+                }
+                __syncwarp();
+                if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
+            }
     }
     // every thread comes here, also after a give-up
     tc_fence_before();
@@ -277,15 +361,19 @@ static EncodeTiled encode_tiled() {
     }();
     return fn;
 }
-// a matrix (rank 2) or a stack of matrices (3) of 16-bit elements: boxes of 64 inner elements, rows swizzled over 128 bytes
-static cudaError_t encode_map(CUtensorMap* map, int dtype, int rank, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t ld, uint64_t stride,
-                              uint32_t box1) {
+// 16-bit elements, boxes of 64 inner elements, rows swizzled over 128 bytes; dims, strides (in elements, from the second dimension on) and
+// box from the innermost out; what lies outside reads as zero
+template <int RANK>
+static cudaError_t encode_map(CUtensorMap* map, int dtype, const void* base, const uint64_t (&dims)[RANK], const uint64_t (&strides)[RANK - 1],
+                              const uint32_t (&box)[RANK]) {
     const EncodeTiled fn = encode_tiled();
     if (!fn) return cudaErrorNotSupported;
-    const cuuint64_t dims[3] = {d0, d1, d2}, strides[2] = {ld * 2, stride * 2};
-    const cuuint32_t box[3] = {64, box1, 1}, step[3] = {1, 1, 1};
-    const CUresult r = fn(map, dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(base),
-                          dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    cuuint64_t d[RANK], s[RANK - 1];
+    cuuint32_t b[RANK], step[RANK];
+    for (int i = 0; i < RANK; ++i) { d[i] = dims[i]; b[i] = box[i]; step[i] = 1; }
+    for (int i = 0; i < RANK - 1; ++i) s[i] = strides[i] * 2;
+    const CUresult r = fn(map, dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)RANK, const_cast<void*>(base),
+                          d, s, b, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
@@ -294,16 +382,32 @@ template <bool SWIGLU, class O>
 static cudaError_t tile_launch(const GroupedArgs& a, cudaStream_t st) {
     TileParams P;
     P.a = a;
-    P.n_ft = (a.N + (SWIGLU ? 127 : 255)) / (SWIGLU ? 128 : 256);
+    P.n_ft = (a.N + (SWIGLU ? 255 : 511)) / (SWIGLU ? 256 : 512);
     P.n_ks = (a.K + GT_KS - 1) / GT_KS;
     P.fmt = a.dtype == DT_BF16 ? UMMA_BF16 : UMMA_F16;
-    cudaError_t e = a.in_out ? encode_map(&P.w, a.dtype, 3, a.w, a.n_w(), a.K, a.G, a.ld_w, a.w_stride, 64)
-                             : encode_map(&P.w, a.dtype, 3, a.w, a.K, a.n_w(), a.G, a.ld_w, a.w_stride, 64);
-    if (e == cudaSuccess) e = encode_map(&P.x, a.dtype, 2, a.x, a.K, a.x_rows, 1, a.ld_x, 0, a.gather ? 1 : 32);
+    P.w_loads = 1;
+    P.cap = a.rows / a.G > 96 ? 256 : 128;
+    cudaError_t e;
+    const uint64_t N = a.N, K = a.K, G = a.G, ld = a.ld_w, gs = a.w_stride;
+    // A box is one CTA's weights of a stage.  Activation: gate rows, then up rows (outputs first), or 64 outputs' gate and up
+    // (inputs first).  Plain, inputs first: four blocks of 64 outputs, by one copy where the outputs are a multiple of 64
+    if (!a.in_out)
+        e = SWIGLU ? encode_map<4>(&P.w, a.dtype, a.w, {K, N, 2, G}, {ld, N * ld, gs}, {64, 128, 2, 1})
+                   : encode_map<4>(&P.w, a.dtype, a.w, {K, N, 1, G}, {ld, ld, gs}, {64, 256, 1, 1});
+    else if (SWIGLU)
+        e = encode_map<4>(&P.w, a.dtype, a.w, {N, K, 2, G}, {ld, N, gs}, {64, 64, 2, 1});
+    else if (N % 64 == 0)
+        e = encode_map<4>(&P.w, a.dtype, a.w, {64, K, N / 64, G}, {ld, 64, gs}, {64, 64, 4, 1});
+    else {
+        P.w_loads = 4;
+        e = encode_map<4>(&P.w, a.dtype, a.w, {N, K, 1, G}, {ld, ld, gs}, {64, 64, 1, 1});
+    }
+    for (uint32_t i = 0; i < GT_BOXES && !a.gather && e == cudaSuccess; ++i)
+        e = encode_map<2>(&P.x[i], a.dtype, a.x, {K, a.x_rows}, {a.ld_x}, {64, gt_box_rows(i)});
     if (e != cudaSuccess) return e;
     const auto kernel = grouped_tile_kernel<SWIGLU, O>;
     if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GT_SMEM)) != cudaSuccess) return e;
-    kernel<<<a.sm_count / 2 * 2, 64 + GT_EPI_WARPS * 32, GT_SMEM, st>>>(P);
+    kernel<<<a.sm_count / 2 * 2, GT_THREADS, GT_SMEM, st>>>(P);
     return cudaGetLastError();
 }
 template <class O>
