@@ -36,8 +36,8 @@ constexpr uint32_t GT_A_BYTES = 2 * GT_A_HALF;                   // a CTA's outp
 constexpr uint32_t GT_B_BYTES = 128 * GT_KS * 2;                 // at most: a CTA's half of 256 rows
 constexpr uint32_t GT_STAGE = GT_A_BYTES + GT_B_BYTES;
 constexpr uint32_t GT_MAX_G = 1024;
-constexpr uint32_t GT_EPI_WARPS = 8, GT_GATHER_WARPS = 4;
-constexpr uint32_t GT_THREADS = 64 + (GT_EPI_WARPS + GT_GATHER_WARPS + 1) * 32;
+constexpr uint32_t GT_EPI_WARPS = 8, GT_GATHER_WARPS = GT_STAGES;   // gathered rows: a warp to a ring slot
+constexpr uint32_t GT_THREADS = 64 + (GT_EPI_WARPS + GT_GATHER_WARPS) * 32;
 constexpr uint32_t GT_TURN = 8 * 32 * 4;                         // an epilogue warp's turn of 16 rows x 32 outputs, two rows to a word
 constexpr uint32_t GT_SMEM = GT_STAGES * GT_STAGE + GT_EPI_WARPS * 2 * GT_TURN + 1024;
 
@@ -81,10 +81,6 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
 }
-// one arrival of this thread on `bar` once all its copies so far have landed
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ void st_shared4(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
     uint4 v;
@@ -103,14 +99,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
 template <bool SWIGLU, class O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __grid_constant__ TileParams P) {
     extern __shared__ uint8_t smem_any[];
-    __shared__ __align__(8) uint64_t full_bar[GT_STAGES], empty_bar[GT_STAGES], acc_full[2], acc_empty[2], row_bar[GT_STAGES];
-    __shared__ uint32_t s_tmem, s_off[2 * GT_MAX_G], s_tiles[GT_MAX_G + 1];
+    __shared__ __align__(8) uint64_t full_bar[GT_STAGES], empty_bar[GT_STAGES], acc_full[2], acc_empty[2];
+    __shared__ uint32_t s_tmem, s_off[2 * GT_MAX_G], s_tiles[GT_MAX_G + 1], s_row[GT_GATHER_WARPS][128];
     __shared__ volatile int s_abort;
     const GroupedArgs& a = P.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, rank = cluster_rank();
     const uint32_t ring = (smem_u32(smem_any) + 1023u) & ~1023u;
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < GT_STAGES; ++s) { mbar_init(&full_bar[s], a.gather ? 3 : 1); mbar_init(&empty_bar[s], 1); mbar_init(&row_bar[s], GT_GATHER_WARPS * 32); }
+        for (uint32_t s = 0; s < GT_STAGES; ++s) { mbar_init(&full_bar[s], a.gather ? 3 : 1); mbar_init(&empty_bar[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * GT_EPI_WARPS); }
         s_abort = 0;
         mbar_fence_init();
@@ -292,54 +288,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) group
             if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[buf]), 0));
             ++n_done;
         }
-    } else if (a.gather && warp < 2 + GT_EPI_WARPS + GT_GATHER_WARPS) {
-        // ---------------- gathered rows: eight lanes copy 128 bytes of a row, a warp 32 rows of a stage ----------------
-        const uint32_t r_in = (warp - 2 - GT_EPI_WARPS) * 32 + (lane >> 3), chunk = lane & 7u;
-        uint32_t s = 0, ph = 0;
+    } else if (a.gather) {
+        // ---------------- gathered rows: a warp to a ring slot, so that waiting for its copies keeps nobody; eight lanes copy 128 bytes of a row ----------------
+        // (one arrival per warp and stage: with one per thread, posted by the copies themselves, the arrivals took longer than the stage)
+        const uint32_t slot = warp - 2 - GT_EPI_WARPS, r_in = lane >> 3, chunk = lane & 7u;
+        const uint32_t sb = ring + slot * GT_STAGE + GT_A_BYTES, full = map_to_rank(smem_u32(&full_bar[slot]), 0);
+        uint32_t ph = 0, base = 0;                                // stages of the items before, modulo the ring
         bool ok = true;
         for (uint32_t i = pair; i < n_items && ok; i += n_pairs) {
             const GtItem it = walk.at(i / P.n_ft);
-            const uint32_t hb = it.n / 2, t0 = rank * hb;         // this CTA's rows of the tile: t0 .. t0 + hb
-            const uint16_t* src[8];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) {
-                // rows behind the tile's last are not copied (what their columns hold is not stored), an index out of range reads row 0
-                const uint32_t r = r_in + j * 4;
-                src[j] = nullptr;
-                if (r < hb && t0 + r < it.rows) {
-                    const uint32_t xr = a.order[it.p0 + t0 + r] / a.x_div;
-                    src[j] = static_cast<const uint16_t*>(a.x) + (size_t)(xr < a.x_rows ? xr : 0) * a.ld_x + chunk * 8;
-                }
+            // this CTA's rows of the tile; what the columns behind the tile's last row hold is not stored
+            const uint32_t hb = it.n / 2, t0 = rank * hb, valid = it.rows > t0 ? min(hb, it.rows - t0) : 0;
+            __syncwarp();
+            for (uint32_t r = lane; r < valid; r += 32) {
+                const uint32_t xr = a.order[it.p0 + t0 + r] / a.x_div;
+                s_row[slot][r] = xr < a.x_rows ? xr : 0;          // out of range: reads row 0, the epilogue skips it
             }
-            for (uint32_t ks = 0; ks < P.n_ks; ++ks) {
-                if (!mbar_wait_warp_at(smem_u32(&empty_bar[s]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
-                const uint32_t sb = ring + s * GT_STAGE + GT_A_BYTES, k = ks * GT_KS;
-                const bool there = k + chunk * 8 < a.K;           // K is a multiple of 8
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    const uint32_t r = r_in + j * 4;
-                    if (src[j]) cp_async16(sb + r * 128 + ((chunk ^ (r & 7u)) << 4), src[j] + (there ? k : 0u), there);
-                }
-                cp_async_arrive(smem_u32(&row_bar[s]));
-                if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
-            }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (a.gather) {
-        // ---------------- a stage's gathered rows have landed: make them the tensor core's to read, and say so to the even CTA's issuer ----------------
-        // (a warp of its own, so that the copying warps run ahead as far as the ring lets them)
-        uint32_t s = 0, ph = 0;
-        bool ok = true;
-        for (uint32_t i = pair; i < n_items && ok; i += n_pairs)
-            for (uint32_t ks = 0; ks < P.n_ks; ++ks) {
-                if (!mbar_wait_warp_at(smem_u32(&row_bar[s]), ph, &s_abort)) { give_up(ST_WAIT_FULL); ok = false; break; }
-                if (lane == 0) {
-                    fence_async_smem();
-                    mbar_arrive_cluster(map_to_rank(smem_u32(&full_bar[s]), 0));
-                }
+            __syncwarp();
+            for (uint32_t ks = (slot + GT_STAGES - base) % GT_STAGES; ks < P.n_ks; ks += GT_STAGES) {
+                if (!mbar_wait_warp_at(smem_u32(&empty_bar[slot]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
+                const uint32_t k = ks * GT_KS + chunk * 8;
+                const bool there = k < a.K;                       // K is a multiple of 8
+                const uint16_t* x = static_cast<const uint16_t*>(a.x) + (there ? k : 0);
+#pragma unroll 8
+                for (uint32_t r = r_in; r < valid; r += 4)
+                    cp_async16(sb + r * 128 + ((chunk ^ (r & 7u)) << 4), x + (size_t)s_row[slot][r] * a.ld_x, there);
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async_smem();
                 __syncwarp();
-                if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
+                if (lane == 0) mbar_arrive_cluster(full);
+                ph ^= 1u;
             }
+            base = (base + P.n_ks) % GT_STAGES;
+        }
     }
     // every thread comes here, also after a give-up
     tc_fence_before();
