@@ -373,6 +373,15 @@ def test_adapters_against_64_bits(moe, T, kind):
         c.check((dtype, out))
 
 
+@pytest.mark.parametrize("n, T", [(511, 700), (512, 700), (3, 4096), (3, 4097), (511, 9000), (600, 130), (2, 65)])
+@pytest.mark.parametrize("kind", ["mixed", "runs", "same"])
+def test_adapters_many_tokens_and_many_adapters(moe, n, T, kind):
+    """Around the sorting form's limits: 511 adapters, segments of 4096 tokens, units of 64."""
+    c = Adapters(some_ids(T, n, kind), n, 8, 40, 24, "bf16", "f32", pad=8)
+    c.call(moe)
+    c.check()
+
+
 @pytest.mark.parametrize("R", [8, 16, 24, 64, 72, 128, 200, 256])
 @pytest.mark.parametrize("K, N", [(8, 8), (72, 264), (1032, 1400), (2304, 512)])
 def test_adapters_widths(moe, R, K, N):
