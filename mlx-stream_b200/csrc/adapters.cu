@@ -23,6 +23,8 @@ namespace mlxs {
 constexpr uint32_t AD_TT = 64;          // tokens of a tile
 constexpr uint32_t AD_WARPS = 8;
 constexpr uint32_t AD_MR = 64;          // rank rows of a pass
+constexpr uint32_t AD_KS = 64, AD_STAGES = 4;   // inputs of a stage, stages of the ring (more than 16 tokens)
+constexpr uint32_t AD_ROW = AD_KS * 2;          // bytes of a row of a stage
 
 __device__ __forceinline__ uint4 ad_ld16(const void* p) {
     uint4 v;
@@ -74,45 +76,63 @@ __device__ __forceinline__ void ad_st_cluster(uint32_t addr, uint32_t v) { asm v
 
 struct AdSmem {                          // dynamic shared memory, byte offsets
     // rp: rank rows that a pass writes; pitch: bytes of a token's parts, 64 modulo 128 (rows on other banks)
-    uint32_t part, u_hi, u_lo, bytes, r16, rp, pitch;
+    uint32_t part, u_hi, u_lo, bytes, r16, rp, pitch, stage;
 };
-__host__ __device__ inline AdSmem ad_smem(uint32_t R) {
+__host__ __device__ inline AdSmem ad_smem(uint32_t R, uint32_t tokens) {
     AdSmem s;
     s.r16 = (R + 15) / 16 * 16;
     s.rp = R <= 16 ? 16 : R <= 32 ? 32 : AD_MR;
     s.pitch = (R + 31) / 32 * 64;
     if (s.pitch % 128 == 0) s.pitch += 64;
-    // the warps' sums, and later, when these have been added, the 16-bit parts
+    // one after the other: the ring of operands, the warps' sums, the 16-bit parts
     s.u_hi = 0;
     s.u_lo = AD_TT * s.pitch;
-    const uint32_t warps = AD_WARPS * s.rp * 16 * 4;
+    s.stage = (AD_TT + s.rp) * AD_ROW;
+    const uint32_t warps = AD_WARPS * 16 * (s.rp + 4) * 4, ring = tokens > 16 ? AD_STAGES * s.stage : 0;
     s.part = 2 * s.u_lo > warps ? 2 * s.u_lo : warps;
+    if (ring > s.part) s.part = ring;
     s.bytes = s.part + s.r16 * AD_TT * 4;
     return s;
 }
 
+// The sums of a warp, one token's rank rows side by side, rows of rp + 4 floats: a fragment's stores and the reads along the rank meet no bank twice
+template <int MT, int NT>
+__device__ __forceinline__ void ad_put_sums(const float (&acc)[MT][NT][4], float* out, uint32_t rp, uint32_t m0) {
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[(n * 8 + 2 * t + (e & 1)) * (rp + 4) + (m0 + m) * 16 + g + (e >> 1) * 8] = acc[m][n][e];
+}
+
 // One warp's share of the inner products of MT x 16 rank rows from r0 on and NT x 8 tokens: k blocks of 32 from kb on, every `step`-th.
-// The next block's operands are asked for before a block's products run.
+// The next block's operands are asked for before a block's products run.  Rows behind the last token, and rank rows behind the last, read the
+// first: what their products are is not looked at.
 template <class T, int MT, int NT>
 __device__ __forceinline__ void ad_inner(const AdaptersArgs& a, const T* A, uint32_t R, uint32_t r0, const uint32_t* rows, uint32_t n_rows, uint32_t t0,
-                                         uint32_t kb, uint32_t kb_end, uint32_t step, float* out) {
+                                         uint32_t kb, uint32_t kb_end, uint32_t step, float* out, uint32_t rp) {
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     const uint4 zero = make_uint4(0, 0, 0, 0);
     float acc[MT][NT][4] = {};
-    const T* xr[NT];
+    const T *xr[NT], *ar[MT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) xr[n] = n * 8 + g < n_rows ? static_cast<const T*>(a.x) + (size_t)(t0 + rows[n * 8 + g]) * a.ld_x + t * 8 : nullptr;
-    const T* ar = A + (size_t)(r0 + g) * a.K + t * 8;
+    for (int n = 0; n < NT; ++n) xr[n] = static_cast<const T*>(a.x) + (size_t)(t0 + rows[n * 8 + g < n_rows ? n * 8 + g : 0]) * a.ld_x + t * 8;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) ar[m][h] = A + (size_t)(r0 + m * 16 + h * 8 + g < R ? r0 + m * 16 + h * 8 + g : r0) * a.K + t * 8;
     struct Block { uint4 x[NT], w[MT][2]; } b0, b1;
     auto ask = [&](Block& b, uint32_t at) {
         const uint32_t k = at * 32;
         const bool in = at < kb_end && k + t * 8 < a.K;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) b.x[n] = xr[n] && in ? ad_ld16(xr[n] + k) : zero;
+        for (int n = 0; n < NT; ++n) b.x[n] = in ? ad_ld16(xr[n] + k) : zero;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) b.w[m][h] = r0 + m * 16 + h * 8 + g < R && in ? ad_ld16(ar + (size_t)(m * 16 + h * 8) * a.K + k) : zero;
+            for (int h = 0; h < 2; ++h) b.w[m][h] = in ? ad_ld16(ar[m][h] + k) : zero;
     };
     auto multiply = [&](const Block& b) {
 #pragma unroll
@@ -124,96 +144,216 @@ __device__ __forceinline__ void ad_inner(const AdaptersArgs& a, const T* A, uint
             }
     };
     ask(b0, kb);
+#pragma unroll 1
     for (; kb < kb_end; kb += 2 * step) {
         ask(b1, kb + step);
         multiply(b0);
         ask(b0, kb + 2 * step);
         multiply(b1);
     }
+    ad_put_sums<MT, NT>(acc, out, rp, 0);
+}
+
+__device__ __forceinline__ void ad_copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ uint4 ad_lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// 17 .. 64 tokens: the rows of x and A go through a ring of stages of 64 inputs in shared memory (fragment loads straight from memory keep too few
+// bytes in flight: 2 TB/s over the GPU).  In a stage 16-byte chunk c of row r lies at c ^ (4 (r odd)): the eight lanes of a load phase (two rows,
+// four chunks) meet no bank twice.  A warp takes 16 NH tokens from row n0 on, block kq of the stage's two blocks of 32 inputs, and MT of the pass'
+// m-tiles from m0 on.  Rows that were not copied give products that are not looked at.
+template <class T, int MT, int NT>
+__device__ __forceinline__ void ad_inner_ring(const AdaptersArgs& a, const AdSmem& L, const T* A, uint32_t r0, uint32_t rr, const uint32_t* rows,
+                                              uint32_t n_rows, uint32_t t0, uint32_t k0, uint32_t k1, uint32_t smem, uint32_t n0, uint32_t kq, uint32_t m0,
+                                              float* out) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t n_st = (k1 - k0 + AD_KS - 1) / AD_KS, chunk = tid & 7u, row0 = tid >> 3;      // eight threads to a row, 32 rows at a time
+    const uint32_t a_at = AD_TT * AD_ROW, to0 = smem + row0 * AD_ROW + ((chunk ^ ((row0 & 1u) << 2)) << 4);
+    const T *xs[2], *as[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t r = row0 + i * 32;
+        xs[i] = r < n_rows ? static_cast<const T*>(a.x) + (size_t)(t0 + rows[r]) * a.ld_x + k0 + chunk * 8 : nullptr;
+        as[i] = r < rr ? A + (size_t)(r0 + r) * a.K + k0 + chunk * 8 : nullptr;
+    }
+    float acc[MT][NT][4] = {};
+    uint32_t ask_slot = 0, ask_st = 0;
+    auto ask = [&]() {
+        if (ask_st < n_st) {
+            const uint32_t to = to0 + ask_slot * L.stage, k = ask_st * AD_KS;
+            const bool in = k0 + k + chunk * 8 < k1;          // else: zeros, from the row's first bytes
+            const uint32_t from = in ? k : 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+                if (xs[i]) ad_copy16(to + i * 32 * AD_ROW, (in ? xs[i] : xs[i] - chunk * 8) + from, in);
+                if (as[i]) ad_copy16(to + a_at + i * 32 * AD_ROW, (in ? as[i] : as[i] - chunk * 8) + from, in);
+            }
+        }
+        ask_slot = ask_slot + 1 == AD_STAGES ? 0 : ask_slot + 1;
+        ++ask_st;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (uint32_t st = 0; st + 1 < AD_STAGES; ++st) ask();
+    const uint32_t frag = smem + g * AD_ROW + (((kq * 4 + t) ^ ((g & 1u) << 2)) << 4);     // rows g and g + 8 have the same parity
+    const uint32_t x_frag = frag + n0 * AD_ROW, a_frag = frag + a_at + m0 * 16 * AD_ROW;
+    uint32_t slot = 0;
+#pragma unroll 1
+    for (uint32_t st = 0; st < n_st; ++st) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(AD_STAGES - 2) : "memory");
+        __syncthreads();
+        ask();
+        const uint32_t xa = x_frag + slot * L.stage, aa = a_frag + slot * L.stage;
+        slot = slot + 1 == AD_STAGES ? 0 : slot + 1;
+        uint4 x[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) x[n] = ad_lds16(xa + n * 8 * AD_ROW);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const uint4 lo = ad_lds16(aa + m * 16 * AD_ROW), hi = ad_lds16(aa + (m * 16 + 8) * AD_ROW);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                ad_mma<T>(acc[m][n], lo.x, hi.x, lo.y, hi.y, x[n].x, x[n].y);
+                ad_mma<T>(acc[m][n], lo.z, hi.z, lo.w, hi.w, x[n].z, x[n].w);
+            }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                                     // the warps' sums lie where the ring was
+    ad_put_sums<MT, NT>(acc, out, L.rp, m0);
+}
+
+// two 16-bit values to f32
+__device__ __forceinline__ float2 ad_unpack(uint32_t v, __nv_bfloat16) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
+__device__ __forceinline__ float2 ad_unpack(uint32_t v, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ uint32_t ad_pack(float x, float y, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t ad_pack(float x, float y, __half) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Up to MT x 16 tokens times the outputs of blocks of 32 from fb on, every eighth block.  Column c of product j stands for output
+// (c / 2) 8 + 2 j + c % 2 of the block, so that a lane ends up with eight consecutive outputs of a token.  The next 32 rank columns of B are
+// asked for before a product, 16-bit bases a block ahead.  The parts' rows behind the last token hold anything, those of rank columns behind
+// the last hold zeros.
+template <class T, class O, int MT>
+__device__ __forceinline__ void ad_outer(const AdaptersArgs& a, const T* B, uint32_t R, uint32_t fb, uint32_t fb_end, const uint32_t* rows, uint32_t n_rows,
+                                         uint32_t t0, uint32_t u_hi, uint32_t u_lo, uint32_t pitch, const float* row_scale) {
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    constexpr int V = sizeof(O) / 2;                      // 16-byte words of eight outputs
+    constexpr bool AHEAD = sizeof(O) == 2;
+    if (fb >= fb_end) return;
+    O* y[MT][2];
+    const O* base[MT][2];
+    float scale[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float* o = out + (m * 16 + g) * 16 + n * 8 + 2 * t;
-            *reinterpret_cast<float2*>(o) = make_float2(acc[m][n][0], acc[m][n][1]);
-            *reinterpret_cast<float2*>(o + 8 * 16) = make_float2(acc[m][n][2], acc[m][n][3]);
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t i = m * 16 + h * 8 + g;
+            y[m][h] = nullptr; base[m][h] = nullptr; scale[m][h] = 1.f;
+            if (i < n_rows) {
+                const size_t row = t0 + rows[i];
+                y[m][h] = static_cast<O*>(a.y) + row * a.ld_y + t * 8;
+                if (a.base) base[m][h] = static_cast<const O*>(a.base) + row * a.ld_base + t * 8;
+                if (std::is_same<T, __half>::value) scale[m][h] = row_scale[i];
+            }
         }
-}
-
-// MT x 16 tokens times 32 outputs from f0 on.  Column c of product j stands for output (c / 2) 8 + 2 j + c % 2, so that a lane ends up
-// with eight consecutive outputs of a token.  base, and the next 32 rank columns of B, are asked for ahead.
-template <class T, class O, int MT>
-__device__ __forceinline__ void ad_outer(const AdaptersArgs& a, const T* B, uint32_t R, uint32_t f0, const uint32_t* rows, uint32_t n_rows, uint32_t t0,
-                                         uint32_t u_hi, uint32_t u_lo, uint32_t pitch, const float* row_scale) {
-    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, f = f0 + t * 8;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    constexpr int V = sizeof(O) / 2;                      // 16-byte words of eight outputs
-    float acc[MT][4][4] = {};
-    uint4 bv[2][4], base[MT][2][V];
-    auto ask = [&](uint4 (&b)[4], uint32_t k) {
-        const int left = (int)R - (int)(k + t * 8);       // of this lane's eight rank rows, those that count
+    const uint32_t u0 = u_hi + g * pitch + t * 16, k_end = (R + 31) / 32 * 32;
+    uint4 bv[2][4], bs[MT][2][V];
+    auto ask = [&](uint4 (&b)[4], uint32_t block, uint32_t k) {
+        // outputs behind the last read the last one's row (their products go nowhere), rank columns behind the last are zeros
+        const int left = (int)R - (int)(k + t * 8);
+        const bool in = block < fb_end && left > 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t o = f0 + (g >> 1) * 8 + 2 * j + (g & 1u);
-            b[j] = o < a.N && left > 0 ? ad_ld16(B + (size_t)o * a.R + k + t * 8) : zero;
+            const uint32_t o = block * 32 + (g >> 1) * 8 + 2 * j + (g & 1u);
+            b[j] = in ? ad_ld16(B + (size_t)(o < a.N ? o : a.N - 1) * a.R + k + t * 8) : zero;
         }
-    };
-    auto multiply = [&](const uint4 (&b)[4], uint32_t k) {
-        const int left = (int)R - (int)(k + t * 8);
-        uint4 w[4];
+        if (in && left < 8)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = left >= 8 ? b[j] : ad_first(b[j], left);
+            for (int j = 0; j < 4; ++j) b[j] = ad_first(b[j], left);
+    };
+    auto ask_base = [&](uint4 (&to)[MT][2][V], uint32_t block) {
+        const bool in = block < fb_end && block * 32 + t * 8 < a.N;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-                const uint32_t at = (part ? u_lo : u_hi) + (m * 16 + g) * pitch + k * 2 + t * 16;
-                uint4 lo = zero, hi = zero;
-                if (left > 0 && m * 16 + g < n_rows) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w) : "r"(at));
-                if (left > 0 && m * 16 + g + 8 < n_rows) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w) : "r"(at + 8 * pitch));
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    ad_mma<T>(acc[m][j], lo.x, hi.x, lo.y, hi.y, w[j].x, w[j].y);
-                    ad_mma<T>(acc[m][j], lo.z, hi.z, lo.w, hi.w, w[j].z, w[j].w);
-                }
-            }
+                for (int v = 0; v < V; ++v)    // plain loads: in place, y's own rows are read here
+                    to[m][h][v] = in && base[m][h] ? *reinterpret_cast<const uint4*>(base[m][h] + block * 32 + v * (8 / V)) : zero;
     };
-    ask(bv[0], 0);
+    ask(bv[0], fb, 0);
+    if (AHEAD) ask_base(bs, fb);
+#pragma unroll 1
+    for (; fb < fb_end; fb += AD_WARPS) {
+        float acc[MT][4][4] = {};
+        auto multiply = [&](const uint4 (&b)[4], uint32_t k) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+            for (int part = 0; part < 2; ++part)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t i = m * 16 + h * 8 + g;
+                for (int m = 0; m < MT; ++m) {
+                    const uint32_t at = u0 + (part ? u_lo - u_hi : 0) + m * 16 * pitch + k * 2;
+                    const uint4 lo = ad_lds16(at), hi = ad_lds16(at + 8 * pitch);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                base[m][h][v] = zero;
-                // plain loads: in place, y's own rows are read here
-                if (a.base && i < n_rows && f < a.N)
-                    base[m][h][v] = *reinterpret_cast<const uint4*>(static_cast<const O*>(a.base) + (size_t)(t0 + rows[i]) * a.ld_base + f + v * (8 / V));
+                    for (int j = 0; j < 4; ++j) {
+                        ad_mma<T>(acc[m][j], lo.x, hi.x, lo.y, hi.y, b[j].x, b[j].y);
+                        ad_mma<T>(acc[m][j], lo.z, hi.z, lo.w, hi.w, b[j].z, b[j].w);
+                    }
+                }
+        };
+        if (!AHEAD) ask_base(bs, fb);
+#pragma unroll 1
+        for (uint32_t k = 0; k < k_end; k += 64) {
+            const bool more = k + 32 < k_end;
+            ask(bv[1], more ? fb : fb + AD_WARPS, more ? k + 32 : 0);
+            multiply(bv[0], k);
+            if (more) {
+                const bool last = k + 64 >= k_end;
+                ask(bv[0], last ? fb + AD_WARPS : fb, last ? 0 : k + 64);
+                multiply(bv[1], k + 32);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) bv[0][j] = bv[1][j];
             }
         }
-    for (uint32_t k = 0; k < R; k += 64) {
-        ask(bv[1], k + 32);
-        multiply(bv[0], k);
-        ask(bv[0], k + 64);
-        if (k + 32 < R) multiply(bv[1], k + 32);
-    }
-    if (f >= a.N) return;
+        if (fb * 32 + t * 8 < a.N) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t i = m * 16 + h * 8 + g;
-            if (i >= n_rows) continue;
-            const float s = row_scale[i];
-            O* y = static_cast<O*>(a.y) + (size_t)(t0 + rows[i]) * a.ld_y + f;
-            const O* b = reinterpret_cast<const O*>(base[m][h]);
-            O o[8];
+                for (int h = 0; h < 2; ++h) {
+                    if (!y[m][h]) continue;
+                    const float s = scale[m][h];
+                    if constexpr (sizeof(O) == 4) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) ad_round(fmaf(acc[m][c >> 1][2 * h + (c & 1)], s, ad_f32(b[c])), o[c]);
+                        for (int v = 0; v < 2; ++v) {
+                            const uint4 b = bs[m][h][v];
+                            *reinterpret_cast<float4*>(y[m][h] + fb * 32 + v * 4) =
+                                make_float4(fmaf(acc[m][2 * v][2 * h], s, __uint_as_float(b.x)), fmaf(acc[m][2 * v][2 * h + 1], s, __uint_as_float(b.y)),
+                                            fmaf(acc[m][2 * v + 1][2 * h], s, __uint_as_float(b.z)), fmaf(acc[m][2 * v + 1][2 * h + 1], s, __uint_as_float(b.w)));
+                        }
+                    } else {
+                        const uint32_t b[4] = {bs[m][h][0].x, bs[m][h][0].y, bs[m][h][0].z, bs[m][h][0].w};
+                        uint32_t o[4];
 #pragma unroll
-            for (int v = 0; v < V; ++v) reinterpret_cast<uint4*>(y)[v] = reinterpret_cast<const uint4*>(o)[v];
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 f = ad_unpack(b[j], O());
+                            o[j] = ad_pack(fmaf(acc[m][j][2 * h], s, f.x), fmaf(acc[m][j][2 * h + 1], s, f.y), O());
+                        }
+                        *reinterpret_cast<uint4*>(y[m][h] + fb * 32) = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                }
         }
+        if (AHEAD) ask_base(bs, fb + AD_WARPS);
+    }
 }
 
 struct AdShared {
@@ -240,8 +380,7 @@ __device__ __forceinline__ void ad_copy(const AdaptersArgs& a, const uint32_t* r
     }
 }
 
-// One adapter's n_rows <= 16 n_q tokens t0 + sh.rows[..], by the whole cluster: the warps split the tokens n_q = 1, 2 or 4 ways (sixteen each)
-// and the inputs 8 / n_q ways.
+// One adapter's n_rows <= 16 n_q tokens t0 + sh.rows[..], by the whole cluster, n_q = 1, 2 or 4.
 template <class T, class O>
 __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, uint8_t* smem, AdShared& sh, uint32_t C, uint32_t rank, int32_t id,
                                         uint32_t n_rows, uint32_t n_q, uint32_t t0) {
@@ -256,29 +395,45 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
     const T* B = static_cast<const T*>(a.b) + (size_t)id * a.b_stride;
 
     // ---- inner product: this CTA's inputs ----
-    const uint32_t n_split = 8 / n_q, q = warp / n_split, kb = kb0 + warp % n_split;
-    const uint32_t q_rows = n_rows > q * 16 ? min(n_rows - q * 16, 16u) : 0, *q_row = sh.rows + q * 16;
     for (uint32_t r0 = 0; r0 < R; r0 += AD_MR) {
         const uint32_t rr = min(R - r0, AD_MR);                      // rank rows of the pass
-        float* const mine = warp_part + warp * L.rp * 16;
-        if (q_rows <= 8) {
-            if (rr <= 16) ad_inner<T, 1, 1>(a, A, R, r0, q_row, q_rows, t0, kb, kb1, n_split, mine);
-            else if (rr <= 32) ad_inner<T, 2, 1>(a, A, R, r0, q_row, q_rows, t0, kb, kb1, n_split, mine);
-            else ad_inner<T, 4, 1>(a, A, R, r0, q_row, q_rows, t0, kb, kb1, n_split, mine);
+        uint32_t n_sums;                                             // partial sums of a value, one after the other n_next floats apart
+        const uint32_t region = 16 * (L.rp + 4);                     // floats of a warp's sums
+        if (n_q == 1) {
+            float* const mine = warp_part + warp * region;
+            n_sums = AD_WARPS;
+            if (n_rows <= 8) {
+                if (rr <= 16) ad_inner<T, 1, 1>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                else if (rr <= 32) ad_inner<T, 2, 1>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                else ad_inner<T, 4, 1>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+            } else {
+                if (rr <= 16) ad_inner<T, 1, 2>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                else if (rr <= 32) ad_inner<T, 2, 2>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                else ad_inner<T, 4, 2>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+            }
         } else {
-            if (rr <= 16) ad_inner<T, 1, 2>(a, A, R, r0, q_row, q_rows, t0, kb, kb1, n_split, mine);
-            else if (rr <= 32) ad_inner<T, 2, 2>(a, A, R, r0, q_row, q_rows, t0, kb, kb1, n_split, mine);
-            else ad_inner<T, 4, 2>(a, A, R, r0, q_row, q_rows, t0, kb, kb1, n_split, mine);
+            // warp = (tokens, inputs, m-tiles): 4 x 2 x 1, or 2 x 2 x 2 (where there is one m-tile, both halves take it)
+            const uint32_t q = n_q == 4 ? warp >> 1 : warp >> 2, kq = warp & 1u, mh = warp >> 1 & 1u, k_end = min(kb1 * 32, a.K);
+            float* const mine = warp_part + (q * 2 + kq) * region;
+            n_sums = 2;
+            if (n_q == 4) {
+                if (L.rp == 16) ad_inner_ring<T, 1, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, 0, mine);
+                else if (L.rp == 32) ad_inner_ring<T, 2, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, 0, mine);
+                else ad_inner_ring<T, 4, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, 0, mine);
+            } else {
+                if (L.rp <= 32) ad_inner_ring<T, 1, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, L.rp == 16 ? 0 : mh, mine);
+                else ad_inner_ring<T, 2, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, mh * 2, mine);
+            }
         }
         __syncthreads();
-        // the warps' sums in order
-        for (uint32_t i = tid; i < rr * 64; i += AD_WARPS * 32) {
-            const uint32_t r = i / 64, c = i % 64;
-            if (c >= n_rows) continue;
-            const float* p = warp_part + (c / 16 * n_split) * L.rp * 16 + r * 16 + c % 16;
-            float s = p[0];
-            for (uint32_t w = 1; w < n_split; ++w) s += p[w * L.rp * 16];
-            part[c * L.r16 + r0 + r] = s;
+        // the warps' sums in order, a warp to a token
+        for (uint32_t c = warp; c < n_rows; c += AD_WARPS) {
+            const float* p = warp_part + c / 16 * n_sums * region + c % 16 * (L.rp + 4);
+            for (uint32_t r = lane; r < rr; r += 32) {
+                float s = p[r];
+                for (uint32_t w = 1; w < n_sums; ++w) s += p[w * region + r];
+                part[c * L.r16 + r0 + r] = s;
+            }
         }
         __syncthreads();
     }
@@ -313,7 +468,7 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
             const uint32_t r = j * 64 + lane * 2;
-            if (r >= a.R) continue;
+            if (r >= (R + 31) / 32 * 32) continue;                   // zeros behind the last rank column
             uint32_t hi, lo;
             ad_split<T>(v[j][0] * down, v[j][1] * down, hi, lo);
             for (uint32_t c = 0; c < C; ++c) {
@@ -326,14 +481,12 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
     }
     cluster_sync_all();
     // ---- outer product: this CTA's outputs ----
-    for (uint32_t fb = fb0 + warp; fb < fb1; fb += AD_WARPS) {
-        if (n_rows <= 16) ad_outer<T, O, 1>(a, B, R, fb * 32, sh.rows, n_rows, t0, base_s + L.u_hi, base_s + L.u_lo, L.pitch, sh.scale);
-        else if (n_rows <= 32) ad_outer<T, O, 2>(a, B, R, fb * 32, sh.rows, n_rows, t0, base_s + L.u_hi, base_s + L.u_lo, L.pitch, sh.scale);
-        else
-            for (uint32_t h = 0; h < n_rows; h += 32)
-                ad_outer<T, O, 2>(a, B, R, fb * 32, sh.rows + h, min(n_rows - h, 32u), t0, base_s + L.u_hi + h * L.pitch, base_s + L.u_lo + h * L.pitch, L.pitch,
-                                  sh.scale + h);
-    }
+    if (n_rows <= 16)
+        ad_outer<T, O, 1>(a, B, R, fb0 + warp, fb1, sh.rows, n_rows, t0, base_s + L.u_hi, base_s + L.u_lo, L.pitch, sh.scale);
+    else
+        for (uint32_t h = 0; h < n_rows; h += 32)
+            ad_outer<T, O, 2>(a, B, R, fb0 + warp, fb1, sh.rows + h, min(n_rows - h, 32u), t0, base_s + L.u_hi + h * L.pitch, base_s + L.u_lo + h * L.pitch,
+                              L.pitch, sh.scale + h);
     __syncthreads();
 }
 
@@ -349,7 +502,7 @@ template <class T, class O>
 __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const AdaptersArgs a, const uint32_t C, const uint32_t slots) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ AdShared sh;
-    const AdSmem L = ad_smem(a.R);
+    const AdSmem L = ad_smem(a.R, a.T);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = cluster_rank();
     const uint32_t unit = blockIdx.x / C, tile = unit / slots, slot = unit % slots, t0 = tile * AD_TT;
 
@@ -408,9 +561,9 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const A
     }
 }
 
-// More tokens: every CTA sorts the ids of a segment of up to 4096 tokens in its own shared memory (stable, so that all CTAs have the same order),
+// More tokens: every CTA sorts the ids of a segment of up to 2048 tokens in its own shared memory (stable, so that all CTAs have the same order),
 // then the segment's clusters take units of one adapter and up to 64 of its tokens, wherever they lie.
-constexpr uint32_t AD_SEG = 4096, AD_PLACES = 512;                   // tokens of a segment; adapters that are counted, and none
+constexpr uint32_t AD_SEG = 2048, AD_PLACES = 512;                   // tokens of a segment; adapters that are counted, and none
 struct AdSort {                          // dynamic shared memory behind AdSmem
     uint32_t first[AD_PLACES + 1];       // first token in the order (low half), first unit (high half)
     uint16_t cursor[AD_WARPS][AD_PLACES];
@@ -421,7 +574,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ AdShared sh;
     __shared__ uint32_t s_scan[AD_WARPS];
-    const AdSmem L = ad_smem(a.R);
+    const AdSmem L = ad_smem(a.R, a.T);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = cluster_rank();
     const uint32_t cl = blockIdx.x / C, seg = cl / per_seg, t0 = seg * AD_SEG, n_tok = min(AD_SEG, a.T - t0), n_places = a.n_adapters + 1;
     AdSort& so = *reinterpret_cast<AdSort*>(smem + L.bytes);
@@ -431,10 +584,20 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
     const uint32_t run_len = (n_tok + AD_WARPS * 32 - 1) / (AD_WARPS * 32) * 32, run0 = warp * run_len, run1 = min(run0 + run_len, n_tok);
     for (uint32_t i = tid; i < AD_WARPS * AD_PLACES / 2; i += AD_WARPS * 32) reinterpret_cast<uint32_t*>(so.cursor)[i] = 0;
     __syncthreads();
-    for (uint32_t i = run0; i < run1; i += 32) {
-        const bool in = i + lane < run1;
-        const uint32_t place = in ? ad_place(a, t0 + i + lane, cl % per_seg == 0 && rank == 0) : 0xFFFFFFFFu, same = __match_any_sync(0xFFFFFFFFu, place);
-        if (in && (same & ((1u << lane) - 1)) == 0) so.cursor[warp][place] += (uint16_t)__popc(same);
+    // a token's place, and its number among the run's tokens of that place (the operands' memory is free here)
+    uint16_t* const place_of = reinterpret_cast<uint16_t*>(smem);
+    uint16_t* const number_of = place_of + AD_SEG;
+#pragma unroll 4
+    for (uint32_t i = run0 + lane; i < run1; i += 32) place_of[i] = (uint16_t)ad_place(a, t0 + i, cl % per_seg == 0 && rank == 0);
+    __syncwarp();
+#pragma unroll 1
+    for (uint32_t i = run0 + lane; i < run0 + run_len && i - lane < run1; i += 32) {
+        const bool in = i < run1;
+        const uint32_t place = in ? place_of[i] : 0xFFFFu, same = __match_any_sync(0xFFFFFFFFu, place), before = __popc(same & ((1u << lane) - 1));
+        const uint32_t at = in ? so.cursor[warp][place] : 0;
+        __syncwarp();
+        if (in) number_of[i] = (uint16_t)(at + before);
+        if (in && before == 0) so.cursor[warp][place] = (uint16_t)(at + __popc(same));
         __syncwarp();
     }
     __syncthreads();
@@ -470,16 +633,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
         }
     }
     __syncthreads();
-    for (uint32_t i = run0; i < run1; i += 32) {
-        const bool in = i + lane < run1;
-        const uint32_t place = in ? ad_place(a, t0 + i + lane, false) : 0xFFFFFFFFu, same = __match_any_sync(0xFFFFFFFFu, place);
-        const uint32_t before = __popc(same & ((1u << lane) - 1));
-        const uint32_t at = in ? so.cursor[warp][place] : 0;
-        __syncwarp();
-        if (in) so.order[at + before] = (uint16_t)(i + lane);
-        if (in && before == 0) so.cursor[warp][place] = (uint16_t)(at + __popc(same));
-        __syncwarp();
-    }
+    for (uint32_t i = run0 + lane; i < run1; i += 32) so.order[so.cursor[warp][place_of[i]] + number_of[i]] = (uint16_t)i;
     __syncthreads();
     const uint32_t n_units = first[n_places] >> 16;
     for (uint32_t u = cl % per_seg; u < n_units; u += per_seg) {
@@ -515,7 +669,7 @@ static cudaError_t ad_launch(void (*kernel)(Params...), uint32_t C, uint32_t clu
 }
 template <class T, class O>
 static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
-    const AdSmem L = ad_smem(a.R);
+    const AdSmem L = ad_smem(a.R, a.T);
     const uint32_t room = 2 * (uint32_t)a.sm_count;                // CTAs that run at once
     if (a.T <= AD_TT || a.n_adapters >= AD_PLACES) {
         const uint32_t tiles = (a.T + AD_TT - 1) / AD_TT, most = a.T < a.n_adapters ? a.T : a.n_adapters, distinct = most < AD_TT ? most : AD_TT;
