@@ -27,6 +27,200 @@ __device__ __forceinline__ bool gp_range(const GroupedArgs& a, uint32_t g, uint3
 }
 
 // ------------------------------------------------------------------------------------------------------------
+// few rows
+// ------------------------------------------------------------------------------------------------------------
+// Calls of up to 16 rows (a token's or two tokens' experts): the weights' bytes are everything, and tiles of 512 outputs would leave most SMs
+// without work.  A CTA takes 32 rows of a group's matrix (inputs first: 64) and all the group's rows; its eight warps split the inputs and stream
+// the weights from memory straight into mma fragments, 16 bytes per lane, four blocks ahead.  The warps' sums meet in shared memory, in order.
+constexpr uint32_t GN_ROWS = 16, GN_WARPS = 8, GN_AHEAD = 4;
+
+__device__ __forceinline__ uint4 gn_stream16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 gn_ld16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 gn_ld8(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+template <bool BF16>
+__device__ __forceinline__ void gn_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    const uint32_t a[4] = {a0, a1, a2, a3};
+    if (BF16) mma_bf16(d, a, b0, b1);
+    else mma_f16(d, a, b0, b1);
+}
+
+// Outputs first.  W row r of the CTA's 32 (r < 16: m-tile 0) is w + row_of(r) ld_w.  A lane's eight consecutive inputs stand for the k positions 2t,
+// 2t+1, 2t+8, 2t+9 of two products, the same for both operands.
+template <bool BF16, int NT, class RowOf>
+__device__ __forceinline__ void gn_out_in(const GroupedArgs& a, const uint16_t* w, RowOf row_of, const uint32_t* xrow, uint32_t n_rows, float* out) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const uint16_t *wp[4], *xp[NT];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) wp[r] = w + (size_t)row_of(r * 8 + g) * a.ld_w + t * 8;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) xp[n] = static_cast<const uint16_t*>(a.x) + (size_t)xrow[n * 8 + g < n_rows ? n * 8 + g : 0] * a.ld_x + t * 8;
+    float acc[2][NT][4] = {};
+    struct Block { uint4 w[4], x[NT]; } b[GN_AHEAD];
+    const uint32_t n_kb = (a.K + 31) / 32;
+    auto ask = [&](Block& to, uint32_t kb) {
+        const bool in = kb < n_kb && kb * 32 + t * 8 < a.K;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to.w[r] = in ? gn_stream16(wp[r] + kb * 32) : zero;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) to.x[n] = in ? gn_ld16(xp[n] + kb * 32) : zero;
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < GN_AHEAD; ++i) ask(b[i], warp + i * GN_WARPS);
+#pragma unroll 1
+    for (uint32_t kb = warp; kb < n_kb; kb += GN_AHEAD * GN_WARPS) {
+#pragma unroll
+        for (uint32_t i = 0; i < GN_AHEAD; ++i) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint4 lo = b[i].w[2 * m], hi = b[i].w[2 * m + 1], x = b[i].x[n];
+                    gn_mma<BF16>(acc[m][n], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+                    gn_mma<BF16>(acc[m][n], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+                }
+            ask(b[i], kb + (GN_AHEAD + i) * GN_WARPS);
+        }
+    }
+    // [row of W][row of x], eight columns to a fragment
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<float2*>(out + (m * 16 + h * 8 + g) * GN_ROWS + n * 8 + 2 * t) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
+}
+
+// Inputs first: a lane takes eight outputs (lane / 4) of the inputs 4t .. 4t + 3 of a block of 16, which stand for the k positions 2t, 2t+1, 2t+8,
+// 2t+9; two inputs' words are permuted into pairs along k.  Row i of m-tile j is output (i % 8) 8 + 2 j + i / 8.
+template <bool BF16, int NT>
+__device__ __forceinline__ void gn_in_out(const GroupedArgs& a, const uint16_t* w8, const uint32_t* xrow, uint32_t n_rows, float* out) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const uint16_t* xp[NT];
+    w8 += (size_t)(t * 4) * a.ld_w;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) xp[n] = static_cast<const uint16_t*>(a.x) + (size_t)xrow[n * 8 + g < n_rows ? n * 8 + g : 0] * a.ld_x + t * 4;
+    float acc[4][NT][4] = {};
+    struct Block { uint4 w[4]; uint2 x[NT]; } b[GN_AHEAD];
+    const uint32_t n_kb = (a.K + 15) / 16;
+    auto ask = [&](Block& to, uint32_t kb) {
+        const bool in = kb < n_kb && kb * 16 + t * 4 < a.K;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to.w[r] = in ? gn_stream16(w8 + (size_t)(kb * 16 + r) * a.ld_w) : zero;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) to.x[n] = in ? gn_ld8(xp[n] + kb * 16) : make_uint2(0, 0);
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < GN_AHEAD; ++i) ask(b[i], warp + i * GN_WARPS);
+#pragma unroll 1
+    for (uint32_t kb = warp; kb < n_kb; kb += GN_AHEAD * GN_WARPS) {
+#pragma unroll
+        for (uint32_t i = 0; i < GN_AHEAD; ++i) {
+            const uint32_t r0[4] = {b[i].w[0].x, b[i].w[0].y, b[i].w[0].z, b[i].w[0].w}, r1[4] = {b[i].w[1].x, b[i].w[1].y, b[i].w[1].z, b[i].w[1].w};
+            const uint32_t r2[4] = {b[i].w[2].x, b[i].w[2].y, b[i].w[2].z, b[i].w[2].w}, r3[4] = {b[i].w[3].x, b[i].w[3].y, b[i].w[3].z, b[i].w[3].w};
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    gn_mma<BF16>(acc[m][n], __byte_perm(r0[m], r1[m], 0x5410), __byte_perm(r0[m], r1[m], 0x7632), __byte_perm(r2[m], r3[m], 0x5410),
+                                 __byte_perm(r2[m], r3[m], 0x7632), b[i].x[n].x, b[i].x[n].y);
+            ask(b[i], kb + (GN_AHEAD + i) * GN_WARPS);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *reinterpret_cast<float2*>(out + (g * 8 + 2 * m + h) * GN_ROWS + n * 8 + 2 * t) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
+}
+
+__device__ __forceinline__ void gn_put(float v, __nv_bfloat16* o) { *o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void gn_put(float v, __half* o) { *o = __float2half_rn(v); }
+__device__ __forceinline__ void gn_put(float v, float* o) { *o = v; }
+
+template <bool BF16, bool IN_OUT, bool SWIGLU, class O>
+__global__ void __launch_bounds__(GN_WARPS * 32, 2) grouped_few_kernel(const GroupedArgs a) {
+    constexpr uint32_t W_ROWS = IN_OUT ? 64 : 32, OUTS = SWIGLU ? W_ROWS / 2 : W_ROWS;
+    __shared__ __align__(16) float sums[GN_WARPS][W_ROWS * GN_ROWS];
+    __shared__ uint32_t s_xrow[GN_ROWS], s_yrow[GN_ROWS], s_group;
+    const uint32_t tid = threadIdx.x, p0 = blockIdx.y, f0 = blockIdx.x * OUTS;
+    // the group whose rows begin at p0, if one does
+    if (tid == 0) s_group = 0xFFFFFFFFu;
+    __syncthreads();
+    for (uint32_t g = tid; g < a.G; g += GN_WARPS * 32) {
+        uint32_t r0, r1;
+        const bool ok = gp_range(a, g, r0, r1);
+        if (!ok && blockIdx.x == 0 && p0 == 0) atomicMax(a.status, ST_BAD_OFFSETS);
+        if (r0 == p0 && r1 > p0) atomicMin(&s_group, g);
+    }
+    __syncthreads();
+    const uint32_t g = s_group;
+    if (g == 0xFFFFFFFFu) return;
+    uint32_t r0, r1;
+    gp_range(a, g, r0, r1);
+    const uint32_t n_rows = r1 - r0;                                  // at most the call's rows: 16
+    if (tid < n_rows) {
+        const uint32_t p = p0 + tid, o = a.order ? a.order[p] : p;
+        uint32_t xr = a.gather ? o / a.x_div : p, yr = a.scatter ? o : p;
+        if (xr >= a.x_rows || yr >= a.y_rows) { xr = 0; yr = 0xFFFFFFFFu; atomicMax(a.status, ST_BAD_ROW); }
+        s_xrow[tid] = xr; s_yrow[tid] = yr;
+    }
+    __syncthreads();
+    const uint16_t* w = static_cast<const uint16_t*>(a.w) + (size_t)g * a.w_stride;
+    float* const mine = sums[tid >> 5];
+    if (IN_OUT) {
+        // this lane's eight outputs; behind the last: the last eight
+        const uint32_t lane8 = (tid & 31u) >> 2, f = f0 + (SWIGLU ? lane8 % 4 : lane8) * 8;
+        const uint16_t* w8 = w + (SWIGLU && lane8 >= 4 ? a.N : 0) + (f < a.N ? f : a.N - 8);
+        if (n_rows <= 8) gn_in_out<BF16, 1>(a, w8, s_xrow, n_rows, mine);
+        else gn_in_out<BF16, 2>(a, w8, s_xrow, n_rows, mine);
+    } else {
+        const auto row_of = [&](uint32_t r) {
+            const uint32_t f = f0 + (SWIGLU ? r % 16 : r), c = f < a.N ? f : a.N - 1;
+            return SWIGLU && r >= 16 ? a.N + c : c;
+        };
+        if (n_rows <= 8) gn_out_in<BF16, 1>(a, w, row_of, s_xrow, n_rows, mine);
+        else gn_out_in<BF16, 2>(a, w, row_of, s_xrow, n_rows, mine);
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < OUTS * n_rows; i += GN_WARPS * 32) {
+        const uint32_t f = i % OUTS, r = i / OUTS;
+        float v = sums[0][f * GN_ROWS + r], u = 0.f;
+        for (uint32_t k = 1; k < GN_WARPS; ++k) v += sums[k][f * GN_ROWS + r];
+        if (SWIGLU) {
+            u = sums[0][(OUTS + f) * GN_ROWS + r];
+            for (uint32_t k = 1; k < GN_WARPS; ++k) u += sums[k][(OUTS + f) * GN_ROWS + r];
+            v = gp_swiglu<sizeof(O) == 4>(v, u, a.limit);
+        }
+        const uint32_t yr = s_yrow[r];
+        if (yr != 0xFFFFFFFFu && f0 + f < a.N) gn_put(v, static_cast<O*>(a.y) + (size_t)yr * a.ld_y + f0 + f);
+    }
+}
+
+template <bool BF16, bool IN_OUT, bool SWIGLU, class O>
+static cudaError_t few_launch(const GroupedArgs& a, cudaStream_t st) {
+    constexpr uint32_t OUTS = (IN_OUT ? 64 : 32) / (SWIGLU ? 2 : 1);
+    grouped_few_kernel<BF16, IN_OUT, SWIGLU, O><<<dim3((a.N + OUTS - 1) / OUTS, a.rows), GN_WARPS * 32, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------------------
 // tensor-core tiles
 // ------------------------------------------------------------------------------------------------------------
 constexpr uint32_t GT_KS = 64;                                   // inputs per stage: 128 bytes, one swizzle row
@@ -391,13 +585,17 @@ static cudaError_t tile_launch(const GroupedArgs& a, cudaStream_t st) {
     kernel<<<a.sm_count / 2 * 2, GT_THREADS, GT_SMEM, st>>>(P);
     return cudaGetLastError();
 }
-template <class O>
+template <bool BF16, class O>
 static cudaError_t grouped_out(const GroupedArgs& a, cudaStream_t st) {
+    if (a.rows <= GN_ROWS) {
+        if (a.in_out) return a.swiglu ? few_launch<BF16, true, true, O>(a, st) : few_launch<BF16, true, false, O>(a, st);
+        return a.swiglu ? few_launch<BF16, false, true, O>(a, st) : few_launch<BF16, false, false, O>(a, st);
+    }
     return a.swiglu ? tile_launch<true, O>(a, st) : tile_launch<false, O>(a, st);
 }
 cudaError_t launch_grouped(const GroupedArgs& a, cudaStream_t st) {
-    if (a.out_dtype == DT_F32) return grouped_out<float>(a, st);
-    return a.dtype == DT_BF16 ? grouped_out<__nv_bfloat16>(a, st) : grouped_out<__half>(a, st);
+    if (a.dtype == DT_BF16) return a.out_dtype == DT_F32 ? grouped_out<true, float>(a, st) : grouped_out<true, __nv_bfloat16>(a, st);
+    return a.out_dtype == DT_F32 ? grouped_out<false, float>(a, st) : grouped_out<false, __half>(a, st);
 }
 
 }  // namespace mlxs
