@@ -243,17 +243,25 @@ struct TileParams {
     GroupedArgs a;
     uint32_t n_ft, n_ks;          // output tiles of a row tile, stages
     uint32_t cap;                 // most rows of a tile: 128 or 256
-    uint32_t w_loads;             // copies that a stage of weights takes: 1, or 2 x 2 halves
+    uint32_t w_loads;             // copies that a stage of weights takes
     uint32_t fmt;
+    uint32_t parts;               // parts of the reduction, a CTA pair of the item's cluster to each (1: no cluster, pairs walk the items)
 };
 
 struct GtItem { uint32_t g, p0, rows, n; };   // group, first position, rows, MMA N (a multiple of 32)
 // walks the call's row tiles: tile number -> group and rows.  A group's rows are cut into as few tiles as hold them, all alike.
 struct GtWalk {
     const uint32_t *off, *tiles;   // [G][first, end], [G + 1] first row tile
-    uint32_t g = 0;
+    uint32_t G, g = 0;
     __device__ GtItem at(uint32_t tile) {
-        while (tiles[g + 1] <= tile) ++g;
+        if (tiles[g + 1] <= tile) {
+            uint32_t lo = g + 1, hi = G;                   // tiles[lo] <= tile < tiles[hi]
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (tiles[mid] <= tile) lo = mid; else hi = mid;
+            }
+            g = lo;
+        }
         const uint32_t r0 = off[2 * g], len = off[2 * g + 1] - r0, nt = tiles[g + 1] - tiles[g];
         const uint32_t per = ((len + nt - 1) / nt + 31) / 32 * 32, i = tile - tiles[g];
         GtItem it;
@@ -281,6 +289,11 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ float4 ld_cluster16(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -291,13 +304,16 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
 }
 
 template <bool SWIGLU, class O>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __grid_constant__ TileParams P) {
+__global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __grid_constant__ TileParams P) {
     extern __shared__ uint8_t smem_any[];
     __shared__ __align__(8) uint64_t full_bar[GT_STAGES], empty_bar[GT_STAGES], acc_full[2], acc_empty[2];
     __shared__ uint32_t s_tmem, s_off[2 * GT_MAX_G], s_tiles[GT_MAX_G + 1], s_row[GT_GATHER_WARPS][128];
     __shared__ volatile int s_abort;
     const GroupedArgs& a = P.a;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, rank = cluster_rank();
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    // the pair's even CTA leads; in a cluster of several pairs each takes a part of the reduction
+    const uint32_t cl_rank = cluster_rank(), rank = cl_rank & 1u, leader = cl_rank & ~1u, part = cl_rank >> 1;
+    const uint16_t pair_mask = (uint16_t)(3u << leader);
     const uint32_t ring = (smem_u32(smem_any) + 1023u) & ~1023u;
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < GT_STAGES; ++s) { mbar_init(&full_bar[s], a.gather ? 3 : 1); mbar_init(&empty_bar[s], 1); }
@@ -328,12 +344,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) group
     tc_fence_before();
     cluster_sync_all();
     tc_fence_after();
-    const uint32_t tmem = s_tmem, n_items = s_tiles[a.G] * P.n_ft, n_pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+    const uint32_t tmem = s_tmem, n_items = s_tiles[a.G] * P.n_ft, pair = blockIdx.x / (2 * P.parts);
+    // pairs walk the items; a cluster of several pairs takes one
+    const uint32_t n_pairs = P.parts == 1 ? gridDim.x / 2 : max(n_items, 1u);
+    const uint32_t ks0 = part * P.n_ks / P.parts, ks1 = (part + 1) * P.n_ks / P.parts;
     constexpr uint32_t FT = SWIGLU ? 256 : 512;                  // outputs of an item: half of them this CTA's
     // tensor memory: buffers of two accumulators of `cap` columns
     const uint32_t n_buf = 256 / P.cap;
     auto give_up = [&](uint32_t code) { if (!s_abort) atomicMax(a.status, code); s_abort = 1; };
-    GtWalk walk{s_off, s_tiles};
+    GtWalk walk{s_off, s_tiles, a.G};
 
     if (warp == 0) {
         // ---------------- producer: this CTA's outputs' weights, and its half of the tile's rows where they lie in order ----------------
@@ -345,10 +364,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) group
             const int32_t f0 = (int32_t)((i % P.n_ft) * FT + rank * (FT / 2)), g = (int32_t)it.g;
             const uint32_t hb = it.n / 2, b0 = it.p0 + rank * hb, bi = hb <= 16 ? 0 : hb <= 32 ? 1 : (hb + 31) / 32;
             const uint32_t bytes = 2 * (GT_A_BYTES + (gather ? 0 : gt_box_rows(bi) * GT_KS * 2));   // both CTAs' copies
-            for (uint32_t ks = 0; ks < P.n_ks; ++ks) {
+            for (uint32_t ks = ks0; ks < ks1; ++ks) {
                 if (!mbar_wait_warp_at(smem_u32(&empty_bar[s]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
                 if (lane == 0) {
-                    const uint32_t full = map_to_rank(smem_u32(&full_bar[s]), 0), sa = ring + s * GT_STAGE;
+                    const uint32_t full = map_to_rank(smem_u32(&full_bar[s]), leader), sa = ring + s * GT_STAGE;
                     const int32_t k = (int32_t)(ks * GT_KS);
                     if (rank == 0) mbar_expect_tx(&full_bar[s], bytes);
                     if (!a.in_out) {
@@ -385,7 +404,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) group
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_empty[buf]), (n_done / n_buf & 1u) ^ 1u, &s_abort));
                 if (!ok) { give_up(ST_WAIT_EMPTY); break; }
                 tc_fence_after();
-                for (uint32_t ks = 0; ks < P.n_ks; ++ks) {
+                for (uint32_t ks = ks0; ks < ks1; ++ks) {
                     ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&full_bar[s]), ph, &s_abort));
                     if (!ok) { give_up(ST_WAIT_FULL); break; }
                     tc_fence_after();
@@ -396,14 +415,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) group
 #pragma unroll
                             for (uint32_t j = 0; j < GT_KS / 16; ++j)
                                 umma_f16_pair(acc + h * P.cap, umma_desc_sw128(sa + h * a_next + j * a_step, a_lbo, 1024),
-                                              umma_desc_sw128(sb + j * 32, 16, 1024), idesc, ks | j ? 1u : 0u);
-                        umma_commit_pair(smem_u32(&empty_bar[s]), 3);
+                                              umma_desc_sw128(sb + j * 32, 16, 1024), idesc, ks != ks0 || j ? 1u : 0u);
+                        umma_commit_pair(smem_u32(&empty_bar[s]), pair_mask);
                     }
                     __syncwarp();
                     if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
                 }
                 if (!ok) break;
-                if (elect_one()) umma_commit_pair(smem_u32(&acc_full[buf]), 3);
+                if (elect_one()) umma_commit_pair(smem_u32(&acc_full[buf]), pair_mask);
                 __syncwarp();
                 ++n_done;
             }
@@ -419,6 +438,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) group
             const uint32_t buf = n_done % n_buf, f = (i % P.n_ft) * FT + rank * (FT / 2) + q * 32 + lane;
             if (!__all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_full[buf]), n_done / n_buf & 1u, &s_abort))) { give_up(ST_WAIT_FULL); break; }
             tc_fence_after();
+            if (P.parts > 1) {
+                // a part's sums, where the ring was (its copies have landed, the products have read them): [accumulator][row][128 outputs]
+                for (uint32_t c = half * 16; c < it.rows; c += 32) {
+                    uint32_t v0[16], v1[16];
+                    tmem_ld16_nowait(tmem + c + ((q * 32u) << 16), v0);
+                    tmem_ld16_nowait(tmem + P.cap + c + ((q * 32u) << 16), v1);
+                    tmem_wait_ld();
+                    const uint32_t z = ring + (c * 128 + q * 32 + lane) * 4;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        st_shared4(z + j * 512, v0[j]);
+                        st_shared4(z + (P.cap + j) * 512, v1[j]);
+                    }
+                }
+                break;
+            }
             for (uint32_t c = half * 16; c < it.rows; c += 32) {
                 uint32_t v0[16], v1[16];
                 tmem_ld16_nowait(tmem + buf * 2 * P.cap + c + ((q * 32u) << 16), v0);
@@ -479,14 +514,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) group
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[buf]), 0));
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[buf]), leader));
             ++n_done;
         }
     } else if (a.gather) {
         // ---------------- gathered rows: a warp to a ring slot, so that waiting for its copies keeps nobody; eight lanes copy 128 bytes of a row ----------------
         // (one arrival per warp and stage: with one per thread, posted by the copies themselves, the arrivals took longer than the stage)
         const uint32_t slot = warp - 2 - GT_EPI_WARPS, r_in = lane >> 3, chunk = lane & 7u;
-        const uint32_t sb = ring + slot * GT_STAGE + GT_A_BYTES, full = map_to_rank(smem_u32(&full_bar[slot]), 0);
+        const uint32_t sb = ring + slot * GT_STAGE + GT_A_BYTES, full = map_to_rank(smem_u32(&full_bar[slot]), leader);
         uint32_t ph = 0, base = 0;                                // stages of the items before, modulo the ring
         bool ok = true;
         for (uint32_t i = pair; i < n_items && ok; i += n_pairs) {
@@ -499,7 +534,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) group
                 s_row[slot][r] = xr < a.x_rows ? xr : 0;          // out of range: reads row 0, the epilogue skips it
             }
             __syncwarp();
-            for (uint32_t ks = (slot + GT_STAGES - base) % GT_STAGES; ks < P.n_ks; ks += GT_STAGES) {
+            for (uint32_t ks = ks0 + (slot + GT_STAGES - base) % GT_STAGES; ks < ks1; ks += GT_STAGES) {
                 if (!mbar_wait_warp_at(smem_u32(&empty_bar[slot]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
                 const uint32_t k = ks * GT_KS + chunk * 8;
                 const bool there = k < a.K;                       // K is a multiple of 8
@@ -513,13 +548,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GT_THREADS, 1) group
                 if (lane == 0) mbar_arrive_cluster(full);
                 ph ^= 1u;
             }
-            base = (base + P.n_ks) % GT_STAGES;
+            base = (base + ks1 - ks0) % GT_STAGES;
         }
     }
     // every thread comes here, also after a give-up
     tc_fence_before();
     __syncwarp();
     cluster_sync_all();
+    if (P.parts > 1 && pair < n_items) {
+        // the parts of a share of the rows, in order, over distributed shared memory: a thread four outputs of a row, of both accumulators
+        GtWalk w{s_off, s_tiles, a.G};
+        const GtItem it = w.at(pair / P.n_ft);
+        const uint32_t c0 = part * it.rows / P.parts, c1 = (part + 1) * it.rows / P.parts, f0 = (pair % P.n_ft) * FT + rank * (FT / 2);
+        for (uint32_t i = threadIdx.x; i < (c1 - c0) * 32; i += GT_THREADS) {
+            const uint32_t c = c0 + i / 32, f = f0 + i % 32 * 4, p = it.p0 + c, o = a.order ? a.order[p] : p, yr = a.scatter ? o : p;
+            if ((a.gather && o / a.x_div >= a.x_rows) || yr >= a.y_rows) { atomicMax(a.status, ST_BAD_ROW); continue; }
+            float4 v[2] = {};
+            for (uint32_t s = 0; s < P.parts; ++s) {
+                const uint32_t z = map_to_rank(ring + (c * 128 + i % 32 * 4) * 4, 2 * s + rank);
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const float4 w4 = ld_cluster16(z + h * P.cap * 512);
+                    v[h] = s ? make_float4(v[h].x + w4.x, v[h].y + w4.y, v[h].z + w4.z, v[h].w + w4.w) : w4;
+                }
+            }
+            if (SWIGLU)
+                v[0] = make_float4(gp_swiglu<sizeof(O) == 4>(v[0].x, v[1].x, a.limit), gp_swiglu<sizeof(O) == 4>(v[0].y, v[1].y, a.limit),
+                                   gp_swiglu<sizeof(O) == 4>(v[0].z, v[1].z, a.limit), gp_swiglu<sizeof(O) == 4>(v[0].w, v[1].w, a.limit));
+            O* y = static_cast<O*>(a.y) + (size_t)yr * a.ld_y + f;
+#pragma unroll
+            for (uint32_t h = 0; h < (SWIGLU ? 1u : 2u); ++h) {
+                if (f + h * 128 >= a.N) continue;
+                if constexpr (sizeof(O) == 4) *reinterpret_cast<float4*>(y + h * 128) = v[h];
+                else *reinterpret_cast<uint2*>(y + h * 128) = make_uint2(pack2(v[h].x, v[h].y, O()), pack2(v[h].z, v[h].w, O()));
+            }
+        }
+    }
+    if (P.parts > 1) { __syncwarp(); cluster_sync_all(); }   // nobody's shared memory goes away under a reader
     tc_fence_after();
     if (warp == 1) tmem_free_pair(tmem, 512);
 }
@@ -553,6 +618,39 @@ static cudaError_t encode_map(CUtensorMap* map, int dtype, const void* base, con
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// clusters of 1 .. 4 CTA pairs that the device holds at once
+struct GtClusters { uint32_t n[5]; };
+static GtClusters gt_clusters(const void* kernel, int sm_count) {
+    GtClusters c{};
+    for (uint32_t parts = 1; parts <= 4; ++parts) {
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2 * parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(2 * parts * 74); cfg.blockDim = dim3(GT_THREADS); cfg.dynamicSmemBytes = GT_SMEM; cfg.attrs = &attr; cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = sm_count / (int)(2 * parts); }
+        c.n[parts] = n > 0 ? (uint32_t)n : 1u;
+    }
+    return c;
+}
+// How a call is cut: rows of a tile at most (128: two accumulator buffers, 256: one) and parts of the reduction.  The groups' sizes are on the
+// device; the estimate takes them as equal.  A stage costs its products (4 cycles a row) or its bytes (55 a cycle), whichever is longer; joining parts costs
+// as much as eight stages.  Returns the row tiles that the call can have at most.
+static uint32_t gt_cut(const GroupedArgs& a, uint32_t n_ft, uint32_t n_ks, const GtClusters& room, uint32_t* cap, uint32_t* parts) {
+    const uint32_t groups = a.G < a.rows ? a.G : a.rows, per = (a.rows + groups - 1) / groups;
+    double best = 0;
+    for (uint32_t c = 128; c <= 256; c += 128)
+        for (uint32_t s = 1; s <= (c == 128 ? 4u : 1u) && s <= n_ks; ++s) {
+            const uint32_t tiles = (per + c - 1) / c, n = ((per + tiles - 1) / tiles + 31) / 32 * 32;
+            const uint64_t items = (uint64_t)groups * tiles * n_ft, waves = (items + room.n[s] - 1) / room.n[s];
+            const double stage = 4.0 * n > (32768 + n * 64) / 55.0 ? 4.0 * n : (32768 + n * 64) / 55.0;
+            const double t = (double)waves * ((n_ks + s - 1) / s * stage + (s > 1 ? 8 * stage : 0) + (c == 256 ? 3000 : 0));
+            if (best == 0 || t < best) { best = t; *cap = c; *parts = s; }
+        }
+    return a.rows / *cap + groups;
+}
+
 template <bool SWIGLU, class O>
 static cudaError_t tile_launch(const GroupedArgs& a, cudaStream_t st) {
     TileParams P;
@@ -561,7 +659,11 @@ static cudaError_t tile_launch(const GroupedArgs& a, cudaStream_t st) {
     P.n_ks = (a.K + GT_KS - 1) / GT_KS;
     P.fmt = a.dtype == DT_BF16 ? UMMA_BF16 : UMMA_F16;
     P.w_loads = 1;
-    P.cap = a.rows / a.G > 96 ? 256 : 128;
+    const auto kernel = grouped_tile_kernel<SWIGLU, O>;
+    cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GT_SMEM);
+    if (set != cudaSuccess) return set;
+    static const GtClusters room = gt_clusters(reinterpret_cast<const void*>(kernel), a.sm_count);
+    const uint32_t most_tiles = gt_cut(a, P.n_ft, P.n_ks, room, &P.cap, &P.parts);
     cudaError_t e;
     const uint64_t N = a.N, K = a.K, G = a.G, ld = a.ld_w, gs = a.w_stride;
     // A box is one CTA's weights of a stage.  Activation: gate rows, then up rows (outputs first), or 64 outputs' gate and up
@@ -580,10 +682,13 @@ static cudaError_t tile_launch(const GroupedArgs& a, cudaStream_t st) {
     for (uint32_t i = 0; i < GT_BOXES && !a.gather && e == cudaSuccess; ++i)
         e = encode_map<2>(&P.x[i], a.dtype, a.x, {K, a.x_rows}, {a.ld_x}, {64, gt_box_rows(i)});
     if (e != cudaSuccess) return e;
-    const auto kernel = grouped_tile_kernel<SWIGLU, O>;
-    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GT_SMEM)) != cudaSuccess) return e;
-    kernel<<<a.sm_count / 2 * 2, GT_THREADS, GT_SMEM, st>>>(P);
-    return cudaGetLastError();
+    const uint32_t clusters = P.parts == 1 ? (uint32_t)a.sm_count / 2 : most_tiles * P.n_ft;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2 * P.parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(clusters * 2 * P.parts); cfg.blockDim = dim3(GT_THREADS); cfg.dynamicSmemBytes = GT_SMEM; cfg.stream = st; cfg.attrs = &attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P);
 }
 template <bool BF16, class O>
 static cudaError_t grouped_out(const GroupedArgs& a, cudaStream_t st) {
