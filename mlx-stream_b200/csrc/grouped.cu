@@ -235,6 +235,7 @@ constexpr uint32_t GT_THREADS = 64 + (GT_EPI_WARPS + GT_GATHER_WARPS) * 32;
 constexpr uint32_t GT_TURN = 8 * 32 * 4;                         // an epilogue warp's turn of 16 rows x 32 outputs, two rows to a word
 constexpr uint32_t GT_SMEM = GT_STAGES * GT_STAGE + GT_EPI_WARPS * 2 * GT_TURN + 1024;
 
+constexpr uint32_t GT_PARTS = 4;                                  // most parts of a reduction: a cluster of eight CTAs
 constexpr uint32_t GT_BOXES = 5;
 __host__ __device__ constexpr uint32_t gt_box_rows(uint32_t i) { return i < 3 ? 16u << i : 32 * i; }   // 16 32 64 96 128
 
@@ -242,7 +243,7 @@ struct TileParams {
     CUtensorMap w, x[GT_BOXES];   // x by box height
     GroupedArgs a;
     uint32_t n_ft, n_ks;          // output tiles of a row tile, stages
-    uint32_t cap;                 // most rows of a tile: 128 or 256
+    uint32_t cap;                 // most rows of a tile: 128, 160, 192 or 256
     uint32_t w_loads;             // copies that a stage of weights takes
     uint32_t fmt;
     uint32_t parts;               // parts of the reduction, a CTA pair of the item's cluster to each (1: no cluster, pairs walk the items)
@@ -563,14 +564,20 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
         for (uint32_t i = threadIdx.x; i < (c1 - c0) * 32; i += GT_THREADS) {
             const uint32_t c = c0 + i / 32, f = f0 + i % 32 * 4, p = it.p0 + c, o = a.order ? a.order[p] : p, yr = a.scatter ? o : p;
             if ((a.gather && o / a.x_div >= a.x_rows) || yr >= a.y_rows) { atomicMax(a.status, ST_BAD_ROW); continue; }
-            float4 v[2] = {};
-            for (uint32_t s = 0; s < P.parts; ++s) {
-                const uint32_t z = map_to_rank(ring + (c * 128 + i % 32 * 4) * 4, 2 * s + rank);
+            float4 w4[GT_PARTS][2], v[2];
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    const float4 w4 = ld_cluster16(z + h * P.cap * 512);
-                    v[h] = s ? make_float4(v[h].x + w4.x, v[h].y + w4.y, v[h].z + w4.z, v[h].w + w4.w) : w4;
+            for (uint32_t s = 0; s < GT_PARTS; ++s)          // all on their way before the first is added
+                if (s < P.parts) {
+                    const uint32_t z = map_to_rank(ring + (c * 128 + i % 32 * 4) * 4, 2 * s + rank);
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) w4[s][h] = ld_cluster16(z + h * P.cap * 512);
                 }
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                v[h] = w4[0][h];
+#pragma unroll
+                for (uint32_t s = 1; s < GT_PARTS; ++s)
+                    if (s < P.parts) v[h] = make_float4(v[h].x + w4[s][h].x, v[h].y + w4[s][h].y, v[h].z + w4[s][h].z, v[h].w + w4[s][h].w);
             }
             if (SWIGLU)
                 v[0] = make_float4(gp_swiglu<sizeof(O) == 4>(v[0].x, v[1].x, a.limit), gp_swiglu<sizeof(O) == 4>(v[0].y, v[1].y, a.limit),
@@ -619,10 +626,10 @@ static cudaError_t encode_map(CUtensorMap* map, int dtype, const void* base, con
 }
 
 // clusters of 1 .. 4 CTA pairs that the device holds at once
-struct GtClusters { uint32_t n[5]; };
+struct GtClusters { uint32_t n[GT_PARTS + 1]; };
 static GtClusters gt_clusters(const void* kernel, int sm_count) {
     GtClusters c{};
-    for (uint32_t parts = 1; parts <= 4; ++parts) {
+    for (uint32_t parts = 1; parts <= GT_PARTS; ++parts) {
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = 2 * parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
@@ -634,18 +641,19 @@ static GtClusters gt_clusters(const void* kernel, int sm_count) {
     }
     return c;
 }
-// How a call is cut: rows of a tile at most (128: two accumulator buffers, 256: one) and parts of the reduction.  The groups' sizes are on the
+// How a call is cut: rows of a tile at most (128: two accumulator buffers; more: one; the parts' sums fit where the ring was up to 192) and parts of
+// the reduction.  The groups' sizes are on the
 // device; the estimate takes them as equal.  A stage costs its products (4 cycles a row) or its bytes (55 a cycle), whichever is longer; joining parts costs
 // as much as eight stages.  Returns the row tiles that the call can have at most.
 static uint32_t gt_cut(const GroupedArgs& a, uint32_t n_ft, uint32_t n_ks, const GtClusters& room, uint32_t* cap, uint32_t* parts) {
     const uint32_t groups = a.G < a.rows ? a.G : a.rows, per = (a.rows + groups - 1) / groups;
     double best = 0;
-    for (uint32_t c = 128; c <= 256; c += 128)
-        for (uint32_t s = 1; s <= (c == 128 ? 4u : 1u) && s <= n_ks; ++s) {
+    for (const uint32_t c : {128u, 160u, 192u, 256u})
+        for (uint32_t s = 1; s <= (c <= 192 ? GT_PARTS : 1u) && s <= n_ks; ++s) {
             const uint32_t tiles = (per + c - 1) / c, n = ((per + tiles - 1) / tiles + 31) / 32 * 32;
             const uint64_t items = (uint64_t)groups * tiles * n_ft, waves = (items + room.n[s] - 1) / room.n[s];
             const double stage = 4.0 * n > (32768 + n * 64) / 55.0 ? 4.0 * n : (32768 + n * 64) / 55.0;
-            const double t = (double)waves * ((n_ks + s - 1) / s * stage + (s > 1 ? 8 * stage : 0) + (c == 256 ? 3000 : 0));
+            const double t = (double)waves * ((n_ks + s - 1) / s * stage + (s > 1 ? 8 * stage : 0) + (s == 1 && c > 128 ? 3000 : 0));
             if (best == 0 || t < best) { best = t; *cap = c; *parts = s; }
         }
     return a.rows / *cap + groups;
