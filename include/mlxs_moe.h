@@ -282,7 +282,7 @@ typedef struct {
     uint64_t ld_w, w_stride;      /* elements from row to row of a group's matrix and from group to group, multiples of 8 (0: dense) */
 } mlxs_grouped_desc;
 /* y[p] = W_g x[p], or silu(gate_g x[p]) * (up_g x[p]), for the sorted positions offsets_dev[g] <= p < offsets_dev[g + 1]
- * (u32 [n_groups + 1], as mlxs_moe_sort_rows writes it).  Sums in f32, one rounding to y's type.  Positions of no group, and the
+ * (u32 [n_groups + 1], as mlxs_moe_sort_rows writes it; NULL with n_groups = 1: all rows).  Sums in f32, one rounding to y's type.  Positions of no group, and the
  * rows of y that no position writes, are left as they were; a group may be empty.  Without GATHER position p reads row p of x,
  * without SCATTER it writes row p of y; with SCATTER row order_dev[p] (u32 [rows], as mlxs_moe_sort_rows writes it; positions
  * of one call write different rows).  y overlaps neither x nor w.  An index out of range skips its position, offsets that descend or pass
@@ -309,6 +309,24 @@ typedef struct {
 int mlxs_moe_adapters(mlxs_moe *h, const mlxs_adapters_desc *desc, const void *x_dev, const void *a_dev, const void *b_dev,
                       const int32_t *ids_dev, const float *scales_dev, const int32_t *ranks_dev, const void *base_dev,
                       void *y_dev, void *stream);
+
+/* Adapters on the three linears of a layer's shared expert, for one call: bf16 device arrays of the caller, a1 [n_adapters, rank, hidden], b1
+ * [n_adapters, inter, rank] on w1 (gate), a3 / b3 on w3 (up) the same, a2 [n_adapters, rank, inter], b2 [n_adapters, hidden, rank] on w2 (down); a pair
+ * that is NULL leaves its linear alone.  scales_dev, ranks_dev as for mlxs_moe_adapters. */
+typedef struct {
+    uint32_t struct_size;         /* sizeof(mlxs_shared_adapters) */
+    uint32_t rank, n_adapters;
+    const void *a1_dev, *b1_dev, *a3_dev, *b3_dev, *a2_dev, *b2_dev;
+    const float *scales_dev;
+    const int32_t *ranks_dev;
+} mlxs_shared_adapters;
+/* Allocates what mlxs_moe_experts_adapted needs (f32 [max_tokens, 2 inter]); once per handle, at load time. */
+int mlxs_moe_reserve_adapters(mlxs_moe *h);
+/* mlxs_moe_experts with adapters on the shared expert: token t's adapter is adapter_ids_dev[t] (negative: none), f32 rows between the linears and
+ * their adapters, h rounded to bf16 as without them.  The routed experts are as in mlxs_moe_experts. */
+int mlxs_moe_experts_adapted(mlxs_moe *h, uint32_t layer, const void *x_dev, const int32_t *ids_dev, const float *weights_dev,
+                             uint32_t T, const mlxs_shared_adapters *adapters, const int32_t *adapter_ids_dev, void *y_dev,
+                             void *stream);
 
 /* ---- expert parallel (no counterpart in the reference: it pages experts from SSD on one GPU; here they are HBM
  * resident and sharded, with a dispatch and a combine all-to-all per layer) ---- */

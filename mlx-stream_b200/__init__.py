@@ -38,7 +38,7 @@ EXPORTS = [
     "mlxs_moe_ep_window_bytes", "mlxs_moe_ep_overloaded_rank",
     "mlxs_moe_status_clear", "mlxs_moe_sort_rows", "mlxs_moe_debug_wait", "mlxs_moe_exl3_decode_rate", "mlxs_moe_fp4_native_probe", "mlxs_moe_mma_rate",
     "mlxs_moe_bank_verify", "mlxs_moe_usage_enable", "mlxs_moe_usage_add", "mlxs_moe_usage_read", "mlxs_moe_usage_reset", "mlxs_moe_plan_placement",
-    "mlxs_moe_grouped", "mlxs_moe_adapters",
+    "mlxs_moe_grouped", "mlxs_moe_adapters", "mlxs_moe_reserve_adapters", "mlxs_moe_experts_adapted",
 ]
 
 
@@ -87,6 +87,16 @@ class AdaptersDesc(C.Structure):
     _fields_ = [("struct_size", C.c_uint32), ("dtype", C.c_uint32), ("out_dtype", C.c_uint32), ("n_in", C.c_uint32), ("n_out", C.c_uint32),
                 ("rank", C.c_uint32), ("n_adapters", C.c_uint32), ("tokens", C.c_uint32), ("ld_x", C.c_uint64), ("ld_base", C.c_uint64),
                 ("ld_y", C.c_uint64), ("a_stride", C.c_uint64), ("b_stride", C.c_uint64)]
+
+
+class SharedAdapters(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("rank", C.c_uint32), ("n_adapters", C.c_uint32), ("a1", C.c_void_p), ("b1", C.c_void_p),
+                ("a3", C.c_void_p), ("b3", C.c_void_p), ("a2", C.c_void_p), ("b2", C.c_void_p), ("scales", C.c_void_p), ("ranks", C.c_void_p)]
+
+
+def make_shared_adapters(rank, n_adapters, a1=None, b1=None, a3=None, b3=None, a2=None, b2=None, scales=None, ranks=None):
+    """Adapters on a shared expert's linears (gate: a1, b1; up: a3, b3; down: a2, b2), device pointers; None leaves a linear alone."""
+    return SharedAdapters(C.sizeof(SharedAdapters), rank, n_adapters, a1, b1, a3, b3, a2, b2, scales, ranks)
 
 
 class MlxsError(RuntimeError):
@@ -159,6 +169,9 @@ def lib():
         L.mlxs_moe_debug_wait.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32]
         L.mlxs_moe_grouped.argtypes = [C.c_void_p, C.POINTER(GroupedDesc)] + [C.c_void_p] * 6
         L.mlxs_moe_adapters.argtypes = [C.c_void_p, C.POINTER(AdaptersDesc)] + [C.c_void_p] * 9
+        L.mlxs_moe_reserve_adapters.argtypes = [C.c_void_p]
+        L.mlxs_moe_experts_adapted.argtypes = [C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.POINTER(SharedAdapters),
+                                               C.c_void_p, C.c_void_p, C.c_void_p]
         if L.mlxs_moe_abi() != ABI:
             raise RuntimeError(f"libmlxs_moe.so ABI {L.mlxs_moe_abi()} != binding ABI {ABI}")
         _lib = L
@@ -360,6 +373,14 @@ class MoE:
         d = AdaptersDesc(C.sizeof(AdaptersDesc), dtype, dtype if out_dtype is None else out_dtype, n_in, n_out, rank, n_adapters, T,
                          ld_x, ld_base, ld_y, a_stride, b_stride)
         _check(lib().mlxs_moe_adapters(self._h, C.byref(d), x, a, b, ids, scales, ranks, base, y, stream))
+
+    def reserve_adapters(self):
+        """The workspace of experts_adapted; once, at load time."""
+        _check(lib().mlxs_moe_reserve_adapters(self._h))
+
+    def experts_adapted(self, layer, x, ids, weights, T, adapters, adapter_ids, y, stream=None):
+        """experts with adapters (make_shared_adapters) on the shared expert; token t's adapter is adapter_ids[t], negative: none."""
+        _check(lib().mlxs_moe_experts_adapted(self._h, layer, x, ids, weights, T, C.byref(adapters), adapter_ids, y, stream))
 
     def debug_wait(self, poll_limit=0, withhold_stage=0):
         """Self-test hook of the bounded waits: a short poll limit and one withheld ring stage."""

@@ -326,8 +326,13 @@ static bool front_applies(const mlxs_moe* h, uint32_t T, bool from_x) {
     return front_fits((int)h->cfg.n_experts, (int)h->cfg.top_k, T, h->cfg.hidden, from_x, h->front_smem_max);
 }
 
+// adapters on the shared expert of one call
+struct AdaptedCall {
+    const mlxs_shared_adapters* d;
+    const int32_t* ids;
+};
 static int experts_impl(mlxs_moe* h, uint32_t layer, const void* x_dev, const int32_t* ids_dev, const float* weights_dev,
-                        uint32_t T, void* y_dev, void* stream, const FrontCall* front, bool fork_recorded = false);
+                        uint32_t T, void* y_dev, void* stream, const FrontCall* front, bool fork_recorded = false, const AdaptedCall* adapted = nullptr);
 
 int mlxs_bank_for_each_record(const char* dir, uint32_t bank_kind, uint64_t H, uint64_t I, uint64_t E, uint64_t n_layers,
                               uint32_t e_first, uint32_t e_count, int (*layer_begin)(void* ctx, uint32_t layer, uint32_t bits),
@@ -753,7 +758,7 @@ extern "C" int mlxs_moe_routed(mlxs_moe* h, uint32_t layer, const void* x_dev, c
 }
 
 static int experts_impl(mlxs_moe* h, uint32_t layer, const void* x_dev, const int32_t* ids_dev, const float* weights_dev,
-                        uint32_t T, void* y_dev, void* stream, const FrontCall* front, bool fork_recorded) {
+                        uint32_t T, void* y_dev, void* stream, const FrontCall* front, bool fork_recorded, const AdaptedCall* adapted) {
     int rc = check_call(h, layer, T, "experts");
     if (rc) return rc;
     if (T == 0 && h->cfg.ep_world == 1) return MLXS_OK;  // with expert parallelism an empty rank still serves its peers
@@ -780,7 +785,9 @@ static int experts_impl(mlxs_moe* h, uint32_t layer, const void* x_dev, const in
     const float* shared = nullptr;
     auto run_shared = [&](cudaStream_t s) -> int {
         const float lim = c.act == MLXS_ACT_SWIGLU_CLAMPED ? c.act_limit : 0.f;
-        if (T >= shared_dense_min() && L.sh_gu_t) {
+        if (adapted) {
+            if (T) CU(mlxs_run_shared_adapted(h, L, x_dev, T, *adapted->d, adapted->ids, h->sh_out, s));
+        } else if (T >= shared_dense_min() && L.sh_gu_t) {
             DenseSharedArgs da{};
             da.x = static_cast<const __nv_bfloat16*>(x_dev); da.w_gu = L.sh_gu_t; da.w_d = L.sh_d_t;
             da.T = T; da.H = c.hidden; da.I = c.inter; da.limit = lim; da.xb = h->dg_xb; da.hb = h->dg_hb; da.out = h->sh_out;
@@ -858,6 +865,17 @@ static int experts_impl(mlxs_moe* h, uint32_t layer, const void* x_dev, const in
 extern "C" int mlxs_moe_experts(mlxs_moe* h, uint32_t layer, const void* x_dev, const int32_t* ids_dev,
                                 const float* weights_dev, uint32_t T, void* y_dev, void* stream) {
     return experts_impl(h, layer, x_dev, ids_dev, weights_dev, T, y_dev, stream, nullptr);
+}
+
+extern "C" int mlxs_moe_experts_adapted(mlxs_moe* h, uint32_t layer, const void* x_dev, const int32_t* ids_dev, const float* weights_dev,
+                                        uint32_t T, const mlxs_shared_adapters* adapters, const int32_t* adapter_ids_dev, void* y_dev, void* stream) {
+    int rc = T ? mlxs_check_shared_adapters(adapters, adapter_ids_dev) : 0;
+    if (rc) return rc;
+    if (!h) return fail(MLXS_E_ARG, "experts_adapted: null handle");
+    if (!h->cfg.shared_expert) return fail(MLXS_E_CONFIG, "experts_adapted: the handle was created without a shared expert");
+    if (T && !h->sh_gate_up) return fail(MLXS_E_NOT_LOADED, "experts_adapted: no workspace (mlxs_moe_reserve_adapters)");
+    const AdaptedCall ac{adapters, adapter_ids_dev};
+    return experts_impl(h, layer, x_dev, ids_dev, weights_dev, T, y_dev, stream, nullptr, false, &ac);
 }
 
 extern "C" int mlxs_moe_forward(mlxs_moe* h, uint32_t layer, const void* x_dev, const float* logits_dev, uint32_t T,

@@ -77,7 +77,7 @@ extern "C" int mlxs_moe_grouped(mlxs_moe* h, const mlxs_grouped_desc* d, const v
     if (!a.gather && !a.scatter) order_dev = nullptr;
     else if ((rc = check_ptr(who, "order_dev", order_dev, 4))) return rc;
     if ((rc = check_ptr(who, "x_dev", x_dev, 16)) || (rc = check_ptr(who, "w_dev", w_dev, 16)) || (rc = check_ptr(who, "y_dev", y_dev, 16)) ||
-        (rc = check_ptr(who, "offsets_dev", offsets_dev, 4)))
+        ((offsets_dev || a.G != 1) && (rc = check_ptr(who, "offsets_dev", offsets_dev, 4))))
         return rc;
     if (a.x_rows == 0 || a.y_rows == 0) return mlxs_fail(MLXS_E_ARG, "grouped: x_rows %u, y_rows %u with %u rows", a.x_rows, a.y_rows, a.rows);
     if (!h) return mlxs_fail(MLXS_E_ARG, "grouped: null handle");
@@ -125,4 +125,65 @@ extern "C" int mlxs_moe_adapters(mlxs_moe* h, const mlxs_adapters_desc* d, const
     if (e == cudaSuccess) e = launch_adapters(a, (cudaStream_t)stream);
     if (e != cudaSuccess) return mlxs_fail(MLXS_E_CUDA, "adapters: %s", cudaGetErrorString(e));
     return MLXS_OK;
+}
+
+extern "C" int mlxs_moe_reserve_adapters(mlxs_moe* h) {
+    if (!h) return mlxs_fail(MLXS_E_ARG, "reserve_adapters: null handle");
+    if (!h->cfg.shared_expert) return mlxs_fail(MLXS_E_CONFIG, "reserve_adapters: the handle was created without a shared expert");
+    if (h->sh_gate_up) return MLXS_OK;
+    DeviceGuard dev;
+    const cudaError_t e = dev.enter(h->cfg.device);
+    if (e != cudaSuccess) return mlxs_fail(MLXS_E_CUDA, "reserve_adapters: %s", cudaGetErrorString(e));
+    return h->alloc(&h->sh_gate_up, (size_t)h->cfg.max_tokens * 2 * h->cfg.inter * 4);
+}
+
+// what mlxs_moe_experts_adapted is given, before any device is touched
+int mlxs_check_shared_adapters(const mlxs_shared_adapters* d, const int32_t* adapter_ids_dev) {
+    const char* who = "experts_adapted";
+    if (!d) return mlxs_fail(MLXS_E_ARG, "experts_adapted: null descriptor");
+    if (d->struct_size != sizeof *d) return mlxs_fail(MLXS_E_CONFIG, "experts_adapted: struct_size %u, this library has %zu", d->struct_size, sizeof *d);
+    if (d->rank == 0 || d->rank % 8 || d->rank > MAX_RANK) return mlxs_fail(MLXS_E_CONFIG, "experts_adapted: rank %u is not a multiple of 8 in 8..%u", d->rank, MAX_RANK);
+    if (d->n_adapters == 0 || d->n_adapters > MAX_ROWS) return mlxs_fail(MLXS_E_CONFIG, "experts_adapted: n_adapters %u outside 1..%u", d->n_adapters, MAX_ROWS);
+    const void* const pairs[3][2] = {{d->a1_dev, d->b1_dev}, {d->a3_dev, d->b3_dev}, {d->a2_dev, d->b2_dev}};
+    const char* const names[3] = {"a1_dev / b1_dev", "a3_dev / b3_dev", "a2_dev / b2_dev"};
+    int rc;
+    for (int i = 0; i < 3; ++i) {
+        if (!pairs[i][0] != !pairs[i][1]) return mlxs_fail(MLXS_E_ARG, "experts_adapted: one of %s is null", names[i]);
+        for (int k = 0; k < 2; ++k)
+            if (pairs[i][k] && (rc = check_ptr(who, names[i], pairs[i][k], 16))) return rc;
+    }
+    if ((rc = check_ptr(who, "adapter_ids_dev", adapter_ids_dev, 4)) || (d->scales_dev && (rc = check_ptr(who, "scales_dev", d->scales_dev, 4))) ||
+        (d->ranks_dev && (rc = check_ptr(who, "ranks_dev", d->ranks_dev, 4))))
+        return rc;
+    return 0;
+}
+
+// The shared expert with adapters on its three linears: f32 gate and up rows, adapters on both, the activation, the down product, its adapters.
+cudaError_t mlxs_run_shared_adapted(mlxs_moe* h, const LayerBank& L, const void* x_dev, uint32_t T, const mlxs_shared_adapters& d,
+                                    const int32_t* adapter_ids_dev, float* out, cudaStream_t st) {
+    const uint32_t H = h->cfg.hidden, I = h->cfg.inter;
+    cudaError_t e;
+    auto product = [&](const void* x, const void* w, uint32_t K, uint32_t N, float* y, size_t ld_y) {
+        GroupedArgs a{};
+        a.x = x; a.w = w; a.y = y; a.G = 1; a.K = K; a.N = N; a.rows = a.x_rows = a.y_rows = T; a.x_div = 1;
+        a.dtype = DT_BF16; a.out_dtype = DT_F32; a.ld_x = a.ld_w = K; a.ld_y = ld_y; a.w_stride = (size_t)N * K;
+        a.status = h->status; a.sm_count = h->sm_count;
+        return launch_grouped(a, st);
+    };
+    auto adapt = [&](const void* x, const void* A, const void* B, uint32_t K, uint32_t N, float* y, size_t ld_y) {
+        if (!A) return cudaSuccess;
+        AdaptersArgs a{};
+        a.x = x; a.a = A; a.b = B; a.base = a.y = y; a.ids = adapter_ids_dev; a.scales = d.scales_dev; a.ranks = d.ranks_dev;
+        a.K = K; a.N = N; a.R = d.rank; a.n_adapters = d.n_adapters; a.T = T; a.dtype = DT_BF16; a.out_dtype = DT_F32;
+        a.ld_x = K; a.ld_base = a.ld_y = ld_y; a.a_stride = (size_t)d.rank * K; a.b_stride = (size_t)N * d.rank;
+        a.status = h->status; a.sm_count = h->sm_count;
+        return launch_adapters(a, st);
+    };
+    const float limit = h->cfg.act == MLXS_ACT_SWIGLU_CLAMPED ? h->cfg.act_limit : 0.f;
+    float* const gu = h->sh_gate_up;
+    if ((e = product(x_dev, L.sh_w1, H, I, gu, 2 * (size_t)I)) != cudaSuccess || (e = product(x_dev, L.sh_w3, H, I, gu + I, 2 * (size_t)I)) != cudaSuccess ||
+        (e = adapt(x_dev, d.a1_dev, d.b1_dev, H, I, gu, 2 * (size_t)I)) != cudaSuccess || (e = adapt(x_dev, d.a3_dev, d.b3_dev, H, I, gu + I, 2 * (size_t)I)) != cudaSuccess ||
+        (e = launch_gate_up_act(gu, T, I, limit, h->sh_h, st)) != cudaSuccess || (e = product(h->sh_h, L.sh_w2, I, H, out, H)) != cudaSuccess)
+        return e;
+    return adapt(h->sh_h, d.a2_dev, d.b2_dev, I, H, out, H);
 }

@@ -20,6 +20,7 @@ __device__ __forceinline__ float gp_swiglu(float g, float u, float limit) {
 
 // The rows [r0, r1) of group g, cut to the call's rows; false where the offsets had to be cut
 __device__ __forceinline__ bool gp_range(const GroupedArgs& a, uint32_t g, uint32_t& r0, uint32_t& r1) {
+    if (!a.offsets) { r0 = 0; r1 = a.rows; return true; }   // one group
     const uint32_t o0 = a.offsets[g], o1 = a.offsets[g + 1];
     r0 = min(o0, a.rows);
     r1 = max(min(o1, a.rows), r0);
@@ -709,6 +710,22 @@ static cudaError_t grouped_out(const GroupedArgs& a, cudaStream_t st) {
 cudaError_t launch_grouped(const GroupedArgs& a, cudaStream_t st) {
     if (a.dtype == DT_BF16) return a.out_dtype == DT_F32 ? grouped_out<true, float>(a, st) : grouped_out<true, __nv_bfloat16>(a, st);
     return a.out_dtype == DT_F32 ? grouped_out<false, float>(a, st) : grouped_out<false, __half>(a, st);
+}
+
+__global__ void __launch_bounds__(256) gate_up_act_kernel(const float* __restrict__ gate_up, uint32_t T, uint32_t I, float limit, __nv_bfloat16* __restrict__ h) {
+    const size_t n = (size_t)T * (I / 4);                   // four outputs to a thread
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const size_t t = i / (I / 4), f = i % (I / 4) * 4;
+        const float4 g = *reinterpret_cast<const float4*>(gate_up + t * 2 * I + f), u = *reinterpret_cast<const float4*>(gate_up + t * 2 * I + I + f);
+        *reinterpret_cast<uint2*>(h + t * I + f) =
+            make_uint2(pack2(gp_swiglu<true>(g.x, u.x, limit), gp_swiglu<true>(g.y, u.y, limit), __nv_bfloat16()),
+                       pack2(gp_swiglu<true>(g.z, u.z, limit), gp_swiglu<true>(g.w, u.w, limit), __nv_bfloat16()));
+    }
+}
+cudaError_t launch_gate_up_act(const float* gate_up, uint32_t T, uint32_t I, float limit, __nv_bfloat16* h, cudaStream_t st) {
+    const size_t blocks = ((size_t)T * (I / 4) + 255) / 256;
+    gate_up_act_kernel<<<(uint32_t)(blocks < 2368 ? blocks : 2368), 256, 0, st>>>(gate_up, T, I, limit, h);
+    return cudaGetLastError();
 }
 
 }  // namespace mlxs

@@ -81,6 +81,7 @@ struct mlxs_moe {
     cudaStream_t lane_stream = nullptr;
     cudaEvent_t lane_fork = nullptr, lane_join = nullptr;
     float* sh_out = nullptr;
+    float* sh_gate_up = nullptr;      // [max_tokens, 2 inter] f32: the shared expert's rows under adapters (mlxs_moe_reserve_adapters), or null
     uint32_t* status = nullptr;
     uint8_t* staging = nullptr;
     void *x_io = nullptr, *y_io = nullptr;
@@ -158,3 +159,7 @@ int mlxs_ep_transport(const mlxs_moe* h);                         // 0 none, 1 N
 void mlxs_ep_bytes(mlxs_moe* h, uint64_t* sent, uint64_t* recv);  // adds the peer-store transport's device-side byte counts
 // sum of a u64 array over the ranks, in place (expert-parallel handles)
 int mlxs_ep_allreduce_u64(mlxs_moe* h, unsigned long long* buf_dev, size_t n, cudaStream_t st);
+// the shared expert with adapters (api_products.cu)
+int mlxs_check_shared_adapters(const mlxs_shared_adapters* d, const int32_t* adapter_ids_dev);
+cudaError_t mlxs_run_shared_adapted(mlxs_moe* h, const LayerBank& L, const void* x_dev, uint32_t T, const mlxs_shared_adapters& d,
+                                    const int32_t* adapter_ids_dev, float* out, cudaStream_t st);

@@ -292,7 +292,7 @@ struct GroupedArgs {
     const void* x;
     const void* w;
     void* y;
-    const uint32_t* offsets;     // [G + 1]
+    const uint32_t* offsets;     // [G + 1], or null: one group of all rows
     const uint32_t* order;       // [rows] or null
     uint32_t G, K, N, rows;      // N outputs of y; a group's matrix has n_w() of them
     uint32_t x_div, x_rows, y_rows;
@@ -305,6 +305,9 @@ struct GroupedArgs {
     __host__ __device__ uint32_t n_w() const { return swiglu ? 2 * N : N; }
 };
 cudaError_t launch_grouped(const GroupedArgs& a, cudaStream_t st);
+
+// h[t] = bf16(act(gate, up)) of f32 rows [T, 2 I], the gate's inputs first
+cudaError_t launch_gate_up_act(const float* gate_up, uint32_t T, uint32_t I, float limit, __nv_bfloat16* h, cudaStream_t st);
 
 // ---- low-rank adapters (adapters.cu) ----
 struct AdaptersArgs {

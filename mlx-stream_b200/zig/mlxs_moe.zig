@@ -165,6 +165,21 @@ pub const AdaptersDesc = extern struct {
     b_stride: u64 = 0,
 };
 pub extern fn mlxs_moe_adapters(h: *Moe, desc: *const AdaptersDesc, x_dev: ?*const anyopaque, a_dev: ?*const anyopaque, b_dev: ?*const anyopaque, ids_dev: ?[*]const i32, scales_dev: ?[*]const f32, ranks_dev: ?[*]const i32, base_dev: ?*const anyopaque, y_dev: ?*anyopaque, stream: ?*anyopaque) c_int;
+pub const SharedAdapters = extern struct {
+    struct_size: u32 = @sizeOf(SharedAdapters),
+    rank: u32,
+    n_adapters: u32,
+    a1_dev: ?*const anyopaque = null,
+    b1_dev: ?*const anyopaque = null,
+    a3_dev: ?*const anyopaque = null,
+    b3_dev: ?*const anyopaque = null,
+    a2_dev: ?*const anyopaque = null,
+    b2_dev: ?*const anyopaque = null,
+    scales_dev: ?[*]const f32 = null,
+    ranks_dev: ?[*]const i32 = null,
+};
+pub extern fn mlxs_moe_reserve_adapters(h: *Moe) c_int;
+pub extern fn mlxs_moe_experts_adapted(h: *Moe, layer: u32, x_dev: ?*const anyopaque, ids_dev: ?[*]const i32, weights_dev: ?[*]const f32, T: u32, adapters: ?*const SharedAdapters, adapter_ids_dev: ?[*]const i32, y_dev: ?*anyopaque, stream: ?*anyopaque) c_int;
 
 pub const Error = error{ Arg, Config, Cuda, Bank, NotLoaded, TooManyTokens, DeviceStatus, Manifest, Ep };
 

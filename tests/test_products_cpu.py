@@ -42,6 +42,7 @@ def test_descriptors_match_the_header_layout():
     (dict(w_stride=256 * 127), pkg.E_ARG, "w_stride"), (dict(w_stride=1 << 40), pkg.E_ARG, "w_stride"), (dict(x=None), pkg.E_ARG, "x_dev"),
     (dict(w=P + 8), pkg.E_ARG, "w_dev"), (dict(y=P + 2), pkg.E_ARG, "y_dev"), (dict(x=P + 8), pkg.E_ARG, "x_dev"),
     (dict(offsets=P + 2), pkg.E_ARG, "offsets_dev"), (dict(offsets=None), pkg.E_ARG, "offsets_dev"),
+    (dict(offsets=None, n_groups=1), pkg.E_ARG, "null handle"),
     (dict(row_flags=1, order=None), pkg.E_ARG, "order_dev"), (dict(row_flags=2, order=P + 1), pkg.E_ARG, "order_dev"),
     (dict(), pkg.E_ARG, "null handle"), (dict(rows=0), pkg.E_ARG, "null handle"),
 ])
@@ -66,7 +67,24 @@ def test_adapters_refuse_by_name(kw, rc, word):
     assert pkg.last_error().startswith("adapters: ") and word in pkg.last_error()
 
 
+@pytest.mark.parametrize("kw, rc, word", [
+    (dict(struct_size=8), pkg.E_CONFIG, "struct_size"), (dict(rank=4), pkg.E_CONFIG, "rank"), (dict(rank=512), pkg.E_CONFIG, "rank"),
+    (dict(n_adapters=0), pkg.E_CONFIG, "n_adapters"), (dict(a1=None), pkg.E_ARG, "a1_dev"), (dict(b3=None), pkg.E_ARG, "a3_dev"),
+    (dict(a2=P + 8), pkg.E_ARG, "a2_dev"), (dict(scales=P + 2), pkg.E_ARG, "scales_dev"), (dict(ranks=P + 1), pkg.E_ARG, "ranks_dev"),
+    (dict(ids=None), pkg.E_ARG, "adapter_ids_dev"), (dict(), pkg.E_ARG, "null handle"),
+])
+def test_experts_adapted_refuses_by_name(kw, rc, word):
+    f = dict(struct_size=C.sizeof(pkg.SharedAdapters), rank=16, n_adapters=2, a1=P, b1=P, a3=P, b3=P, a2=P, b2=P, scales=P, ranks=P)
+    ids = kw.pop("ids", P)
+    f.update(kw)
+    assert pkg.lib().mlxs_moe_experts_adapted(None, 0, P, P, P, 3, C.byref(pkg.SharedAdapters(**f)), ids, P, None) == rc, pkg.last_error()
+    assert pkg.last_error().startswith("experts_adapted: ") and word in pkg.last_error()
+
+
 def test_null_descriptors_are_refused():
+    assert C.sizeof(pkg.SharedAdapters) == 16 + 8 * 8
+    assert pkg.lib().mlxs_moe_experts_adapted(None, 0, P, P, P, 3, None, P, P, None) == pkg.E_ARG
+    assert pkg.lib().mlxs_moe_reserve_adapters(None) == pkg.E_ARG
     L = pkg.lib()
     assert L.mlxs_moe_grouped(None, None, P, P, P, P, P, None) == pkg.E_ARG
     assert L.mlxs_moe_adapters(None, None, P, P, P, P, None, None, P, P, None) == pkg.E_ARG

@@ -160,6 +160,13 @@ def test_grouped_many_or_one_group(moe, G, rows):
     c.check()
 
 
+@pytest.mark.parametrize("rows", [1, 16, 17, 200])
+def test_grouped_one_group_without_offsets(moe, rows):
+    c = Grouped([rows], 264, 136)
+    moe.grouped(c.x_all.data_ptr(), c.w_all.data_ptr(), None, c.y_all.data_ptr(), rows, 1, 264, 136, stream=torch.cuda.current_stream().cuda_stream)
+    c.check()
+
+
 @pytest.mark.parametrize("H, I, tokens", [(5120, 2304, 1), (4096, 2048, 9), (6144, 2048, 70)])
 def test_grouped_layer_geometries(moe, H, I, tokens):
     rng = np.random.default_rng(tokens)
@@ -511,3 +518,61 @@ def test_a_layer_from_the_two_operators(moe):
         at = (adapter == i).nonzero().squeeze(1)
         want[at] += X[at] @ a[i].double().T @ b[i].double().T
     assert float((y.double() - want).norm() / want.norm()) <= 2.0 ** -15
+
+
+@pytest.mark.parametrize("T", [1, 16, 17, 64, 65, 200])
+def test_shared_expert_with_adapters_in_the_layer_call(T):
+    """mlxs_moe_experts_adapted with the routed rows weighted by zero: what is left is the shared expert with its adapters."""
+    H, I, E, k, n, R = 512, 256, 4, 2, 5, 24
+    m = pkg.MoE(pkg.make_config(H, I, E, k, bank_kind=pkg.BANK_MXFP4, act_limit=1.5, shared_expert=True, max_tokens=T))
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    logical, _ = m.record_bytes()
+    record = torch.zeros(logical, device="cuda", dtype=torch.uint8)
+    record[0::7] = 127                                        # finite codes and scales of any kind
+    for e in range(E):
+        m.load_expert(0, e, record.data_ptr(), logical, True)
+    rnd = lambda *s, std=1.0: (torch.randn(*s, device="cuda", generator=gen) * std).to(torch.bfloat16)  # noqa: E731
+    w1, w3, w2 = rnd(I, H, std=H ** -0.5), rnd(I, H, std=H ** -0.5), rnd(H, I, std=I ** -0.5)
+    m.set_shared(0, w1.data_ptr(), w3.data_ptr(), w2.data_ptr(), True)
+    ad = {"a1": rnd(n, R, H, std=H ** -0.5), "b1": rnd(n, I, R, std=0.2), "a3": rnd(n, R, H, std=H ** -0.5), "b3": rnd(n, I, R, std=0.2),
+          "a2": rnd(n, R, I, std=I ** -0.5), "b2": rnd(n, H, R, std=0.2)}
+    scales = torch.rand(n, device="cuda", generator=gen) + 0.5
+    ranks = torch.tensor([24, 8, 16, 24, 1], device="cuda", dtype=torch.int32)
+    x = rnd(T, H)
+    ids = torch.zeros(T, k, device="cuda", dtype=torch.int32)
+    ids[:, 1] = 1
+    weights = torch.zeros(T, k, device="cuda")
+    aid = torch.tensor(some_ids(T, n, "mixed", T), device="cuda", dtype=torch.int32)
+    st = torch.cuda.current_stream().cuda_stream
+    y, plain, none = (torch.empty(T, H, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+    full = pkg.make_shared_adapters(R, n, scales=scales.data_ptr(), ranks=ranks.data_ptr(), **{c: v.data_ptr() for c, v in ad.items()})
+    with pytest.raises(pkg.MlxsError) as ei:
+        m.experts_adapted(0, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, full, aid.data_ptr(), y.data_ptr(), st)
+    assert ei.value.rc == pkg.E_NOT_LOADED and "reserve_adapters" in ei.value.msg
+    m.reserve_adapters()
+    m.reserve_adapters()
+    m.experts_adapted(0, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, full, aid.data_ptr(), y.data_ptr(), st)
+    m.experts(0, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, plain.data_ptr(), st)
+    m.experts_adapted(0, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, pkg.make_shared_adapters(R, n), aid.data_ptr(), none.data_ptr(), st)
+    torch.cuda.synchronize()
+    assert m.stats().device_status == 0
+
+    def low_rank(v, a, b):
+        out = torch.zeros(T, b.shape[1], dtype=torch.float64, device="cuda")
+        for i in range(n):
+            at, r = (aid == i).nonzero().squeeze(1), int(ranks[i])
+            out[at] = float(scales[i]) * (v[at] @ a[i, :r].double().T @ b[i, :, :r].double().T)
+        return out
+    X = x.double()
+    for got, on in ((y, 1.0), (plain, 0.0), (none, 0.0)):
+        gate = X @ w1.double().T + on * low_rank(X, ad["a1"], ad["b1"])
+        up = X @ w3.double().T + on * low_rank(X, ad["a3"], ad["b3"])
+        gate, up = gate.clamp(max=1.5), up.clamp(-1.5, 1.5)
+        h = (gate * torch.sigmoid(gate) * up).to(torch.bfloat16).double()
+        want = h @ w2.double().T + on * low_rank(h, ad["a2"], ad["b2"])
+        # half a step of the output, and of some of h where the 32-bit sums lie next to a border (one in a hundred at most): under a whole step together
+        rel = float((got.double() - want).norm() / want.norm())
+        assert rel <= 2.0 ** -8 * 1.1, (T, on, rel)
+    assert float((y.double() - plain.double()).norm() / plain.double().norm()) > 0.05     # the adapters do something
+    bare = aid < 0
+    assert float((y[bare].double() - none[bare].double()).abs().max() if bare.any() else 0.0) == 0.0
