@@ -16,6 +16,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "tensor_map.cuh"
 #include "umma_pair.cuh"
 
 namespace mlxs {
@@ -364,12 +365,12 @@ struct AdShared {
 };
 
 // y = base for n tokens without an adapter: this CTA's outputs
-template <class O>
-__device__ __forceinline__ void ad_copy(const AdaptersArgs& a, const uint32_t* rows, uint32_t n_rows, uint32_t t0, uint32_t C, uint32_t rank) {
+template <class O, class Row>
+__device__ __forceinline__ void ad_copy(const AdaptersArgs& a, const Row* rows, uint32_t n_rows, uint32_t t0, uint32_t C, uint32_t rank, uint32_t tid, uint32_t n_threads) {
     if (a.base == a.y) return;
     const uint32_t c0 = (uint32_t)((uint64_t)rank * (a.N / 8) / C), c1 = (uint32_t)((uint64_t)(rank + 1) * (a.N / 8) / C), n = n_rows * (c1 - c0);
     constexpr uint32_t VEC = 16 / sizeof(O);
-    for (uint32_t i = threadIdx.x; i < n; i += AD_WARPS * 32) {
+    for (uint32_t i = tid; i < n; i += n_threads) {
         const size_t row = t0 + rows[i / (c1 - c0)], f = (size_t)(c0 + i % (c1 - c0)) * 8;
 #pragma unroll
         for (uint32_t v = 0; v < 8 / VEC; ++v) {
@@ -377,6 +378,61 @@ __device__ __forceinline__ void ad_copy(const AdaptersArgs& a, const uint32_t* r
             if (a.base) w = *reinterpret_cast<const uint4*>(static_cast<const O*>(a.base) + row * a.ld_base + f + v * VEC);
             *reinterpret_cast<uint4*>(static_cast<O*>(a.y) + row * a.ld_y + f + v * VEC) = w;
         }
+    }
+}
+
+// where the 16-bit parts of rank columns r, r + 1 (r even) of a token go
+struct AdParts {                         // rows of `pitch` bytes
+    uint32_t hi_, lo_, pitch;
+    __device__ uint32_t hi(uint32_t i, uint32_t r) const { return hi_ + i * pitch + r * 2; }
+    __device__ uint32_t lo(uint32_t i, uint32_t r) const { return lo_ + i * pitch + r * 2; }
+};
+// The CTAs' sums in order (part: f32 [tokens][r16], in every CTA at the same place), a warp to a token; the parts, and a power of two that the outputs
+// are multiplied by, go to every CTA.  Eight warps.
+template <class T, class Parts>
+__device__ __forceinline__ void ad_fold(const AdaptersArgs& a, uint32_t C, uint32_t rank, int32_t id, uint32_t R, uint32_t n_rows, uint32_t warp,
+                                        uint32_t part, uint32_t r16, uint32_t scales, const Parts& parts) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const float scale = a.scales ? a.scales[id] : 1.f;
+    for (uint32_t i = rank + C * warp; i < n_rows; i += C * AD_WARPS) {
+        float v[4][2];
+        float most = 0.f;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t r = j * 64 + lane * 2;
+            v[j][0] = v[j][1] = 0.f;
+            if (r >= R) continue;
+            const uint32_t at = part + (i * r16 + r) * 4;
+            float2 p[8];
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c)                 // all on their way before the first is added
+                if (c < C) p[c] = ad_ld_cluster2(map_to_rank(at, c));
+#pragma unroll
+            for (uint32_t c = 0; c < 8; ++c)
+                if (c < C) { v[j][0] += p[c].x; v[j][1] += p[c].y; }
+            v[j][0] *= scale;
+            v[j][1] = r + 1 < R ? v[j][1] * scale : 0.f;
+            most = fmaxf(most, fmaxf(fabsf(v[j][0]), fabsf(v[j][1])));
+        }
+        float down = 1.f, up = 1.f;
+        if (std::is_same<T, __half>::value) {
+            for (uint32_t o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+            // a power of two next to the row's largest: the parts lie in (-2, 2); rows of zeros, and of infinities, as they are
+            const uint32_t e = __float_as_uint(most) & 0x7F800000u;
+            if (e >= 0x00800000u && e <= 0x7E800000u) { up = __uint_as_float(e); down = __uint_as_float(0x7F000000u - e); }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t r = j * 64 + lane * 2;
+            if (r >= (R + 31) / 32 * 32) continue;                   // zeros behind the last rank column
+            uint32_t hi, lo;
+            ad_split<T>(v[j][0] * down, v[j][1] * down, hi, lo);
+            for (uint32_t c = 0; c < C; ++c) {
+                ad_st_cluster(map_to_rank(parts.hi(i, r), c), hi);
+                ad_st_cluster(map_to_rank(parts.lo(i, r), c), lo);
+            }
+        }
+        if (lane < C) ad_st_cluster(map_to_rank(scales + i * 4, lane), __float_as_uint(up));
     }
 }
 
@@ -438,47 +494,8 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
         __syncthreads();
     }
     cluster_sync_all();
-    // ---- the CTAs' sums in order, a warp to a token; the parts go to every CTA ----
-    for (uint32_t i = rank + C * warp; i < n_rows; i += C * AD_WARPS) {
-        const float scale = a.scales ? a.scales[id] : 1.f;
-        float v[4][2];
-        float most = 0.f;
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t r = j * 64 + lane * 2;
-            v[j][0] = v[j][1] = 0.f;
-            if (r >= R) continue;
-            const uint32_t at = base_s + L.part + (i * L.r16 + r) * 4;
-            for (uint32_t c = 0; c < C; ++c) {
-                const float2 p = ad_ld_cluster2(map_to_rank(at, c));
-                v[j][0] += p.x;
-                v[j][1] += p.y;
-            }
-            v[j][0] *= scale;
-            v[j][1] = r + 1 < R ? v[j][1] * scale : 0.f;
-            most = fmaxf(most, fmaxf(fabsf(v[j][0]), fabsf(v[j][1])));
-        }
-        float down = 1.f, up = 1.f;
-        if (std::is_same<T, __half>::value) {
-            for (uint32_t o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-            // a power of two next to the row's largest: the parts lie in (-2, 2); rows of zeros, and of infinities, as they are
-            const uint32_t e = __float_as_uint(most) & 0x7F800000u;
-            if (e >= 0x00800000u && e <= 0x7E800000u) { up = __uint_as_float(e); down = __uint_as_float(0x7F000000u - e); }
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t r = j * 64 + lane * 2;
-            if (r >= (R + 31) / 32 * 32) continue;                   // zeros behind the last rank column
-            uint32_t hi, lo;
-            ad_split<T>(v[j][0] * down, v[j][1] * down, hi, lo);
-            for (uint32_t c = 0; c < C; ++c) {
-                const uint32_t to = map_to_rank(base_s + L.u_hi + i * L.pitch + r * 2, c);
-                ad_st_cluster(to, hi);
-                ad_st_cluster(to + (L.u_lo - L.u_hi), lo);
-            }
-        }
-        if (lane < C) ad_st_cluster(map_to_rank(smem_u32(&sh.scale[i]), lane), __float_as_uint(up));
-    }
+    const AdParts parts{base_s + L.u_hi, base_s + L.u_lo, L.pitch};
+    ad_fold<T>(a, C, rank, id, R, n_rows, warp, base_s + L.part, L.r16, smem_u32(sh.scale), parts);
     cluster_sync_all();
     // ---- outer product: this CTA's outputs ----
     if (n_rows <= 16)
@@ -543,7 +560,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const A
     }
     __syncthreads();
     const uint32_t n_adapters = sh.n[0];
-    if (slot == 0) ad_copy<O>(a, sh.bare, sh.n[2], t0, C, rank);
+    if (slot == 0) ad_copy<O>(a, sh.bare, sh.n[2], t0, C, rank, tid, AD_WARPS * 32);
     for (uint32_t d = slot; d < n_adapters; d += slots) {
         const int32_t id = sh.adapter[d];
         if (warp == 0) {
@@ -569,26 +586,18 @@ struct AdSort {                          // dynamic shared memory behind AdSmem
     uint16_t cursor[AD_WARPS][AD_PLACES];
     uint16_t order[AD_SEG];
 };
-template <class T, class O>
-__global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const AdaptersArgs a, const uint32_t C, const uint32_t per_seg) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ AdShared sh;
-    __shared__ uint32_t s_scan[AD_WARPS];
-    const AdSmem L = ad_smem(a.R, a.T);
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = cluster_rank();
-    const uint32_t cl = blockIdx.x / C, seg = cl / per_seg, t0 = seg * AD_SEG, n_tok = min(AD_SEG, a.T - t0), n_places = a.n_adapters + 1;
-    AdSort& so = *reinterpret_cast<AdSort*>(smem + L.bytes);
-    uint32_t* const first = so.first;
-
+// `scratch`: 2 x AD_SEG x 2 bytes, free again afterwards.  All threads of the CTA (AD_WARPS warps or more; the first AD_WARPS work).
+__device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint16_t* scratch, uint32_t* s_scan, uint32_t t0, uint32_t n_tok, bool report) {
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     // a warp counts the places of its run of tokens, then the runs of a place follow one another
-    const uint32_t run_len = (n_tok + AD_WARPS * 32 - 1) / (AD_WARPS * 32) * 32, run0 = warp * run_len, run1 = min(run0 + run_len, n_tok);
-    for (uint32_t i = tid; i < AD_WARPS * AD_PLACES / 2; i += AD_WARPS * 32) reinterpret_cast<uint32_t*>(so.cursor)[i] = 0;
+    const uint32_t run_len = (n_tok + AD_WARPS * 32 - 1) / (AD_WARPS * 32) * 32, run0 = warp < AD_WARPS ? warp * run_len : n_tok, run1 = min(run0 + run_len, n_tok);
+    for (uint32_t i = tid; i < AD_WARPS * AD_PLACES / 2; i += blockDim.x) reinterpret_cast<uint32_t*>(so.cursor)[i] = 0;
     __syncthreads();
-    // a token's place, and its number among the run's tokens of that place (the operands' memory is free here)
-    uint16_t* const place_of = reinterpret_cast<uint16_t*>(smem);
+    // a token's place, and its number among the run's tokens of that place
+    uint16_t* const place_of = scratch;
     uint16_t* const number_of = place_of + AD_SEG;
 #pragma unroll 4
-    for (uint32_t i = run0 + lane; i < run1; i += 32) place_of[i] = (uint16_t)ad_place(a, t0 + i, cl % per_seg == 0 && rank == 0);
+    for (uint32_t i = run0 + lane; i < run1; i += 32) place_of[i] = (uint16_t)ad_place(a, t0 + i, report);
     __syncwarp();
 #pragma unroll 1
     for (uint32_t i = run0 + lane; i < run0 + run_len && i - lane < run1; i += 32) {
@@ -601,9 +610,9 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
         __syncwarp();
     }
     __syncthreads();
-    {
-        // two places to a thread: counts and units (64 tokens) summed side by side
-        uint32_t v[2], sum = 0;
+    // two places to a thread: counts and units (64 tokens) summed side by side
+    uint32_t v[2] = {0, 0}, sum = 0, run = 0;
+    if (warp < AD_WARPS) {
 #pragma unroll
         for (uint32_t j = 0; j < 2; ++j) {
             const uint32_t p = tid * 2 + j;
@@ -612,16 +621,18 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
             v[j] = n | ((n + AD_TT - 1) / AD_TT) << 16;
             sum += v[j];
         }
-        uint32_t run = sum;
+        run = sum;
         for (uint32_t o = 1; o < 32; o <<= 1) { const uint32_t w = __shfl_up_sync(0xFFFFFFFFu, run, o); if (lane >= o) run += w; }
         if (lane == 31) s_scan[warp] = run;
-        __syncthreads();
+    }
+    __syncthreads();
+    if (warp < AD_WARPS) {
         uint32_t at = run - sum;
         for (uint32_t w = 0; w < warp; ++w) at += s_scan[w];
 #pragma unroll
         for (uint32_t j = 0; j < 2; ++j) {
             const uint32_t p = tid * 2 + j;
-            first[p] = at;
+            so.first[p] = at;
             uint32_t pos = at & 0xFFFFu;
             for (uint32_t w = 0; w < AD_WARPS; ++w) {
                 const uint32_t n = so.cursor[w][p];
@@ -629,62 +640,402 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
                 pos += n;
             }
             at += v[j];
-            if (p == AD_PLACES - 1) first[AD_PLACES] = at;
+            if (p == AD_PLACES - 1) so.first[AD_PLACES] = at;
         }
     }
     __syncthreads();
     for (uint32_t i = run0 + lane; i < run1; i += 32) so.order[so.cursor[warp][place_of[i]] + number_of[i]] = (uint16_t)i;
     __syncthreads();
-    const uint32_t n_units = first[n_places] >> 16;
+}
+// unit u of the sorted segment: its place (n_adapters: no adapter), its tokens so.order[at .. at + rows), and the most tokens that a unit of its place has
+struct AdUnit { uint32_t place, at, rows, per; };
+__device__ __forceinline__ AdUnit ad_find(const AdSort& so, uint32_t n_places, uint32_t u) {
+    uint32_t lo = 0, hi = n_places;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (so.first[mid] >> 16 <= u) lo = mid; else hi = mid;
+    }
+    const uint32_t at = so.first[lo] & 0xFFFFu, n = (so.first[lo + 1] & 0xFFFFu) - at, n_chunks = (n + AD_TT - 1) / AD_TT;
+    AdUnit r;
+    r.place = lo;
+    r.per = (n + n_chunks - 1) / n_chunks;
+    const uint32_t c0 = (u - (so.first[lo] >> 16)) * r.per;
+    r.at = at + c0;
+    r.rows = min(r.per, n - c0);
+    return r;
+}
+
+template <class T, class O>
+__global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const AdaptersArgs a, const uint32_t C, const uint32_t per_seg) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ AdShared sh;
+    __shared__ uint32_t s_scan[AD_WARPS];
+    const AdSmem L = ad_smem(a.R, a.T);
+    const uint32_t tid = threadIdx.x, rank = cluster_rank();
+    const uint32_t cl = blockIdx.x / C, seg = cl / per_seg, t0 = seg * AD_SEG, n_tok = min(AD_SEG, a.T - t0), n_places = a.n_adapters + 1;
+    AdSort& so = *reinterpret_cast<AdSort*>(smem + L.bytes);
+    ad_sort(a, so, reinterpret_cast<uint16_t*>(smem), s_scan, t0, n_tok, cl % per_seg == 0 && rank == 0);
+    const uint32_t n_units = so.first[n_places] >> 16;
     for (uint32_t u = cl % per_seg; u < n_units; u += per_seg) {
-        // the place whose units hold u
-        uint32_t lo = 0, hi = n_places;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (first[mid] >> 16 <= u) lo = mid; else hi = mid;
-        }
-        const uint32_t at = first[lo] & 0xFFFFu, n = (first[lo + 1] & 0xFFFFu) - at, n_chunks = (n + AD_TT - 1) / AD_TT, per = (n + n_chunks - 1) / n_chunks;
-        const uint32_t c0 = (u - (first[lo] >> 16)) * per, n_rows = min(per, n - c0);
-        if (tid < n_rows) sh.rows[tid] = so.order[at + c0 + tid];
+        const AdUnit un = ad_find(so, n_places, u);
+        if (tid < un.rows) sh.rows[tid] = so.order[un.at + tid];
         __syncthreads();
-        if (lo == a.n_adapters) {
-            ad_copy<O>(a, sh.rows, n_rows, t0, C, rank);
+        if (un.place == a.n_adapters) {
+            ad_copy<O>(a, sh.rows, un.rows, t0, C, rank, tid, AD_WARPS * 32);
             __syncthreads();
         } else {
-            ad_unit<T, O>(a, L, smem, sh, C, rank, (int32_t)lo, n_rows, per <= 16 ? 1 : per <= 32 ? 2 : 4, t0);   // one split for all units of an adapter
+            ad_unit<T, O>(a, L, smem, sh, C, rank, (int32_t)un.place, un.rows, un.per <= 16 ? 1 : un.per <= 32 ? 2 : 4, t0);   // one split for all units of an adapter
         }
     }
 }
 
+// ------------------------------------------------------------------------------------------------------------
+// many tokens per adapter: the same cut, both products on the tensor cores
+// ------------------------------------------------------------------------------------------------------------
+// For units of 16 tokens and more mma.sync's operands, read from shared memory by every warp again, take longer than the bytes.  Here a
+// unit's inner product is D1[rank 128][tokens 64] = A x^T and its outer product, per block of 128 outputs, D2[outputs 128][tokens 64] = B u^T (both parts of u, one after
+// the other, into one accumulator): tcgen05.mma with M = 128, N = 64, accumulators in tensor memory.  A ring of stages: 64 inputs of A (a tensor-map copy)
+// and of the unit's x rows (asynchronous copies, eight lanes to a row), later 64 rank columns of a block of B (asynchronous copies, which zero what lies behind
+// the adapter's rank).  A warp to a ring slot, one that issues the products, eight that read accumulators: inner sums -> shared memory -> the cluster's fold ->
+// parts of u as operand rows; outputs -> turned through shared memory -> + base -> y.  The fold's steps are joined by mbarriers between the CTAs, so the
+// ring runs on underneath.  Every wait is bounded: a give-up sets the status word, and everybody still meets at the end.
+constexpr uint32_t AB_SLOTS = 5, AB_MAX_R = 128, AB_MIN_ROWS = 16;   // from so many tokens per unit on
+constexpr uint32_t AB_A_BYTES = 128 * 128, AB_X_BYTES = 64 * 128, AB_SLOT = AB_A_BYTES + AB_X_BYTES;
+constexpr uint32_t AB_U_BYTES = 64 * 128;                            // one part of 64 rank columns of the unit's tokens
+constexpr uint32_t AB_TURN = 16 * 32 * 4;                            // an epilogue warp's turn of 16 tokens x 32 outputs
+constexpr uint32_t AB_THREADS = (1 + AD_WARPS + AB_SLOTS) * 32;
+struct AbSmem { uint32_t u, part, turn, sort, bytes; };              // behind the ring, offsets from its 1024-byte boundary
+__host__ __device__ inline AbSmem ab_smem(uint32_t R) {
+    AbSmem s;
+    const uint32_t chunks = (R + 63) / 64;
+    s.u = AB_SLOTS * AB_SLOT;
+    s.part = s.u + chunks * 2 * AB_U_BYTES;
+    s.turn = s.part + (R + 15) / 16 * 16 * 64 * 4;
+    s.sort = s.turn + AD_WARPS * AB_TURN;
+    s.bytes = s.sort + (uint32_t)sizeof(AdSort) + 1024;
+    return s;
+}
+// operand rows of 64 rank columns, 128 bytes, 16-byte chunks swizzled by the row: [64-column chunk][part][64 tokens]
+struct AbParts {
+    uint32_t u;
+    __device__ uint32_t at(uint32_t i, uint32_t r) const { return u + (r >> 6) * (2 * AB_U_BYTES) + i * 128 + ((((r & 63u) >> 3) ^ (i & 7u)) << 4) + (r & 7u) * 2; }
+    __device__ uint32_t hi(uint32_t i, uint32_t r) const { return at(i, r); }
+    __device__ uint32_t lo(uint32_t i, uint32_t r) const { return at(i, r) + AB_U_BYTES; }
+};
+struct AbParams {
+    CUtensorMap a;                       // [n_adapters][R][K], boxes of R rows x 64 inputs
+    AdaptersArgs p;
+    uint32_t C, per_seg;
+};
+__device__ __forceinline__ void ab_tma_3d(uint32_t dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(c0),
+                 "r"(c1), "r"(c2), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void ab_expect(uint32_t bar, uint32_t bytes) {   // bytes to wait for, no arrival
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// the first n bytes of 16, zeros behind
+__device__ __forceinline__ void ab_copy(uint32_t dst, const void* src, uint32_t n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+template <class O> struct AbBase;        // four outputs of base
+template <> struct AbBase<float> { typedef uint4 Word; };
+template <> struct AbBase<__nv_bfloat16> { typedef uint2 Word; };
+template <> struct AbBase<__half> { typedef uint2 Word; };
+
+template <class T, class O>
+__global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __grid_constant__ AbParams P) {
+    extern __shared__ uint8_t smem_any[];
+    __shared__ __align__(8) uint64_t full_bar[AB_SLOTS], empty_bar[AB_SLOTS], d1_full, d1_empty, d2_full[2], d2_empty[2], part_ready, u_ready, u_go;
+    __shared__ uint32_t s_tmem, s_scan[AD_WARPS];
+    __shared__ float s_scale[AD_TT];
+    __shared__ volatile int s_abort;
+    const AdaptersArgs& a = P.p;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = cluster_rank(), C = P.C;
+    const uint32_t ring = (smem_u32(smem_any) + 1023u) & ~1023u;
+    uint8_t* const ring_p = smem_any + (ring - smem_u32(smem_any));
+    const AbSmem L = ab_smem(a.R);
+    const uint32_t cl = blockIdx.x / C, seg = cl / P.per_seg, t0 = seg * AD_SEG, n_tok = min(AD_SEG, a.T - t0), n_places = a.n_adapters + 1;
+    AdSort& so = *reinterpret_cast<AdSort*>(ring_p + L.sort);
+    if (tid == 0) {
+        for (uint32_t s = 0; s < AB_SLOTS; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        mbar_init(&d1_full, 1); mbar_init(&d1_empty, AD_WARPS);
+        for (int b = 0; b < 2; ++b) { mbar_init(&d2_full[b], 1); mbar_init(&d2_empty[b], AD_WARPS); }
+        mbar_init(&part_ready, C); mbar_init(&u_ready, C); mbar_init(&u_go, 1);
+        s_abort = 0;
+        mbar_fence_init();
+        tma_prefetch_map(&P.a);
+    }
+    if (warp == AD_WARPS) tmem_alloc(&s_tmem, 256);                   // the issuer's warp
+    ad_sort(a, so, reinterpret_cast<uint16_t*>(ring_p), s_scan, t0, n_tok, cl % P.per_seg == 0 && rank == 0);
+    fence_async_smem();                                               // the sort's scratch was where copies land
+    tc_fence_before();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem, n_units = so.first[n_places] >> 16;
+    const uint32_t n_ks = (a.K + 63) / 64, ks0 = rank * n_ks / C, ks1 = (rank + 1) * n_ks / C;
+    const uint32_t n_fb = (a.N + 127) / 128, fb0 = rank * n_fb / C, fb1 = (rank + 1) * n_fb / C;
+    auto give_up = [&](uint32_t code) { if (!s_abort) atomicMax(a.status, code); s_abort = 1; };
+    auto rank_of = [&](uint32_t place) {
+        const int32_t given = a.ranks ? a.ranks[place] : (int32_t)a.R;
+        return given < 0 ? 0u : min((uint32_t)given, a.R);
+    };
+
+    if (warp > AD_WARPS) {
+        // ---------------- a ring slot's warp: every AB_SLOTS-th stage ----------------
+        const uint32_t slot = warp - AD_WARPS - 1, full = smem_u32(&full_bar[slot]), empty = smem_u32(&empty_bar[slot]), at = ring + slot * AB_SLOT;
+        const uint32_t chunk = lane & 7u, row0 = lane >> 3;
+        uint32_t ph = 0, base = 0;                                    // stages of the units before, modulo the ring
+        bool ok = true;
+        for (uint32_t u = cl % P.per_seg; u < n_units && ok; u += P.per_seg) {
+            const AdUnit un = ad_find(so, n_places, u);
+            if (un.place == a.n_adapters) continue;
+            const uint32_t R = rank_of(un.place), chunks = (R + 63) / 64, n_in = R ? ks1 - ks0 : 0, n_st = n_in + (fb1 - fb0) * chunks;
+            const T* const B = static_cast<const T*>(a.b) + (size_t)un.place * a.b_stride;
+            for (uint32_t st = (slot + AB_SLOTS - base) % AB_SLOTS; st < n_st; st += AB_SLOTS) {
+                if (!mbar_wait_warp_at(empty, ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
+                if (st < n_in) {
+                    const uint32_t k = (ks0 + st) * 64;
+                    if (lane == 0) {
+                        ab_expect(full, a.R * 128);
+                        ab_tma_3d(at, &P.a, (int32_t)k, 0, (int32_t)un.place, full);
+                    }
+                    const bool in = k + chunk * 8 < a.K;
+                    const T* x = static_cast<const T*>(a.x) + (in ? k + chunk * 8 : 0);
+#pragma unroll 4
+                    for (uint32_t r = row0; r < un.rows; r += 4)
+                        ab_copy(at + AB_A_BYTES + r * 128 + ((chunk ^ (r & 7u)) << 4), x + (size_t)(t0 + so.order[un.at + r]) * a.ld_x, in ? 16 : 0);
+                } else {
+                    const uint32_t i = st - n_in, f0 = (fb0 + i / chunks) * 128, r = (i % chunks) * 64 + chunk * 8;
+                    const uint32_t n = r >= R ? 0 : R - r < 8 ? (R - r) * 2 : 16;       // bytes of this lane's eight rank columns that count
+                    const T* b = B + (n ? r : 0);
+                    const uint32_t n_f = min(a.N - f0, 128u);
+#pragma unroll 4
+                    for (uint32_t f = row0; f < n_f; f += 4) ab_copy(at + f * 128 + ((chunk ^ (f & 7u)) << 4), b + (size_t)(f0 + f) * a.R, n);
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(full);
+                ph ^= 1u;
+            }
+            base = (base + n_st) % AB_SLOTS;
+        }
+        if (s_abort) for (int i = 0; i < 2000; ++i) __nanosleep(1000);   // copies in flight land before the memory goes
+    } else if (warp == AD_WARPS) {
+        // ---------------- issuer ----------------
+        const uint32_t fmt = std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16, idesc = umma_idesc(fmt, 64);
+        uint32_t s = 0, ph = 0, n_done = 0, n_blocks = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+            if (!ok) return;
+            ok = mbar_wait_warp(bar, parity, &s_abort);
+            if (!ok) give_up(code);
+            tc_fence_after();
+        };
+        auto next = [&]() { if (++s == AB_SLOTS) { s = 0; ph ^= 1u; } };
+        for (uint32_t u = cl % P.per_seg; u < n_units && ok; u += P.per_seg) {
+            const AdUnit un = ad_find(so, n_places, u);
+            if (un.place == a.n_adapters) continue;
+            const uint32_t R = rank_of(un.place), chunks = (R + 63) / 64;
+            if (R) {
+                wait(&d1_empty, (n_done & 1u) ^ 1u, ST_WAIT_EMPTY);
+                for (uint32_t ks = ks0; ks < ks1 && ok; ++ks) {
+                    wait(&full_bar[s], ph, ST_WAIT_FULL);
+                    if (!ok) break;
+                    const uint32_t at = ring + s * AB_SLOT;
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j)
+                            umma_f16(tmem, umma_desc_sw128(at + j * 32, 16, 1024), umma_desc_sw128(at + AB_A_BYTES + j * 32, 16, 1024), idesc, ks != ks0 || j ? 1u : 0u);
+                        umma_commit(&empty_bar[s]);
+                    }
+                    __syncwarp();
+                    next();
+                }
+                if (!ok) break;
+                if (elect_one()) umma_commit(&d1_full);
+                __syncwarp();
+            }
+            // the parts of u are there (a unit without a rank has none: its outputs are base)
+            if (R) wait(&u_go, n_done & 1u, ST_WAIT_FULL);
+            for (uint32_t fb = fb0; fb < fb1 && ok && R; ++fb, ++n_blocks) {
+                const uint32_t buf = n_blocks & 1u, acc = tmem + 64 + buf * 64;
+                wait(&d2_empty[buf], (n_blocks >> 1 & 1u) ^ 1u, ST_WAIT_EMPTY);
+                for (uint32_t c = 0; c < chunks && ok; ++c) {
+                    wait(&full_bar[s], ph, ST_WAIT_FULL);
+                    if (!ok) break;
+                    const uint32_t at = ring + s * AB_SLOT, ua = ring + L.u + c * 2 * AB_U_BYTES, steps = (min(R - c * 64, 64u) + 15) / 16;
+                    if (elect_one()) {
+                        for (uint32_t part = 0; part < 2; ++part)
+                            for (uint32_t j = 0; j < steps; ++j)
+                                umma_f16(acc, umma_desc_sw128(at + j * 32, 16, 1024), umma_desc_sw128(ua + part * AB_U_BYTES + j * 32, 16, 1024), idesc, c | part | j ? 1u : 0u);
+                        umma_commit(&empty_bar[s]);
+                    }
+                    __syncwarp();
+                    next();
+                }
+                if (!ok) break;
+                if (elect_one()) umma_commit(&d2_full[buf]);
+                __syncwarp();
+            }
+            if (R) ++n_done;
+        }
+    } else {
+        // ---------------- accumulators: warp = (lanes 32 q .. 32 q + 31, tokens 32 half .. 32 half + 31) ----------------
+        const uint32_t q = warp & 3u, half = warp >> 2, etid = tid;   // warps 0 .. 7
+        float* const part = reinterpret_cast<float*>(ring_p + L.part);
+        const uint32_t r16 = (a.R + 15) / 16 * 16, turn = ring + L.turn + warp * AB_TURN;
+        const AbParts parts{ring + L.u};
+        uint32_t n_done = 0, n_blocks = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(bar), parity, &s_abort));
+            if (!ok) give_up(ST_WAIT_FULL);
+            return ok;
+        };
+        // all eight warps go on, or give up, together: they meet at named barriers
+        auto together = [&]() {
+            uint32_t r;
+            asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred r, 1, 256, p;\n\tselp.u32 %0, 1, 0, r;\n\t}" : "=r"(r) : "r"((uint32_t)ok) : "memory");
+            ok = r != 0;
+            return ok;
+        };
+        for (uint32_t u = cl % P.per_seg; u < n_units && ok; u += P.per_seg) {
+            const AdUnit un = ad_find(so, n_places, u);
+            if (un.place == a.n_adapters) { ad_copy<O>(a, so.order + un.at, un.rows, t0, C, rank, etid, AD_WARPS * 32); continue; }
+            const uint32_t R = rank_of(un.place);
+            if (!R) {   // outputs are base
+                ad_copy<O>(a, so.order + un.at, un.rows, t0, C, rank, etid, AD_WARPS * 32);
+                continue;
+            }
+            // inner sums of this CTA's inputs
+            wait(&d1_full, n_done & 1u);
+            tc_fence_after();
+            if (ok && q * 32 < R)
+                for (uint32_t c = half * 32; c < half * 32 + 32 && c < un.rows; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(tmem + c + ((q * 32u) << 16), v);
+                    if (q * 32 + lane < r16)
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; ++j) part[(c + j) * r16 + q * 32 + lane] = __uint_as_float(v[j]);
+                }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&d1_empty);
+            if (!together()) break;
+            if (etid < C) mbar_arrive_cluster(map_to_rank(smem_u32(&part_ready), etid));
+            wait(&part_ready, n_done & 1u);
+            if (!together()) break;
+            ad_fold<T>(a, C, rank, (int32_t)un.place, R, un.rows, warp, ring + L.part, r16, smem_u32(s_scale), parts);
+            together();
+            if (etid < C) mbar_arrive_cluster(map_to_rank(smem_u32(&u_ready), etid));
+            wait(&u_ready, n_done & 1u);
+            fence_async_smem();
+            if (!together()) break;
+            if (etid == 0) mbar_arrive(&u_go);
+            ++n_done;
+            // outputs: a lane four of a token, eight lanes a token's 32, a warp four tokens at a time
+            const uint32_t i0 = half * 32 + (lane >> 3), f4 = q * 32 + (lane & 7u) * 4;
+            for (uint32_t fb = fb0; fb < fb1 && ok; ++fb, ++n_blocks) {
+                const uint32_t buf = n_blocks & 1u, f = fb * 128 + f4;
+                typename AbBase<O>::Word b[2][4] = {};
+                const bool in = f < a.N;
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t i = i0 + h * 16 + j * 4;
+                        if (a.base && in && i < un.rows)
+                            b[h][j] = *reinterpret_cast<const typename AbBase<O>::Word*>(static_cast<const O*>(a.base) + (size_t)(t0 + so.order[un.at + i]) * a.ld_base + f);
+                    }
+                if (!wait(&d2_full[buf], n_blocks >> 1 & 1u)) break;
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    if (half * 32 + h * 16 >= un.rows) break;
+                    uint32_t v[16];
+                    tmem_ld16(tmem + 64 + buf * 64 + half * 32 + h * 16 + ((q * 32u) << 16), v);
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; ++j) asm volatile("st.shared.u32 [%0], %1;" ::"r"(turn + (j * 32 + lane) * 4), "r"(v[j]) : "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t i = i0 + h * 16 + j * 4;
+                        const uint4 w = ad_lds16(turn + ((lane >> 3) + j * 4) * 128 + (lane & 7u) * 16);
+                        if (!in || i >= un.rows) continue;
+                        const float s = std::is_same<T, __half>::value ? s_scale[i] : 1.f;
+                        O* y = static_cast<O*>(a.y) + (size_t)(t0 + so.order[un.at + i]) * a.ld_y + f;
+                        if constexpr (sizeof(O) == 4) {
+                            const uint4 c = b[h][j];
+                            *reinterpret_cast<float4*>(y) = make_float4(fmaf(__uint_as_float(w.x), s, __uint_as_float(c.x)), fmaf(__uint_as_float(w.y), s, __uint_as_float(c.y)),
+                                                                       fmaf(__uint_as_float(w.z), s, __uint_as_float(c.z)), fmaf(__uint_as_float(w.w), s, __uint_as_float(c.w)));
+                        } else {
+                            const float2 c0 = ad_unpack(b[h][j].x, O()), c1 = ad_unpack(b[h][j].y, O());
+                            *reinterpret_cast<uint2*>(y) = make_uint2(ad_pack(fmaf(__uint_as_float(w.x), s, c0.x), fmaf(__uint_as_float(w.y), s, c0.y), O()),
+                                                                     ad_pack(fmaf(__uint_as_float(w.z), s, c1.x), fmaf(__uint_as_float(w.w), s, c1.y), O()));
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d2_empty[buf]);
+            }
+            together();
+        }
+    }
+    // every thread comes here, also after a give-up
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync_all();
+    tc_fence_after();
+    if (warp == AD_WARPS) tmem_free(tmem, 256);
+}
+
 template <class... Params, class... Args>
-static cudaError_t ad_launch(void (*kernel)(Params...), uint32_t C, uint32_t clusters, size_t smem, cudaStream_t st, Args... args) {
+static cudaError_t ad_launch(void (*kernel)(Params...), uint32_t C, uint32_t clusters, uint32_t threads, size_t smem, cudaStream_t st, const Args&... args) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = C; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(C * clusters); cfg.blockDim = dim3(AD_WARPS * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = &attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+    cfg.gridDim = dim3(C * clusters); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = &attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 template <class T, class O>
 static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     const AdSmem L = ad_smem(a.R, a.T);
-    const uint32_t room = 2 * (uint32_t)a.sm_count;                // CTAs that run at once
+    const uint32_t sms = (uint32_t)a.sm_count, room = 2 * sms;     // CTAs of the mma.sync kernels that run at once
+    // a cluster is as large as the units leave SMs for
+    const auto spread = [](uint64_t units, uint32_t ctas, uint32_t least) { uint32_t C = 8; while (C > least && units * C > ctas) C /= 2; return C; };
     if (a.T <= AD_TT || a.n_adapters >= AD_PLACES) {
         const uint32_t tiles = (a.T + AD_TT - 1) / AD_TT, most = a.T < a.n_adapters ? a.T : a.n_adapters, distinct = most < AD_TT ? most : AD_TT;
-        const uint64_t units = (uint64_t)tiles * distinct;         // at most
-        const uint32_t C = units * 16 <= room * 3 ? 8 : units * 8 <= room * 3 ? 4 : 2;
+        const uint32_t C = spread((uint64_t)tiles * distinct, room, 2);
         uint32_t slots = room / (C * tiles);
         slots = slots < 1 ? 1 : slots > distinct ? distinct : slots;
-        return ad_launch(adapters_tile_kernel<T, O>, C, slots * tiles, L.bytes, st, a, C, slots);
+        return ad_launch(adapters_tile_kernel<T, O>, C, slots * tiles, AD_WARPS * 32, L.bytes, st, a, C, slots);
     }
     const uint32_t segs = (a.T + AD_SEG - 1) / AD_SEG, tokens = a.T < AD_SEG ? a.T : AD_SEG;
-    const uint32_t units = tokens / AD_TT + (a.n_adapters < tokens ? a.n_adapters : tokens);   // of a segment, at most
-    const uint32_t C = (uint64_t)units * segs * 16 <= room * 3 ? 8 : (uint64_t)units * segs * 8 <= room * 3 ? 4 : 2;
+    // a segment's units: about as many as it has adapters, or 64 tokens
+    const uint32_t units = tokens / AD_TT > a.n_adapters ? tokens / AD_TT : a.n_adapters < tokens ? a.n_adapters : tokens;
+    if (a.R <= AB_MAX_R && tokens >= AB_MIN_ROWS * units) {
+        AbParams P;
+        P.p = a;
+        cudaError_t e = encode_map<3>(&P.a, a.dtype, a.a, {a.K, a.R, a.n_adapters}, {a.K, a.a_stride}, {64, a.R, 1});
+        if (e != cudaSuccess) return e;
+        P.C = spread((uint64_t)units * segs, sms, 1);
+        while (P.C > (a.K + 63) / 64) P.C /= 2;                     // every CTA has inputs to sum
+        P.per_seg = sms / (P.C * segs);
+        P.per_seg = P.per_seg < 1 ? 1 : P.per_seg > units + tokens / AD_TT + 1 ? units + tokens / AD_TT + 1 : P.per_seg;
+        return ad_launch(adapters_tensor_kernel<T, O>, P.C, P.per_seg * segs, AB_THREADS, ab_smem(a.R).bytes, st, P);
+    }
+    const uint32_t C = spread((uint64_t)units * segs, room, 2);
     uint32_t per_seg = room / (C * segs);
-    per_seg = per_seg < 1 ? 1 : per_seg > units ? units : per_seg;
-    return ad_launch(adapters_sorted_kernel<T, O>, C, per_seg * segs, L.bytes + sizeof(AdSort), st, a, C, per_seg);
+    per_seg = per_seg < 1 ? 1 : per_seg > units + tokens / AD_TT + 1 ? units + tokens / AD_TT + 1 : per_seg;
+    return ad_launch(adapters_sorted_kernel<T, O>, C, per_seg * segs, AD_WARPS * 32, L.bytes + sizeof(AdSort), st, a, C, per_seg);
 }
 cudaError_t launch_adapters(const AdaptersArgs& a, cudaStream_t st) {
     if (a.dtype == DT_BF16) return a.out_dtype == DT_F32 ? adapters_launch<__nv_bfloat16, float>(a, st) : adapters_launch<__nv_bfloat16, __nv_bfloat16>(a, st);

@@ -389,6 +389,18 @@ def test_adapters_many_tokens_and_many_adapters(moe, n, T, kind):
     c.check()
 
 
+@pytest.mark.parametrize("R", [8, 16, 40, 64, 72, 128])
+@pytest.mark.parametrize("K, N", [(8, 8), (72, 264), (1032, 1400), (2304, 512)])
+@pytest.mark.parametrize("T, n", [(66, 1), (500, 7), (5000, 5)])
+def test_adapters_many_tokens_each(moe, T, n, R, K, N):
+    """Units of 16 tokens and more: both products on the tensor cores."""
+    for dtype, out, kind in (("bf16", "bf16", "runs"), ("f16", "f32", "mixed")):
+        ranks = None if dtype == "bf16" else [max(1, R - 3 * i) for i in range(n)]
+        c = Adapters(some_ids(T, n, kind), n, R, K, N, dtype, out, ranks=ranks, pad=8, in_place=dtype == "f16")
+        c.call(moe)
+        c.check((dtype, out))
+
+
 @pytest.mark.parametrize("R", [8, 16, 24, 64, 72, 128, 200, 256])
 @pytest.mark.parametrize("K, N", [(8, 8), (72, 264), (1032, 1400), (2304, 512)])
 def test_adapters_widths(moe, R, K, N):
