@@ -364,19 +364,25 @@ struct AdShared {
     float scale[AD_TT];
 };
 
-// y = base for n tokens without an adapter: this CTA's outputs
+// y = base for n tokens without an adapter: this CTA's outputs, a warp to a row
 template <class O, class Row>
-__device__ __forceinline__ void ad_copy(const AdaptersArgs& a, const Row* rows, uint32_t n_rows, uint32_t t0, uint32_t C, uint32_t rank, uint32_t tid, uint32_t n_threads) {
+__device__ __forceinline__ void ad_copy(const AdaptersArgs& a, const Row* rows, uint32_t n_rows, uint32_t t0, uint32_t C, uint32_t rank) {
     if (a.base == a.y) return;
-    const uint32_t c0 = (uint32_t)((uint64_t)rank * (a.N / 8) / C), c1 = (uint32_t)((uint64_t)(rank + 1) * (a.N / 8) / C), n = n_rows * (c1 - c0);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     constexpr uint32_t VEC = 16 / sizeof(O);
-    for (uint32_t i = tid; i < n; i += n_threads) {
-        const size_t row = t0 + rows[i / (c1 - c0)], f = (size_t)(c0 + i % (c1 - c0)) * 8;
+    const uint32_t c0 = (uint32_t)((uint64_t)rank * (a.N / 8) / C) * (8 / VEC), c1 = (uint32_t)((uint64_t)(rank + 1) * (a.N / 8) / C) * (8 / VEC);   // 16-byte words
+    for (uint32_t i = warp; i < n_rows; i += AD_WARPS) {
+        const size_t row = t0 + rows[i];
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const O*>(a.base) + row * a.ld_base);
+        uint4* to = reinterpret_cast<uint4*>(static_cast<O*>(a.y) + row * a.ld_y);
+        for (uint32_t c = c0 + lane; c < c1; c += 128) {
+            uint4 w[4] = {};
 #pragma unroll
-        for (uint32_t v = 0; v < 8 / VEC; ++v) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (a.base) w = *reinterpret_cast<const uint4*>(static_cast<const O*>(a.base) + row * a.ld_base + f + v * VEC);
-            *reinterpret_cast<uint4*>(static_cast<O*>(a.y) + row * a.ld_y + f + v * VEC) = w;
+            for (uint32_t k = 0; k < 4; ++k)
+                if (a.base && c + k * 32 < c1) w[k] = from[c + k * 32];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (c + k * 32 < c1) to[c + k * 32] = w[k];
         }
     }
 }
@@ -389,50 +395,60 @@ struct AdParts {                         // rows of `pitch` bytes
 };
 // The CTAs' sums in order (part: f32 [tokens][r16], in every CTA at the same place), a warp to a token; the parts, and a power of two that the outputs
 // are multiplied by, go to every CTA.  Eight warps.
-template <class T, class Parts>
+// NJ: 64 rank columns at most, NI: tokens of a warp whose reads are under way together.
+template <class T, int NJ, int NI, class Parts>
 __device__ __forceinline__ void ad_fold(const AdaptersArgs& a, uint32_t C, uint32_t rank, int32_t id, uint32_t R, uint32_t n_rows, uint32_t warp,
                                         uint32_t part, uint32_t r16, uint32_t scales, const Parts& parts) {
-    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t lane = threadIdx.x & 31u, step = C * AD_WARPS;
     const float scale = a.scales ? a.scales[id] : 1.f;
-    for (uint32_t i = rank + C * warp; i < n_rows; i += C * AD_WARPS) {
-        float v[4][2];
-        float most = 0.f;
+    for (uint32_t i0 = rank + C * warp; i0 < n_rows; i0 += NI * step) {
+        float v[NI][NJ][2] = {};
+        for (uint32_t c = 0; c < C; ++c) {
+            float2 p[NI][NJ];
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t r = j * 64 + lane * 2;
-            v[j][0] = v[j][1] = 0.f;
-            if (r >= R) continue;
-            const uint32_t at = part + (i * r16 + r) * 4;
-            float2 p[8];
+            for (int n = 0; n < NI; ++n)
 #pragma unroll
-            for (uint32_t c = 0; c < 8; ++c)                 // all on their way before the first is added
-                if (c < C) p[c] = ad_ld_cluster2(map_to_rank(at, c));
+                for (int j = 0; j < NJ; ++j) {
+                    const uint32_t r = j * 64 + lane * 2, i = i0 + n * step;
+                    p[n][j] = make_float2(0.f, 0.f);
+                    if (r < R && i < n_rows) p[n][j] = ad_ld_cluster2(map_to_rank(part + (i * r16 + r) * 4, c));
+                }
 #pragma unroll
-            for (uint32_t c = 0; c < 8; ++c)
-                if (c < C) { v[j][0] += p[c].x; v[j][1] += p[c].y; }
-            v[j][0] *= scale;
-            v[j][1] = r + 1 < R ? v[j][1] * scale : 0.f;
-            most = fmaxf(most, fmaxf(fabsf(v[j][0]), fabsf(v[j][1])));
-        }
-        float down = 1.f, up = 1.f;
-        if (std::is_same<T, __half>::value) {
-            for (uint32_t o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-            // a power of two next to the row's largest: the parts lie in (-2, 2); rows of zeros, and of infinities, as they are
-            const uint32_t e = __float_as_uint(most) & 0x7F800000u;
-            if (e >= 0x00800000u && e <= 0x7E800000u) { up = __uint_as_float(e); down = __uint_as_float(0x7F000000u - e); }
+            for (int n = 0; n < NI; ++n)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) { v[n][j][0] += p[n][j].x; v[n][j][1] += p[n][j].y; }
         }
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t r = j * 64 + lane * 2;
-            if (r >= (R + 31) / 32 * 32) continue;                   // zeros behind the last rank column
-            uint32_t hi, lo;
-            ad_split<T>(v[j][0] * down, v[j][1] * down, hi, lo);
-            for (uint32_t c = 0; c < C; ++c) {
-                ad_st_cluster(map_to_rank(parts.hi(i, r), c), hi);
-                ad_st_cluster(map_to_rank(parts.lo(i, r), c), lo);
+        for (int n = 0; n < NI; ++n) {
+            const uint32_t i = i0 + n * step;
+            if (i >= n_rows) break;
+            float most = 0.f, down = 1.f, up = 1.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t r = j * 64 + lane * 2;
+                v[n][j][0] *= scale;
+                v[n][j][1] = r + 1 < R ? v[n][j][1] * scale : 0.f;
+                most = fmaxf(most, fmaxf(fabsf(v[n][j][0]), fabsf(v[n][j][1])));
             }
+            if (std::is_same<T, __half>::value) {
+                for (uint32_t o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+                // a power of two next to the row's largest: the parts lie in (-2, 2); rows of zeros, and of infinities, as they are
+                const uint32_t e = __float_as_uint(most) & 0x7F800000u;
+                if (e >= 0x00800000u && e <= 0x7E800000u) { up = __uint_as_float(e); down = __uint_as_float(0x7F000000u - e); }
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t r = j * 64 + lane * 2;
+                if (r >= (R + 31) / 32 * 32) continue;               // zeros behind the last rank column
+                uint32_t hi, lo;
+                ad_split<T>(v[n][j][0] * down, v[n][j][1] * down, hi, lo);
+                for (uint32_t c = 0; c < C; ++c) {
+                    ad_st_cluster(map_to_rank(parts.hi(i, r), c), hi);
+                    ad_st_cluster(map_to_rank(parts.lo(i, r), c), lo);
+                }
+            }
+            if (std::is_same<T, __half>::value && lane < C) ad_st_cluster(map_to_rank(scales + i * 4, lane), __float_as_uint(up));
         }
-        if (lane < C) ad_st_cluster(map_to_rank(scales + i * 4, lane), __float_as_uint(up));
     }
 }
 
@@ -495,7 +511,7 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
     }
     cluster_sync_all();
     const AdParts parts{base_s + L.u_hi, base_s + L.u_lo, L.pitch};
-    ad_fold<T>(a, C, rank, id, R, n_rows, warp, base_s + L.part, L.r16, smem_u32(sh.scale), parts);
+    ad_fold<T, 4, 1>(a, C, rank, id, R, n_rows, warp, base_s + L.part, L.r16, smem_u32(sh.scale), parts);
     cluster_sync_all();
     // ---- outer product: this CTA's outputs ----
     if (n_rows <= 16)
@@ -560,7 +576,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const A
     }
     __syncthreads();
     const uint32_t n_adapters = sh.n[0];
-    if (slot == 0) ad_copy<O>(a, sh.bare, sh.n[2], t0, C, rank, tid, AD_WARPS * 32);
+    if (slot == 0) ad_copy<O>(a, sh.bare, sh.n[2], t0, C, rank);
     for (uint32_t d = slot; d < n_adapters; d += slots) {
         const int32_t id = sh.adapter[d];
         if (warp == 0) {
@@ -586,6 +602,16 @@ struct AdSort {                          // dynamic shared memory behind AdSmem
     uint16_t cursor[AD_WARPS][AD_PLACES];
     uint16_t order[AD_SEG];
 };
+// the lanes that hold the same place, by one ballot per bit of the largest (a match of whole words took 700 cycles)
+__device__ __forceinline__ uint32_t ad_same(uint32_t place, uint32_t bits, bool in) {
+    uint32_t same = __ballot_sync(0xFFFFFFFFu, in);
+    for (uint32_t b = 0; b < bits; ++b) {
+        const bool one = place >> b & 1u;
+        const uint32_t m = __ballot_sync(0xFFFFFFFFu, one);
+        same &= one ? m : ~m;
+    }
+    return same;
+}
 // `scratch`: 2 x AD_SEG x 2 bytes, free again afterwards.  All threads of the CTA (AD_WARPS warps or more; the first AD_WARPS work).
 __device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint16_t* scratch, uint32_t* s_scan, uint32_t t0, uint32_t n_tok, bool report) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -596,13 +622,14 @@ __device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint1
     // a token's place, and its number among the run's tokens of that place
     uint16_t* const place_of = scratch;
     uint16_t* const number_of = place_of + AD_SEG;
+    const uint32_t bits = 32 - __clz(a.n_adapters);
 #pragma unroll 4
     for (uint32_t i = run0 + lane; i < run1; i += 32) place_of[i] = (uint16_t)ad_place(a, t0 + i, report);
     __syncwarp();
 #pragma unroll 1
     for (uint32_t i = run0 + lane; i < run0 + run_len && i - lane < run1; i += 32) {
         const bool in = i < run1;
-        const uint32_t place = in ? place_of[i] : 0xFFFFu, same = __match_any_sync(0xFFFFFFFFu, place), before = __popc(same & ((1u << lane) - 1));
+        const uint32_t place = in ? place_of[i] : 0u, same = ad_same(place, bits, in), before = __popc(same & ((1u << lane) - 1));
         const uint32_t at = in ? so.cursor[warp][place] : 0;
         __syncwarp();
         if (in) number_of[i] = (uint16_t)(at + before);
@@ -681,7 +708,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
         if (tid < un.rows) sh.rows[tid] = so.order[un.at + tid];
         __syncthreads();
         if (un.place == a.n_adapters) {
-            ad_copy<O>(a, sh.rows, un.rows, t0, C, rank, tid, AD_WARPS * 32);
+            ad_copy<O>(a, sh.rows, un.rows, t0, C, rank);
             __syncthreads();
         } else {
             ad_unit<T, O>(a, L, smem, sh, C, rank, (int32_t)un.place, un.rows, un.per <= 16 ? 1 : un.per <= 32 ? 2 : 4, t0);   // one split for all units of an adapter
@@ -699,16 +726,21 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
 // the adapter's rank).  A warp to a ring slot, one that issues the products, eight that read accumulators: inner sums -> shared memory -> the cluster's fold ->
 // parts of u as operand rows; outputs -> turned through shared memory -> + base -> y.  The fold's steps are joined by mbarriers between the CTAs, so the
 // ring runs on underneath.  Every wait is bounded: a give-up sets the status word, and everybody still meets at the end.
-constexpr uint32_t AB_SLOTS = 5, AB_MAX_R = 128, AB_MIN_ROWS = 16;   // from so many tokens per unit on
-constexpr uint32_t AB_A_BYTES = 128 * 128, AB_X_BYTES = 64 * 128, AB_SLOT = AB_A_BYTES + AB_X_BYTES;
+constexpr uint32_t AB_MOST_SLOTS = 9, AB_MAX_R = 128, AB_MIN_ROWS = 16;   // from so many tokens per unit on
 constexpr uint32_t AB_U_BYTES = 64 * 128;                            // one part of 64 rank columns of the unit's tokens
 constexpr uint32_t AB_TURN = 16 * 32 * 4;                            // an epilogue warp's turn of 16 tokens x 32 outputs
-constexpr uint32_t AB_THREADS = (1 + AD_WARPS + AB_SLOTS) * 32;
-struct AbSmem { uint32_t u, part, turn, sort, bytes; };              // behind the ring, offsets from its 1024-byte boundary
+struct AbSmem {
+    uint32_t slots, slot, x;                                         // ring slots, their bytes, x rows behind R rows of A (the products read 128: what is there)
+    uint32_t u, part, turn, sort, bytes;                             // behind the ring, offsets from its 1024-byte boundary
+    __host__ __device__ uint32_t threads() const { return (1 + AD_WARPS + slots) * 32; }
+};
 __host__ __device__ inline AbSmem ab_smem(uint32_t R) {
     AbSmem s;
     const uint32_t chunks = (R + 63) / 64;
-    s.u = AB_SLOTS * AB_SLOT;
+    s.x = R * 128;                                                   // a multiple of 1024
+    s.slot = R <= 64 ? 128 * 128 : s.x + 64 * 128;                   // a block of 128 outputs' B fits too
+    s.slots = R <= 64 ? AB_MOST_SLOTS : 5;
+    s.u = s.slots * s.slot;
     s.part = s.u + chunks * 2 * AB_U_BYTES;
     s.turn = s.part + (R + 15) / 16 * 16 * 64 * 4;
     s.sort = s.turn + AD_WARPS * AB_TURN;
@@ -735,9 +767,10 @@ __device__ __forceinline__ void ab_tma_3d(uint32_t dst, const CUtensorMap* map, 
 __device__ __forceinline__ void ab_expect(uint32_t bar, uint32_t bytes) {   // bytes to wait for, no arrival
     asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// the first n bytes of 16, zeros behind
+// The first n bytes of 16, zeros behind.  No clobber of memory: the compiler may load the next rows' numbers meanwhile (a load between every two
+// copies made a stage's 16 copies 1600 cycles); the wait for the copies has one.
 __device__ __forceinline__ void ab_copy(uint32_t dst, const void* src, uint32_t n) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n));
 }
 template <class O> struct AbBase;        // four outputs of base
 template <> struct AbBase<float> { typedef uint4 Word; };
@@ -745,9 +778,9 @@ template <> struct AbBase<__nv_bfloat16> { typedef uint2 Word; };
 template <> struct AbBase<__half> { typedef uint2 Word; };
 
 template <class T, class O>
-__global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __grid_constant__ AbParams P) {
+__global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapters_tensor_kernel(const __grid_constant__ AbParams P) {
     extern __shared__ uint8_t smem_any[];
-    __shared__ __align__(8) uint64_t full_bar[AB_SLOTS], empty_bar[AB_SLOTS], d1_full, d1_empty, d2_full[2], d2_empty[2], part_ready, u_ready, u_go;
+    __shared__ __align__(8) uint64_t full_bar[AB_MOST_SLOTS], empty_bar[AB_MOST_SLOTS], d1_full, d1_empty, d2_full[2], d2_empty[2], part_ready, u_ready, u_go;
     __shared__ uint32_t s_tmem, s_scan[AD_WARPS];
     __shared__ float s_scale[AD_TT];
     __shared__ volatile int s_abort;
@@ -759,7 +792,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
     const uint32_t cl = blockIdx.x / C, seg = cl / P.per_seg, t0 = seg * AD_SEG, n_tok = min(AD_SEG, a.T - t0), n_places = a.n_adapters + 1;
     AdSort& so = *reinterpret_cast<AdSort*>(ring_p + L.sort);
     if (tid == 0) {
-        for (uint32_t s = 0; s < AB_SLOTS; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        for (uint32_t s = 0; s < L.slots; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         mbar_init(&d1_full, 1); mbar_init(&d1_empty, AD_WARPS);
         for (int b = 0; b < 2; ++b) { mbar_init(&d2_full[b], 1); mbar_init(&d2_empty[b], AD_WARPS); }
         mbar_init(&part_ready, C); mbar_init(&u_ready, C); mbar_init(&u_go, 1);
@@ -783,8 +816,8 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
     };
 
     if (warp > AD_WARPS) {
-        // ---------------- a ring slot's warp: every AB_SLOTS-th stage ----------------
-        const uint32_t slot = warp - AD_WARPS - 1, full = smem_u32(&full_bar[slot]), empty = smem_u32(&empty_bar[slot]), at = ring + slot * AB_SLOT;
+        // ---------------- a ring slot's warp: every L.slots-th stage ----------------
+        const uint32_t slot = warp - AD_WARPS - 1, full = smem_u32(&full_bar[slot]), empty = smem_u32(&empty_bar[slot]), at = ring + slot * L.slot;
         const uint32_t chunk = lane & 7u, row0 = lane >> 3;
         uint32_t ph = 0, base = 0;                                    // stages of the units before, modulo the ring
         bool ok = true;
@@ -793,7 +826,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
             if (un.place == a.n_adapters) continue;
             const uint32_t R = rank_of(un.place), chunks = (R + 63) / 64, n_in = R ? ks1 - ks0 : 0, n_st = n_in + (fb1 - fb0) * chunks;
             const T* const B = static_cast<const T*>(a.b) + (size_t)un.place * a.b_stride;
-            for (uint32_t st = (slot + AB_SLOTS - base) % AB_SLOTS; st < n_st; st += AB_SLOTS) {
+            const T* xr[AD_TT / 4];
+#pragma unroll
+            for (uint32_t i = 0; i < AD_TT / 4; ++i) xr[i] = static_cast<const T*>(a.x) + (size_t)(t0 + so.order[un.at + min(row0 + i * 4, un.rows - 1)]) * a.ld_x;
+            for (uint32_t st = (slot + L.slots - base) % L.slots; st < n_st; st += L.slots) {
                 if (!mbar_wait_warp_at(empty, ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
                 if (st < n_in) {
                     const uint32_t k = (ks0 + st) * 64;
@@ -802,10 +838,12 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
                         ab_tma_3d(at, &P.a, (int32_t)k, 0, (int32_t)un.place, full);
                     }
                     const bool in = k + chunk * 8 < a.K;
-                    const T* x = static_cast<const T*>(a.x) + (in ? k + chunk * 8 : 0);
-#pragma unroll 4
-                    for (uint32_t r = row0; r < un.rows; r += 4)
-                        ab_copy(at + AB_A_BYTES + r * 128 + ((chunk ^ (r & 7u)) << 4), x + (size_t)(t0 + so.order[un.at + r]) * a.ld_x, in ? 16 : 0);
+                    const uint32_t from = in ? k + chunk * 8 : 0, n = in ? 16 : 0;
+#pragma unroll
+                    for (uint32_t i = 0; i < AD_TT / 4; ++i) {
+                        const uint32_t r = row0 + i * 4;
+                        if (r < un.rows) ab_copy(at + L.x + r * 128 + ((chunk ^ (r & 7u)) << 4), xr[i] + from, n);
+                    }
                 } else {
                     const uint32_t i = st - n_in, f0 = (fb0 + i / chunks) * 128, r = (i % chunks) * 64 + chunk * 8;
                     const uint32_t n = r >= R ? 0 : R - r < 8 ? (R - r) * 2 : 16;       // bytes of this lane's eight rank columns that count
@@ -820,7 +858,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
                 if (lane == 0) mbar_arrive_at(full);
                 ph ^= 1u;
             }
-            base = (base + n_st) % AB_SLOTS;
+            base = (base + n_st) % L.slots;
         }
         if (s_abort) for (int i = 0; i < 2000; ++i) __nanosleep(1000);   // copies in flight land before the memory goes
     } else if (warp == AD_WARPS) {
@@ -834,7 +872,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
             if (!ok) give_up(code);
             tc_fence_after();
         };
-        auto next = [&]() { if (++s == AB_SLOTS) { s = 0; ph ^= 1u; } };
+        auto next = [&]() { if (++s == L.slots) { s = 0; ph ^= 1u; } };
         for (uint32_t u = cl % P.per_seg; u < n_units && ok; u += P.per_seg) {
             const AdUnit un = ad_find(so, n_places, u);
             if (un.place == a.n_adapters) continue;
@@ -844,11 +882,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
                 for (uint32_t ks = ks0; ks < ks1 && ok; ++ks) {
                     wait(&full_bar[s], ph, ST_WAIT_FULL);
                     if (!ok) break;
-                    const uint32_t at = ring + s * AB_SLOT;
+                    const uint32_t at = __shfl_sync(0xFFFFFFFFu, (ring + s * L.slot) >> 4, 0) | 1u << 16, x_at = at + (L.x >> 4);
                     if (elect_one()) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j)
-                            umma_f16(tmem, umma_desc_sw128(at + j * 32, 16, 1024), umma_desc_sw128(at + AB_A_BYTES + j * 32, 16, 1024), idesc, ks != ks0 || j ? 1u : 0u);
+                        for (uint32_t j = 0; j < 4; ++j) umma_f16_lo(tmem, at + j * 2, x_at + j * 2, UMMA_SW128_HI, idesc, ks != ks0 || j ? 1u : 0u);
                         umma_commit(&empty_bar[s]);
                     }
                     __syncwarp();
@@ -866,11 +903,14 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
                 for (uint32_t c = 0; c < chunks && ok; ++c) {
                     wait(&full_bar[s], ph, ST_WAIT_FULL);
                     if (!ok) break;
-                    const uint32_t at = ring + s * AB_SLOT, ua = ring + L.u + c * 2 * AB_U_BYTES, steps = (min(R - c * 64, 64u) + 15) / 16;
+                    const uint32_t at = __shfl_sync(0xFFFFFFFFu, (ring + s * L.slot) >> 4, 0) | 1u << 16, steps = (min(R - c * 64, 64u) + 15) / 16;
+                    const uint32_t ua = __shfl_sync(0xFFFFFFFFu, (ring + L.u + c * 2 * AB_U_BYTES) >> 4, 0) | 1u << 16;
                     if (elect_one()) {
+#pragma unroll
                         for (uint32_t part = 0; part < 2; ++part)
-                            for (uint32_t j = 0; j < steps; ++j)
-                                umma_f16(acc, umma_desc_sw128(at + j * 32, 16, 1024), umma_desc_sw128(ua + part * AB_U_BYTES + j * 32, 16, 1024), idesc, c | part | j ? 1u : 0u);
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; ++j)
+                                if (j < steps) umma_f16_lo(acc, at + j * 2, ua + part * (AB_U_BYTES >> 4) + j * 2, UMMA_SW128_HI, idesc, c | part | j ? 1u : 0u);
                         umma_commit(&empty_bar[s]);
                     }
                     __syncwarp();
@@ -904,10 +944,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
         };
         for (uint32_t u = cl % P.per_seg; u < n_units && ok; u += P.per_seg) {
             const AdUnit un = ad_find(so, n_places, u);
-            if (un.place == a.n_adapters) { ad_copy<O>(a, so.order + un.at, un.rows, t0, C, rank, etid, AD_WARPS * 32); continue; }
+            if (un.place == a.n_adapters) { ad_copy<O>(a, so.order + un.at, un.rows, t0, C, rank); continue; }
             const uint32_t R = rank_of(un.place);
             if (!R) {   // outputs are base
-                ad_copy<O>(a, so.order + un.at, un.rows, t0, C, rank, etid, AD_WARPS * 32);
+                ad_copy<O>(a, so.order + un.at, un.rows, t0, C, rank);
                 continue;
             }
             // inner sums of this CTA's inputs
@@ -928,7 +968,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
             if (etid < C) mbar_arrive_cluster(map_to_rank(smem_u32(&part_ready), etid));
             wait(&part_ready, n_done & 1u);
             if (!together()) break;
-            ad_fold<T>(a, C, rank, (int32_t)un.place, R, un.rows, warp, ring + L.part, r16, smem_u32(s_scale), parts);
+            ad_fold<T, AB_MAX_R / 64, 4>(a, C, rank, (int32_t)un.place, R, un.rows, warp, ring + L.part, r16, smem_u32(s_scale), parts);
             together();
             if (etid < C) mbar_arrive_cluster(map_to_rank(smem_u32(&u_ready), etid));
             wait(&u_ready, n_done & 1u);
@@ -938,18 +978,23 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
             ++n_done;
             // outputs: a lane four of a token, eight lanes a token's 32, a warp four tokens at a time
             const uint32_t i0 = half * 32 + (lane >> 3), f4 = q * 32 + (lane & 7u) * 4;
-            for (uint32_t fb = fb0; fb < fb1 && ok; ++fb, ++n_blocks) {
-                const uint32_t buf = n_blocks & 1u, f = fb * 128 + f4;
-                typename AbBase<O>::Word b[2][4] = {};
-                const bool in = f < a.N;
+            typename AbBase<O>::Word b[2][4];
+            auto ask_base = [&](uint32_t fb) {
+                const uint32_t f = fb * 128 + f4;
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) {
                         const uint32_t i = i0 + h * 16 + j * 4;
-                        if (a.base && in && i < un.rows)
+                        b[h][j] = {};
+                        if (a.base && fb < fb1 && f < a.N && i < un.rows)
                             b[h][j] = *reinterpret_cast<const typename AbBase<O>::Word*>(static_cast<const O*>(a.base) + (size_t)(t0 + so.order[un.at + i]) * a.ld_base + f);
                     }
+            };
+            ask_base(fb0);
+            for (uint32_t fb = fb0; fb < fb1 && ok; ++fb, ++n_blocks) {
+                const uint32_t buf = n_blocks & 1u, f = fb * 128 + f4;
+                const bool in = f < a.N;
                 if (!wait(&d2_full[buf], n_blocks >> 1 & 1u)) break;
                 tc_fence_after();
 #pragma unroll
@@ -982,6 +1027,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1) adapters_tensor_kernel(const __
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&d2_empty[buf]);
+                ask_base(fb + 1);                        // under the next block's products
             }
             together();
         }
@@ -1030,7 +1076,7 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
         while (P.C > (a.K + 63) / 64) P.C /= 2;                     // every CTA has inputs to sum
         P.per_seg = sms / (P.C * segs);
         P.per_seg = P.per_seg < 1 ? 1 : P.per_seg > units + tokens / AD_TT + 1 ? units + tokens / AD_TT + 1 : P.per_seg;
-        return ad_launch(adapters_tensor_kernel<T, O>, P.C, P.per_seg * segs, AB_THREADS, ab_smem(a.R).bytes, st, P);
+        return ad_launch(adapters_tensor_kernel<T, O>, P.C, P.per_seg * segs, ab_smem(a.R).threads(), ab_smem(a.R).bytes, st, P);
     }
     const uint32_t C = spread((uint64_t)units * segs, room, 2);
     uint32_t per_seg = room / (C * segs);

@@ -282,9 +282,10 @@ __device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&v)[1
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// 16 bytes, or zeros where there is nothing to read
+// 16 bytes, or zeros where there is nothing to read.  No clobber of memory: the compiler may load the next rows' numbers meanwhile; the wait for the
+// copies has one.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u));
 }
 __device__ __forceinline__ void st_shared4(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {

@@ -77,6 +77,15 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr, uint32_t lbo
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) |
            (1ull << 46) | (2ull << 61);
 }
+// K-major descriptors by their low words (address >> 4, lbo 16 bytes: 1 << 16), which alone change along a tile, and the high word they share; one CTA
+constexpr uint32_t UMMA_SW128_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void umma_f16_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
+        ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // M = 256 over the pair; a_m_major: A's descriptor is M-major
 __device__ __forceinline__ uint32_t umma_idesc_pair(uint32_t fmt, uint32_t n, bool a_m_major) {
     return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_m_major ? 1u << 15 : 0u) | ((n >> 3) << 17) | ((256u >> 4) << 24);
