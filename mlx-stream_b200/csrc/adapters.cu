@@ -32,17 +32,15 @@ __device__ __forceinline__ uint4 ad_ld16(const void* p) {
     asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
+// not volatile: the compiler may put operand loads between the products
 template <class T>
-__device__ __forceinline__ void ad_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void ad_mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    const uint32_t a[4] = {a0, a1, a2, a3};
-    mma_bf16(d, a, b0, b1);
-}
-template <>
-__device__ __forceinline__ void ad_mma<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    const uint32_t a[4] = {a0, a1, a2, a3};
-    mma_f16(d, a, b0, b1);
+__device__ __forceinline__ void ad_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ float ad_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float ad_f32(__half v) { return __half2float(v); }
@@ -160,7 +158,7 @@ __device__ __forceinline__ void ad_copy16(uint32_t dst, const void* src, bool th
 }
 __device__ __forceinline__ uint4 ad_lds16(uint32_t addr) {
     uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
     return v;
 }
 // 17 .. 64 tokens: the rows of x and A go through a ring of stages of 64 inputs in shared memory (fragment loads straight from memory keep too few
@@ -978,6 +976,9 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
             ++n_done;
             // outputs: a lane four of a token, eight lanes a token's 32, a warp four tokens at a time
             const uint32_t i0 = half * 32 + (lane >> 3), f4 = q * 32 + (lane & 7u) * 4;
+            uint32_t rows[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) rows[k] = t0 + so.order[un.at + min(i0 + k * 4, un.rows - 1)];
             typename AbBase<O>::Word b[2][4];
             auto ask_base = [&](uint32_t fb) {
                 const uint32_t f = fb * 128 + f4;
@@ -988,7 +989,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
                         const uint32_t i = i0 + h * 16 + j * 4;
                         b[h][j] = {};
                         if (a.base && fb < fb1 && f < a.N && i < un.rows)
-                            b[h][j] = *reinterpret_cast<const typename AbBase<O>::Word*>(static_cast<const O*>(a.base) + (size_t)(t0 + so.order[un.at + i]) * a.ld_base + f);
+                            b[h][j] = *reinterpret_cast<const typename AbBase<O>::Word*>(static_cast<const O*>(a.base) + (size_t)rows[h * 4 + j] * a.ld_base + f);
                     }
             };
             ask_base(fb0);
@@ -1006,13 +1007,16 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
 #pragma unroll
                     for (uint32_t j = 0; j < 16; ++j) asm volatile("st.shared.u32 [%0], %1;" ::"r"(turn + (j * 32 + lane) * 4), "r"(v[j]) : "memory");
                     __syncwarp();
+                    uint4 turned[4];                     // all read before the first is used
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) turned[j] = ad_lds16(turn + ((lane >> 3) + j * 4) * 128 + (lane & 7u) * 16);
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) {
                         const uint32_t i = i0 + h * 16 + j * 4;
-                        const uint4 w = ad_lds16(turn + ((lane >> 3) + j * 4) * 128 + (lane & 7u) * 16);
+                        const uint4 w = turned[j];
                         if (!in || i >= un.rows) continue;
                         const float s = std::is_same<T, __half>::value ? s_scale[i] : 1.f;
-                        O* y = static_cast<O*>(a.y) + (size_t)(t0 + so.order[un.at + i]) * a.ld_y + f;
+                        O* y = static_cast<O*>(a.y) + (size_t)rows[h * 4 + j] * a.ld_y + f;
                         if constexpr (sizeof(O) == 4) {
                             const uint4 c = b[h][j];
                             *reinterpret_cast<float4*>(y) = make_float4(fmaf(__uint_as_float(w.x), s, __uint_as_float(c.x)), fmaf(__uint_as_float(w.y), s, __uint_as_float(c.y)),

@@ -500,17 +500,23 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                     }
                     __syncwarp();
                     const uint32_t fq = f - lane + (lane & 7u) * 4;
+                    constexpr uint32_t HALVES = SWIGLU ? 1 : 2;
+                    uint4 w[2][HALVES];                  // all read before the first is used
+#pragma unroll
+                    for (uint32_t i2 = 0; i2 < 2; ++i2)
+#pragma unroll
+                        for (uint32_t h = 0; h < HALVES; ++h) w[i2][h] = ld_shared16(turn + h * GT_TURN + ((lane >> 3) + 4 * i2) * 128 + (lane & 7u) * 16);
 #pragma unroll
                     for (uint32_t i2 = 0; i2 < 2; ++i2) {
                         const uint32_t k = (lane >> 3) + 4 * i2;
                         const uint32_t ra = __shfl_sync(0xFFFFFFFFu, yr, 2 * k), rb = __shfl_sync(0xFFFFFFFFu, yr, 2 * k + 1);
                         O *oa = y + (size_t)ra * a.ld_y + fq, *ob = y + (size_t)rb * a.ld_y + fq;
 #pragma unroll
-                        for (uint32_t h = 0; h < (SWIGLU ? 1u : 2u); ++h) {
-                            const uint4 w = ld_shared16(turn + h * GT_TURN + k * 128 + (lane & 7u) * 16);
+                        for (uint32_t h = 0; h < HALVES; ++h) {
+                            const uint4 v = w[i2][h];
                             if (fq + h * 128 < a.N) {
-                                if (ra != 0xFFFFFFFFu) *reinterpret_cast<uint2*>(oa + h * 128) = make_uint2(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.z, w.w, 0x5410));
-                                if (rb != 0xFFFFFFFFu) *reinterpret_cast<uint2*>(ob + h * 128) = make_uint2(__byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x7632));
+                                if (ra != 0xFFFFFFFFu) *reinterpret_cast<uint2*>(oa + h * 128) = make_uint2(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.z, v.w, 0x5410));
+                                if (rb != 0xFFFFFFFFu) *reinterpret_cast<uint2*>(ob + h * 128) = make_uint2(__byte_perm(v.x, v.y, 0x7632), __byte_perm(v.z, v.w, 0x7632));
                             }
                         }
                     }
