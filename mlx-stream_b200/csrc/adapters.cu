@@ -724,6 +724,8 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
 // the adapter's rank).  A warp to a ring slot, one that issues the products, eight that read accumulators: inner sums -> shared memory -> the cluster's fold ->
 // parts of u as operand rows; outputs -> turned through shared memory -> + base -> y.  The fold's steps are joined by mbarriers between the CTAs, so the
 // ring runs on underneath.  Every wait is bounded: a give-up sets the status word, and everybody still meets at the end.
+// The inner product's accumulator truncates (see the grouped products): its inputs are dealt out in order to up to six accumulators, added in f32.
+constexpr uint32_t AB_CHAIN = 8, AB_CHAINS = 6, AB_D2 = AB_CHAINS * 64;   // stages, accumulators of 64 columns, the outputs' first column
 constexpr uint32_t AB_MOST_SLOTS = 9, AB_MAX_R = 128, AB_MIN_ROWS = 16;   // from so many tokens per unit on
 constexpr uint32_t AB_U_BYTES = 64 * 128;                            // one part of 64 rank columns of the unit's tokens
 constexpr uint32_t AB_TURN = 16 * 32 * 4;                            // an epilogue warp's turn of 16 tokens x 32 outputs
@@ -798,7 +800,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         mbar_fence_init();
         tma_prefetch_map(&P.a);
     }
-    if (warp == AD_WARPS) tmem_alloc(&s_tmem, 256);                   // the issuer's warp
+    if (warp == AD_WARPS) tmem_alloc(&s_tmem, 512);                   // the issuer's warp
     ad_sort(a, so, reinterpret_cast<uint16_t*>(ring_p), s_scan, t0, n_tok, cl % P.per_seg == 0 && rank == 0);
     fence_async_smem();                                               // the sort's scratch was where copies land
     tc_fence_before();
@@ -807,6 +809,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
     const uint32_t tmem = s_tmem, n_units = so.first[n_places] >> 16;
     const uint32_t n_ks = (a.K + 63) / 64, ks0 = rank * n_ks / C, ks1 = (rank + 1) * n_ks / C;
     const uint32_t n_fb = (a.N + 127) / 128, fb0 = rank * n_fb / C, fb1 = (rank + 1) * n_fb / C;
+    const uint32_t per_chain = max(AB_CHAIN, (ks1 - ks0 + AB_CHAINS - 1) / AB_CHAINS), n_chains = (ks1 - ks0 + per_chain - 1) / per_chain;
     auto give_up = [&](uint32_t code) { if (!s_abort) atomicMax(a.status, code); s_abort = 1; };
     auto rank_of = [&](uint32_t place) {
         const int32_t given = a.ranks ? a.ranks[place] : (int32_t)a.R;
@@ -883,7 +886,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
                     const uint32_t at = __shfl_sync(0xFFFFFFFFu, (ring + s * L.slot) >> 4, 0) | 1u << 16, x_at = at + (L.x >> 4);
                     if (elect_one()) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) umma_f16_lo(tmem, at + j * 2, x_at + j * 2, UMMA_SW128_HI, idesc, ks != ks0 || j ? 1u : 0u);
+                        for (uint32_t j = 0; j < 4; ++j) umma_f16_lo(tmem + (ks - ks0) / per_chain * 64, at + j * 2, x_at + j * 2, UMMA_SW128_HI, idesc, (ks - ks0) % per_chain || j ? 1u : 0u);
                         umma_commit(&empty_bar[s]);
                     }
                     __syncwarp();
@@ -896,7 +899,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
             // the parts of u are there (a unit without a rank has none: its outputs are base)
             if (R) wait(&u_go, n_done & 1u, ST_WAIT_FULL);
             for (uint32_t fb = fb0; fb < fb1 && ok && R; ++fb, ++n_blocks) {
-                const uint32_t buf = n_blocks & 1u, acc = tmem + 64 + buf * 64;
+                const uint32_t buf = n_blocks & 1u, acc = tmem + AB_D2 + buf * 64;
                 wait(&d2_empty[buf], (n_blocks >> 1 & 1u) ^ 1u, ST_WAIT_EMPTY);
                 for (uint32_t c = 0; c < chunks && ok; ++c) {
                     wait(&full_bar[s], ph, ST_WAIT_FULL);
@@ -953,11 +956,16 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
             tc_fence_after();
             if (ok && q * 32 < R)
                 for (uint32_t c = half * 32; c < half * 32 + 32 && c < un.rows; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld16(tmem + c + ((q * 32u) << 16), v);
+                    float sum[16];
+                    for (uint32_t chain = 0; chain < n_chains; ++chain) {
+                        uint32_t v[16];
+                        tmem_ld16(tmem + chain * 64 + c + ((q * 32u) << 16), v);
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; ++j) sum[j] = chain ? sum[j] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
+                    }
                     if (q * 32 + lane < r16)
 #pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j) part[(c + j) * r16 + q * 32 + lane] = __uint_as_float(v[j]);
+                        for (uint32_t j = 0; j < 16; ++j) part[(c + j) * r16 + q * 32 + lane] = sum[j];
                 }
             tc_fence_before();
             __syncwarp();
@@ -1002,7 +1010,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
                 for (uint32_t h = 0; h < 2; ++h) {
                     if (half * 32 + h * 16 >= un.rows) break;
                     uint32_t v[16];
-                    tmem_ld16(tmem + 64 + buf * 64 + half * 32 + h * 16 + ((q * 32u) << 16), v);
+                    tmem_ld16(tmem + AB_D2 + buf * 64 + half * 32 + h * 16 + ((q * 32u) << 16), v);
                     __syncwarp();
 #pragma unroll
                     for (uint32_t j = 0; j < 16; ++j) asm volatile("st.shared.u32 [%0], %1;" ::"r"(turn + (j * 32 + lane) * 4), "r"(v[j]) : "memory");
@@ -1041,7 +1049,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
     __syncwarp();
     cluster_sync_all();
     tc_fence_after();
-    if (warp == AD_WARPS) tmem_free(tmem, 256);
+    if (warp == AD_WARPS) tmem_free(tmem, 512);
 }
 
 template <class... Params, class... Args>

@@ -238,6 +238,10 @@ constexpr uint32_t GT_TURN = 8 * 32 * 4;                         // an epilogue 
 constexpr uint32_t GT_SMEM = GT_STAGES * GT_STAGE + GT_EPI_WARPS * 2 * GT_TURN + 1024;
 
 constexpr uint32_t GT_PARTS = 4;                                  // most parts of a reduction: a cluster of eight CTAs
+// f32 outputs: the accumulator's additions truncate (1.7e-8 of the sum for each product of 16 inputs: 2.4e-6 after 2304 inputs), so after as many stages
+// as this the sums move on: the epilogue warps add them, rounding, to running sums in the tensor memory's second half
+constexpr uint32_t GT_CHAIN = 8;
+constexpr uint32_t GT_RUN = 256;                                 // first column of the running sums
 constexpr uint32_t GT_BOXES = 5;
 __host__ __device__ constexpr uint32_t gt_box_rows(uint32_t i) { return i < 3 ? 16u << i : 32 * i; }   // 16 32 64 96 128
 
@@ -281,6 +285,13 @@ __device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&v)[1
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+        "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // 16 bytes, or zeros where there is nothing to read.  No clobber of memory: the compiler may load the next rows' numbers meanwhile; the wait for the
 // copies has one.
@@ -353,8 +364,9 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
     const uint32_t n_pairs = P.parts == 1 ? gridDim.x / 2 : max(n_items, 1u);
     const uint32_t ks0 = part * P.n_ks / P.parts, ks1 = (part + 1) * P.n_ks / P.parts;
     constexpr uint32_t FT = SWIGLU ? 256 : 512;                  // outputs of an item: half of them this CTA's
-    // tensor memory: buffers of two accumulators of `cap` columns
-    const uint32_t n_buf = 256 / P.cap;
+    // tensor memory: buffers of two accumulators of `cap` columns (f32 outputs: in the first half, with running sums in the second)
+    constexpr bool SUMS = sizeof(O) == 4;
+    const uint32_t n_buf = (SUMS ? 128 : 256) / P.cap, n_chains = SUMS ? (ks1 - ks0 + GT_CHAIN - 1) / GT_CHAIN : 1;
     auto give_up = [&](uint32_t code) { if (!s_abort) atomicMax(a.status, code); s_abort = 1; };
     GtWalk walk{s_off, s_tiles, a.G};
 
@@ -404,31 +416,35 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
             const uint32_t a_next = a.in_out && SWIGLU ? GT_A_HALF / 2 : GT_A_HALF;   // to the second accumulator's tile
             for (uint32_t i = pair; i < n_items && ok; i += n_pairs) {
                 const GtItem it = walk.at(i / P.n_ft);
-                const uint32_t idesc = umma_idesc_pair(P.fmt, it.n, a.in_out), buf = n_done % n_buf, acc = tmem + buf * 2 * P.cap;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_empty[buf]), (n_done / n_buf & 1u) ^ 1u, &s_abort));
-                if (!ok) { give_up(ST_WAIT_EMPTY); break; }
-                tc_fence_after();
-                for (uint32_t ks = ks0; ks < ks1; ++ks) {
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&full_bar[s]), ph, &s_abort));
-                    if (!ok) { give_up(ST_WAIT_FULL); break; }
+                const uint32_t idesc = umma_idesc_pair(P.fmt, it.n, a.in_out);
+                for (uint32_t chain = 0; chain < n_chains && ok; ++chain) {
+                    const uint32_t buf = n_done % n_buf, acc = tmem + buf * 2 * P.cap;
+                    const uint32_t k0 = SUMS ? ks0 + chain * GT_CHAIN : ks0, k1 = SUMS ? min(k0 + GT_CHAIN, ks1) : ks1;
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_empty[buf]), (n_done / n_buf & 1u) ^ 1u, &s_abort));
+                    if (!ok) { give_up(ST_WAIT_EMPTY); break; }
                     tc_fence_after();
-                    const uint32_t sa = ring + s * GT_STAGE, sb = sa + GT_A_BYTES;
-                    if (elect_one()) {
+                    for (uint32_t ks = k0; ks < k1; ++ks) {
+                        ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&full_bar[s]), ph, &s_abort));
+                        if (!ok) { give_up(ST_WAIT_FULL); break; }
+                        tc_fence_after();
+                        const uint32_t sa = ring + s * GT_STAGE, sb = sa + GT_A_BYTES;
+                        if (elect_one()) {
 #pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h)
+                            for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
-                            for (uint32_t j = 0; j < GT_KS / 16; ++j)
-                                umma_f16_pair(acc + h * P.cap, umma_desc_sw128(sa + h * a_next + j * a_step, a_lbo, 1024),
-                                              umma_desc_sw128(sb + j * 32, 16, 1024), idesc, ks != ks0 || j ? 1u : 0u);
-                        umma_commit_pair(smem_u32(&empty_bar[s]), pair_mask);
+                                for (uint32_t j = 0; j < GT_KS / 16; ++j)
+                                    umma_f16_pair(acc + h * P.cap, umma_desc_sw128(sa + h * a_next + j * a_step, a_lbo, 1024),
+                                                  umma_desc_sw128(sb + j * 32, 16, 1024), idesc, ks != k0 || j ? 1u : 0u);
+                            umma_commit_pair(smem_u32(&empty_bar[s]), pair_mask);
+                        }
+                        __syncwarp();
+                        if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
                     }
+                    if (!ok) break;
+                    if (elect_one()) umma_commit_pair(smem_u32(&acc_full[buf]), pair_mask);
                     __syncwarp();
-                    if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
+                    ++n_done;
                 }
-                if (!ok) break;
-                if (elect_one()) umma_commit_pair(smem_u32(&acc_full[buf]), pair_mask);
-                __syncwarp();
-                ++n_done;
             }
         }
     } else if (warp < 2 + GT_EPI_WARPS) {
@@ -439,15 +455,37 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
         const uint32_t turn = ring + GT_STAGES * GT_STAGE + (warp - 2) * 2 * GT_TURN;
         for (uint32_t i = pair; i < n_items; i += n_pairs) {
             const GtItem it = walk.at(i / P.n_ft);
-            const uint32_t buf = n_done % n_buf, f = (i % P.n_ft) * FT + rank * (FT / 2) + q * 32 + lane;
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_full[buf]), n_done / n_buf & 1u, &s_abort))) { give_up(ST_WAIT_FULL); break; }
+            const uint32_t f = (i % P.n_ft) * FT + rank * (FT / 2) + q * 32 + lane;
+            bool ok = true;
+            for (uint32_t chain = 0; chain < n_chains; ++chain) {
+            const uint32_t buf = n_done % n_buf, lanes = (q * 32u) << 16;
+            const bool last = !SUMS || chain + 1 == n_chains;
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_full[buf]), n_done / n_buf & 1u, &s_abort));
+            if (!ok) { give_up(ST_WAIT_FULL); break; }
             tc_fence_after();
-            if (P.parts > 1) {
-                // a part's sums, where the ring was (its copies have landed, the products have read them): [accumulator][row][128 outputs]
-                for (uint32_t c = half * 16; c < it.rows; c += 32) {
-                    uint32_t v0[16], v1[16];
-                    tmem_ld16_nowait(tmem + c + ((q * 32u) << 16), v0);
-                    tmem_ld16_nowait(tmem + P.cap + c + ((q * 32u) << 16), v1);
+            for (uint32_t c = half * 16; c < it.rows; c += 32) {
+                uint32_t v0[16], v1[16];
+                tmem_ld16_nowait(tmem + buf * 2 * P.cap + c + lanes, v0);
+                tmem_ld16_nowait(tmem + buf * 2 * P.cap + P.cap + c + lanes, v1);
+                if (SUMS && chain) {
+                    uint32_t r0[16], r1[16];
+                    tmem_ld16_nowait(tmem + GT_RUN + c + lanes, r0);
+                    tmem_ld16_nowait(tmem + GT_RUN + P.cap + c + lanes, r1);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        v0[j] = __float_as_uint(__uint_as_float(r0[j]) + __uint_as_float(v0[j]));
+                        v1[j] = __float_as_uint(__uint_as_float(r1[j]) + __uint_as_float(v1[j]));
+                    }
+                }
+                if (!last) {
+                    tmem_wait_ld();
+                    tmem_st16(tmem + GT_RUN + c + lanes, v0);
+                    tmem_st16(tmem + GT_RUN + P.cap + c + lanes, v1);
+                    continue;
+                }
+                if (P.parts > 1) {
+                    // a part's sums, where the ring was (its copies have landed, the products have read them): [accumulator][row][128 outputs]
                     tmem_wait_ld();
                     const uint32_t z = ring + (c * 128 + q * 32 + lane) * 4;
 #pragma unroll
@@ -455,13 +493,8 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                         st_shared4(z + j * 512, v0[j]);
                         st_shared4(z + (P.cap + j) * 512, v1[j]);
                     }
+                    continue;
                 }
-                break;
-            }
-            for (uint32_t c = half * 16; c < it.rows; c += 32) {
-                uint32_t v0[16], v1[16];
-                tmem_ld16_nowait(tmem + buf * 2 * P.cap + c + ((q * 32u) << 16), v0);
-                tmem_ld16_nowait(tmem + buf * 2 * P.cap + P.cap + c + ((q * 32u) << 16), v1);
                 // lane j < 16: where row c + j of the tile goes
                 uint32_t yr = 0xFFFFFFFFu;
                 if (lane < 16 && c + lane < it.rows) {
@@ -522,10 +555,13 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                     }
                 }
             }
+            if (!last) tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[buf]), leader));
             ++n_done;
+            }
+            if (!ok) break;
         }
     } else if (a.gather) {
         // ---------------- gathered rows: a warp to a ring slot, so that waiting for its copies keeps nobody; eight lanes copy 128 bytes of a row ----------------
@@ -626,14 +662,16 @@ static GtClusters gt_clusters(const void* kernel, int sm_count) {
 // device; the estimate takes them as equal.  A stage costs its products (4 cycles a row) or its bytes (55 a cycle), whichever is longer; joining parts costs
 // as much as eight stages.  Returns the row tiles that the call can have at most.
 static uint32_t gt_cut(const GroupedArgs& a, uint32_t n_ft, uint32_t n_ks, const GtClusters& room, uint32_t* cap, uint32_t* parts) {
+    const bool sums = a.out_dtype == DT_F32;          // f32 outputs: 64 rows and two buffers, or 128 and one that the products wait for
     const uint32_t groups = a.G < a.rows ? a.G : a.rows, per = (a.rows + groups - 1) / groups;
     double best = 0;
-    for (const uint32_t c : {128u, 160u, 192u, 256u})
+    for (const uint32_t c : {64u, 128u, 160u, 192u, 256u})
         for (uint32_t s = 1; s <= (c <= 192 ? GT_PARTS : 1u) && s <= n_ks; ++s) {
+            if (sums ? c > 128 : c == 64) continue;
             const uint32_t tiles = (per + c - 1) / c, n = ((per + tiles - 1) / tiles + 31) / 32 * 32;
             const uint64_t items = (uint64_t)groups * tiles * n_ft, waves = (items + room.n[s] - 1) / room.n[s];
             const double stage = 4.0 * n > (32768 + n * 64) / 55.0 ? 4.0 * n : (32768 + n * 64) / 55.0;
-            const double t = (double)waves * ((n_ks + s - 1) / s * stage + (s > 1 ? 8 * stage : 0) + (s == 1 && c > 128 ? 3000 : 0));
+            const double t = (double)waves * ((n_ks + s - 1) / s * stage * (sums && c == 128 ? 1.2 : 1.0) + (s > 1 ? 8 * stage : 0) + (s == 1 && c > 128 ? 3000 : 0));
             if (best == 0 || t < best) { best = t; *cap = c; *parts = s; }
         }
     return a.rows / *cap + groups;
