@@ -232,7 +232,7 @@ constexpr uint32_t GT_A_BYTES = 2 * GT_A_HALF;                   // a CTA's outp
 constexpr uint32_t GT_B_BYTES = 128 * GT_KS * 2;                 // at most: a CTA's half of 256 rows
 constexpr uint32_t GT_STAGE = GT_A_BYTES + GT_B_BYTES;
 constexpr uint32_t GT_MAX_G = 1024;
-constexpr uint32_t GT_EPI_WARPS = 8, GT_GATHER_WARPS = GT_STAGES;   // gathered rows: a warp to a ring slot
+constexpr uint32_t GT_EPI_WARPS = 8, GT_SLOT_WARPS = 2, GT_GATHER_WARPS = GT_SLOT_WARPS * GT_STAGES;   // gathered rows: two warps to a ring slot
 constexpr uint32_t GT_THREADS = 64 + (GT_EPI_WARPS + GT_GATHER_WARPS) * 32;
 constexpr uint32_t GT_TURN = 8 * 32 * 4;                         // an epilogue warp's turn of 16 rows x 32 outputs, two rows to a word
 constexpr uint32_t GT_SMEM = GT_STAGES * GT_STAGE + GT_EPI_WARPS * 2 * GT_TURN + 1024;
@@ -322,7 +322,7 @@ template <bool SWIGLU, class O>
 __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __grid_constant__ TileParams P) {
     extern __shared__ uint8_t smem_any[];
     __shared__ __align__(8) uint64_t full_bar[GT_STAGES], empty_bar[GT_STAGES], acc_full[2], acc_empty[2];
-    __shared__ uint32_t s_tmem, s_off[2 * GT_MAX_G], s_tiles[GT_MAX_G + 1], s_row[GT_GATHER_WARPS][128];
+    __shared__ uint32_t s_tmem, s_off[2 * GT_MAX_G], s_tiles[GT_MAX_G + 1], s_row[GT_GATHER_WARPS][128 / GT_SLOT_WARPS];
     __shared__ volatile int s_abort;
     const GroupedArgs& a = P.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
     const uint16_t pair_mask = (uint16_t)(3u << leader);
     const uint32_t ring = (smem_u32(smem_any) + 1023u) & ~1023u;
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < GT_STAGES; ++s) { mbar_init(&full_bar[s], a.gather ? 3 : 1); mbar_init(&empty_bar[s], 1); }
+        for (uint32_t s = 0; s < GT_STAGES; ++s) { mbar_init(&full_bar[s], a.gather ? 1 + 2 * GT_SLOT_WARPS : 1); mbar_init(&empty_bar[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * GT_EPI_WARPS); }
         s_abort = 0;
         mbar_fence_init();
@@ -564,9 +564,9 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
             if (!ok) break;
         }
     } else if (a.gather) {
-        // ---------------- gathered rows: a warp to a ring slot, so that waiting for its copies keeps nobody; eight lanes copy 128 bytes of a row ----------------
+        // ---------------- gathered rows: two warps to a ring slot, so that waiting for its copies keeps nobody; eight lanes copy 128 bytes of a row ----------------
         // (one arrival per warp and stage: with one per thread, posted by the copies themselves, the arrivals took longer than the stage)
-        const uint32_t slot = warp - 2 - GT_EPI_WARPS, r_in = lane >> 3, chunk = lane & 7u;
+        const uint32_t gw = warp - 2 - GT_EPI_WARPS, slot = gw % GT_STAGES, share = gw / GT_STAGES, r_in = lane >> 3, chunk = lane & 7u;
         const uint32_t sb = ring + slot * GT_STAGE + GT_A_BYTES, full = map_to_rank(smem_u32(&full_bar[slot]), leader);
         uint32_t ph = 0, base = 0;                                // stages of the items before, modulo the ring
         bool ok = true;
@@ -575,9 +575,11 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
             // this CTA's rows of the tile; what the columns behind the tile's last row hold is not stored
             const uint32_t hb = it.n / 2, t0 = rank * hb, valid = it.rows > t0 ? min(hb, it.rows - t0) : 0;
             __syncwarp();
-            for (uint32_t r = lane; r < valid; r += 32) {
-                const uint32_t xr = a.order[it.p0 + t0 + r] / a.x_div;
-                s_row[slot][r] = xr < a.x_rows ? xr : 0;          // out of range: reads row 0, the epilogue skips it
+            // every second row is this warp's
+            const uint32_t mine = (valid + GT_SLOT_WARPS - 1 - share) / GT_SLOT_WARPS;
+            for (uint32_t r = lane; r < mine; r += 32) {
+                const uint32_t xr = a.order[it.p0 + t0 + r * GT_SLOT_WARPS + share] / a.x_div;
+                s_row[gw][r] = xr < a.x_rows ? xr : 0;            // out of range: reads row 0, the epilogue skips it
             }
             __syncwarp();
             for (uint32_t ks = ks0 + (slot + GT_STAGES - base) % GT_STAGES; ks < ks1; ks += GT_STAGES) {
@@ -586,8 +588,10 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                 const bool there = k < a.K;                       // K is a multiple of 8
                 const uint16_t* x = static_cast<const uint16_t*>(a.x) + (there ? k : 0);
 #pragma unroll 8
-                for (uint32_t r = r_in; r < valid; r += 4)
-                    cp_async16(sb + r * 128 + ((chunk ^ (r & 7u)) << 4), x + (size_t)s_row[slot][r] * a.ld_x, there);
+                for (uint32_t i = r_in; i < mine; i += 4) {
+                    const uint32_t r = i * GT_SLOT_WARPS + share;
+                    cp_async16(sb + r * 128 + ((chunk ^ (r & 7u)) << 4), x + (size_t)s_row[gw][i] * a.ld_x, there);
+                }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_async_smem();
                 __syncwarp();
