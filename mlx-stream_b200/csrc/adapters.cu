@@ -592,9 +592,9 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const A
     }
 }
 
-// More tokens: every CTA sorts the ids of a segment of up to 2048 tokens in its own shared memory (stable, so that all CTAs have the same order),
+// More tokens: every CTA sorts the ids of a segment of up to 1024 tokens in its own shared memory (stable, so that all CTAs have the same order),
 // then the segment's clusters take units of one adapter and up to 64 of its tokens, wherever they lie.
-constexpr uint32_t AD_SEG = 2048, AD_PLACES = 512;                   // tokens of a segment; adapters that are counted, and none
+constexpr uint32_t AD_SEG = 1024, AD_PLACES = 512;                   // tokens of a segment; adapters that are counted, and none
 struct AdSort {                          // dynamic shared memory behind AdSmem
     uint32_t first[AD_PLACES + 1];       // first token in the order (low half), first unit (high half)
     uint16_t cursor[AD_WARPS][AD_PLACES];
@@ -772,11 +772,6 @@ __device__ __forceinline__ void ab_expect(uint32_t bar, uint32_t bytes) {   // b
 __device__ __forceinline__ void ab_copy(uint32_t dst, const void* src, uint32_t n) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n));
 }
-template <class O> struct AbBase;        // four outputs of base
-template <> struct AbBase<float> { typedef uint4 Word; };
-template <> struct AbBase<__nv_bfloat16> { typedef uint2 Word; };
-template <> struct AbBase<__half> { typedef uint2 Word; };
-
 template <class T, class O>
 __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapters_tensor_kernel(const __grid_constant__ AbParams P) {
     extern __shared__ uint8_t smem_any[];
@@ -880,17 +875,19 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
             const uint32_t R = rank_of(un.place), chunks = (R + 63) / 64;
             if (R) {
                 wait(&d1_empty, (n_done & 1u) ^ 1u, ST_WAIT_EMPTY);
+                uint32_t d1 = tmem, in_chain = 0;
                 for (uint32_t ks = ks0; ks < ks1 && ok; ++ks) {
                     wait(&full_bar[s], ph, ST_WAIT_FULL);
                     if (!ok) break;
                     const uint32_t at = __shfl_sync(0xFFFFFFFFu, (ring + s * L.slot) >> 4, 0) | 1u << 16, x_at = at + (L.x >> 4);
                     if (elect_one()) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) umma_f16_lo(tmem + (ks - ks0) / per_chain * 64, at + j * 2, x_at + j * 2, UMMA_SW128_HI, idesc, (ks - ks0) % per_chain || j ? 1u : 0u);
+                        for (uint32_t j = 0; j < 4; ++j) umma_f16_lo(d1, at + j * 2, x_at + j * 2, UMMA_SW128_HI, idesc, in_chain | j ? 1u : 0u);
                         umma_commit(&empty_bar[s]);
                     }
                     __syncwarp();
                     next();
+                    if (++in_chain == per_chain) { in_chain = 0; d1 += 64; }
                 }
                 if (!ok) break;
                 if (elect_one()) umma_commit(&d1_full);
@@ -982,27 +979,27 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
             if (!together()) break;
             if (etid == 0) mbar_arrive(&u_go);
             ++n_done;
-            // outputs: a lane four of a token, eight lanes a token's 32, a warp four tokens at a time
-            const uint32_t i0 = half * 32 + (lane >> 3), f4 = q * 32 + (lane & 7u) * 4;
-            uint32_t rows[8];
+            // outputs: a lane eight of a token, four lanes a token's 32, a warp eight tokens at a time
+            constexpr int V = sizeof(O) / 2;                          // 16-byte words of eight outputs
+            const uint32_t i0 = half * 32 + (lane >> 2), f8 = q * 32 + (lane & 3u) * 8;
+            uint32_t rows[4];
 #pragma unroll
-            for (uint32_t k = 0; k < 8; ++k) rows[k] = t0 + so.order[un.at + min(i0 + k * 4, un.rows - 1)];
-            typename AbBase<O>::Word b[2][4];
+            for (uint32_t k = 0; k < 4; ++k) rows[k] = t0 + so.order[un.at + min(i0 + k * 8, un.rows - 1)];
+            uint4 b[4][V];
             auto ask_base = [&](uint32_t fb) {
-                const uint32_t f = fb * 128 + f4;
+                const uint32_t f = fb * 128 + f8;
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
+                for (uint32_t k = 0; k < 4; ++k)
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        const uint32_t i = i0 + h * 16 + j * 4;
-                        b[h][j] = {};
-                        if (a.base && fb < fb1 && f < a.N && i < un.rows)
-                            b[h][j] = *reinterpret_cast<const typename AbBase<O>::Word*>(static_cast<const O*>(a.base) + (size_t)rows[h * 4 + j] * a.ld_base + f);
+                    for (int v = 0; v < V; ++v) {
+                        b[k][v] = make_uint4(0, 0, 0, 0);
+                        if (a.base && fb < fb1 && f < a.N && i0 + k * 8 < un.rows)
+                            b[k][v] = *reinterpret_cast<const uint4*>(static_cast<const O*>(a.base) + (size_t)rows[k] * a.ld_base + f + v * (8 / V));
                     }
             };
             ask_base(fb0);
             for (uint32_t fb = fb0; fb < fb1 && ok; ++fb, ++n_blocks) {
-                const uint32_t buf = n_blocks & 1u, f = fb * 128 + f4;
+                const uint32_t buf = n_blocks & 1u, f = fb * 128 + f8;
                 const bool in = f < a.N;
                 if (!wait(&d2_full[buf], n_blocks >> 1 & 1u)) break;
                 tc_fence_after();
@@ -1015,24 +1012,32 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
 #pragma unroll
                     for (uint32_t j = 0; j < 16; ++j) asm volatile("st.shared.u32 [%0], %1;" ::"r"(turn + (j * 32 + lane) * 4), "r"(v[j]) : "memory");
                     __syncwarp();
-                    uint4 turned[4];                     // all read before the first is used
+                    uint4 turned[2][2];                  // all read before the first is used
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) turned[j] = ad_lds16(turn + ((lane >> 3) + j * 4) * 128 + (lane & 7u) * 16);
+                    for (uint32_t j = 0; j < 2; ++j)
 #pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        const uint32_t i = i0 + h * 16 + j * 4;
-                        const uint4 w = turned[j];
+                        for (uint32_t k = 0; k < 2; ++k) turned[j][k] = ad_lds16(turn + ((lane >> 2) + j * 8) * 128 + (lane & 3u) * 32 + k * 16);
+#pragma unroll
+                    for (uint32_t j = 0; j < 2; ++j) {
+                        const uint32_t i = i0 + h * 16 + j * 8;
                         if (!in || i >= un.rows) continue;
                         const float s = std::is_same<T, __half>::value ? s_scale[i] : 1.f;
-                        O* y = static_cast<O*>(a.y) + (size_t)rows[h * 4 + j] * a.ld_y + f;
+                        const uint4 w0 = turned[j][0], w1 = turned[j][1];
+                        uint4* y = reinterpret_cast<uint4*>(static_cast<O*>(a.y) + (size_t)rows[h * 2 + j] * a.ld_y + f);
                         if constexpr (sizeof(O) == 4) {
-                            const uint4 c = b[h][j];
-                            *reinterpret_cast<float4*>(y) = make_float4(fmaf(__uint_as_float(w.x), s, __uint_as_float(c.x)), fmaf(__uint_as_float(w.y), s, __uint_as_float(c.y)),
-                                                                       fmaf(__uint_as_float(w.z), s, __uint_as_float(c.z)), fmaf(__uint_as_float(w.w), s, __uint_as_float(c.w)));
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const uint4 w = k ? w1 : w0, c = b[h * 2 + j][k];
+                                y[k] = make_uint4(__float_as_uint(fmaf(__uint_as_float(w.x), s, __uint_as_float(c.x))), __float_as_uint(fmaf(__uint_as_float(w.y), s, __uint_as_float(c.y))),
+                                                  __float_as_uint(fmaf(__uint_as_float(w.z), s, __uint_as_float(c.z))), __float_as_uint(fmaf(__uint_as_float(w.w), s, __uint_as_float(c.w))));
+                            }
                         } else {
-                            const float2 c0 = ad_unpack(b[h][j].x, O()), c1 = ad_unpack(b[h][j].y, O());
-                            *reinterpret_cast<uint2*>(y) = make_uint2(ad_pack(fmaf(__uint_as_float(w.x), s, c0.x), fmaf(__uint_as_float(w.y), s, c0.y), O()),
-                                                                     ad_pack(fmaf(__uint_as_float(w.z), s, c1.x), fmaf(__uint_as_float(w.w), s, c1.y), O()));
+                            const uint4 c = b[h * 2 + j][0];
+                            const float2 c0 = ad_unpack(c.x, O()), c1 = ad_unpack(c.y, O()), c2 = ad_unpack(c.z, O()), c3 = ad_unpack(c.w, O());
+                            *y = make_uint4(ad_pack(fmaf(__uint_as_float(w0.x), s, c0.x), fmaf(__uint_as_float(w0.y), s, c0.y), O()),
+                                            ad_pack(fmaf(__uint_as_float(w0.z), s, c1.x), fmaf(__uint_as_float(w0.w), s, c1.y), O()),
+                                            ad_pack(fmaf(__uint_as_float(w1.x), s, c2.x), fmaf(__uint_as_float(w1.y), s, c2.y), O()),
+                                            ad_pack(fmaf(__uint_as_float(w1.z), s, c3.x), fmaf(__uint_as_float(w1.w), s, c3.y), O()));
                         }
                     }
                 }

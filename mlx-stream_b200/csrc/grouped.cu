@@ -570,18 +570,33 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
         const uint32_t sb = ring + slot * GT_STAGE + GT_A_BYTES, full = map_to_rank(smem_u32(&full_bar[slot]), leader);
         uint32_t ph = 0, base = 0;                                // stages of the items before, modulo the ring
         bool ok = true;
-        for (uint32_t i = pair; i < n_items && ok; i += n_pairs) {
+        // this CTA's rows of an item's tile (what the columns behind the tile's last row hold is not stored), and how many of them are this warp's: every second
+        const auto rows_of = [&](uint32_t i, uint32_t& p0) {
             const GtItem it = walk.at(i / P.n_ft);
-            // this CTA's rows of the tile; what the columns behind the tile's last row hold is not stored
             const uint32_t hb = it.n / 2, t0 = rank * hb, valid = it.rows > t0 ? min(hb, it.rows - t0) : 0;
+            p0 = it.p0 + t0 + share;
+            return (valid + GT_SLOT_WARPS - 1 - share) / GT_SLOT_WARPS;
+        };
+        uint32_t next[128 / GT_SLOT_WARPS / 32], mine = 0;       // the next item's rows: asked for an item ahead
+        const auto ask_rows = [&](uint32_t i) {
+            if (i >= n_items) return 0u;
+            uint32_t p0;
+            const uint32_t n = rows_of(i, p0);
+#pragma unroll
+            for (uint32_t k = 0; k < 128 / GT_SLOT_WARPS / 32; ++k) next[k] = lane + k * 32 < n ? a.order[p0 + (lane + k * 32) * GT_SLOT_WARPS] : 0;
+            return n;
+        };
+        uint32_t n_next = ask_rows(pair);
+        for (uint32_t i = pair; i < n_items && ok; i += n_pairs) {
             __syncwarp();
-            // every second row is this warp's
-            const uint32_t mine = (valid + GT_SLOT_WARPS - 1 - share) / GT_SLOT_WARPS;
-            for (uint32_t r = lane; r < mine; r += 32) {
-                const uint32_t xr = a.order[it.p0 + t0 + r * GT_SLOT_WARPS + share] / a.x_div;
-                s_row[gw][r] = xr < a.x_rows ? xr : 0;            // out of range: reads row 0, the epilogue skips it
+            mine = n_next;
+#pragma unroll
+            for (uint32_t k = 0; k < 128 / GT_SLOT_WARPS / 32; ++k) {
+                const uint32_t xr = next[k] / a.x_div;
+                s_row[gw][lane + k * 32] = xr < a.x_rows ? xr : 0;    // out of range: reads row 0, the epilogue skips it
             }
             __syncwarp();
+            n_next = ask_rows(i + n_pairs);
             for (uint32_t ks = ks0 + (slot + GT_STAGES - base) % GT_STAGES; ks < ks1; ks += GT_STAGES) {
                 if (!mbar_wait_warp_at(smem_u32(&empty_bar[slot]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
                 const uint32_t k = ks * GT_KS + chunk * 8;
