@@ -537,6 +537,8 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const A
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = cluster_rank();
     const uint32_t unit = blockIdx.x / C, tile = unit / slots, slot = unit % slots, t0 = tile * AD_TT;
 
+    grid_dep_wait();
+    grid_dep_launch();
     // the tile's ids and its distinct adapters, in order of their first token
     if (warp < 2) {
         const uint32_t place = t0 + tid < a.T ? ad_place(a, t0 + tid, slot == 0 && rank == 0) : a.n_adapters;
@@ -699,6 +701,8 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
     const uint32_t tid = threadIdx.x, rank = cluster_rank();
     const uint32_t cl = blockIdx.x / C, seg = cl / per_seg, t0 = seg * AD_SEG, n_tok = min(AD_SEG, a.T - t0), n_places = a.n_adapters + 1;
     AdSort& so = *reinterpret_cast<AdSort*>(smem + L.bytes);
+    grid_dep_wait();
+    grid_dep_launch();
     ad_sort(a, so, reinterpret_cast<uint16_t*>(smem), s_scan, t0, n_tok, cl % per_seg == 0 && rank == 0);
     const uint32_t n_units = so.first[n_places] >> 16;
     for (uint32_t u = cl % per_seg; u < n_units; u += per_seg) {
@@ -796,6 +800,8 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         tma_prefetch_map(&P.a);
     }
     if (warp == AD_WARPS) tmem_alloc(&s_tmem, 512);                   // the issuer's warp
+    grid_dep_wait();
+    grid_dep_launch();
     ad_sort(a, so, reinterpret_cast<uint16_t*>(ring_p), s_scan, t0, n_tok, cl % P.per_seg == 0 && rank == 0);
     fence_async_smem();                                               // the sort's scratch was where copies land
     tc_fence_before();
@@ -1060,13 +1066,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
 template <class... Params, class... Args>
 static cudaError_t ad_launch(void (*kernel)(Params...), uint32_t C, uint32_t clusters, uint32_t threads, size_t smem, cudaStream_t st, const Args&... args) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = C; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(C * clusters); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st; cfg.attrs = &attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
+    return e == cudaSuccess ? launch_dependent_clusters(kernel, C, clusters, threads, smem, st, args...) : e;
 }
 template <class T, class O>
 static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {

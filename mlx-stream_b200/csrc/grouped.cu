@@ -164,6 +164,8 @@ __global__ void __launch_bounds__(GN_WARPS * 32, 2) grouped_few_kernel(const Gro
     const uint32_t tid = threadIdx.x, p0 = blockIdx.y, f0 = blockIdx.x * OUTS;
     // the group whose rows begin at p0, if one does
     if (tid == 0) s_group = 0xFFFFFFFFu;
+    grid_dep_wait();
+    grid_dep_launch();
     __syncthreads();
     for (uint32_t g = tid; g < a.G; g += GN_WARPS * 32) {
         uint32_t r0, r1;
@@ -218,8 +220,7 @@ __global__ void __launch_bounds__(GN_WARPS * 32, 2) grouped_few_kernel(const Gro
 template <bool BF16, bool IN_OUT, bool SWIGLU, class O>
 static cudaError_t few_launch(const GroupedArgs& a, cudaStream_t st) {
     constexpr uint32_t OUTS = (IN_OUT ? 64 : 32) / (SWIGLU ? 2 : 1);
-    grouped_few_kernel<BF16, IN_OUT, SWIGLU, O><<<dim3((a.N + OUTS - 1) / OUTS, a.rows), GN_WARPS * 32, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch_dependent(true, grouped_few_kernel<BF16, IN_OUT, SWIGLU, O>, dim3((a.N + OUTS - 1) / OUTS, a.rows), dim3(GN_WARPS * 32), 0, st, a);
 }
 
 // ------------------------------------------------------------------------------------------------------------
@@ -337,6 +338,10 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
         mbar_fence_init();
         tma_prefetch_map(&P.w);
     }
+    if (warp == 1) tmem_alloc_pair(&s_tmem, 512);
+    // what came before on the stream is complete from here on; what follows may start its own beginning
+    grid_dep_wait();
+    grid_dep_launch();
     // the groups' positions and row tiles
     for (uint32_t g = threadIdx.x; g < a.G; g += blockDim.x) {
         uint32_t r0, r1;
@@ -353,8 +358,6 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
         uint32_t at = sum - mine;
         for (uint32_t g = g0; g < g1; ++g) { s_tiles[g] = at; at += (s_off[2 * g + 1] - s_off[2 * g] + P.cap - 1) / P.cap; }
         if (lane == 31) s_tiles[a.G] = sum;
-    } else if (warp == 1) {
-        tmem_alloc_pair(&s_tmem, 512);
     }
     tc_fence_before();
     cluster_sync_all();
@@ -728,12 +731,7 @@ static cudaError_t tile_launch(const GroupedArgs& a, cudaStream_t st) {
         e = encode_map<2>(&P.x[i], a.dtype, a.x, {K, a.x_rows}, {a.ld_x}, {64, gt_box_rows(i)});
     if (e != cudaSuccess) return e;
     const uint32_t clusters = P.parts == 1 ? (uint32_t)a.sm_count / 2 : most_tiles * P.n_ft;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2 * P.parts; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(clusters * 2 * P.parts); cfg.blockDim = dim3(GT_THREADS); cfg.dynamicSmemBytes = GT_SMEM; cfg.stream = st; cfg.attrs = &attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, P);
+    return launch_dependent_clusters(kernel, 2 * P.parts, clusters, GT_THREADS, GT_SMEM, st, P);
 }
 template <bool BF16, class O>
 static cudaError_t grouped_out(const GroupedArgs& a, cudaStream_t st) {
@@ -750,6 +748,8 @@ cudaError_t launch_grouped(const GroupedArgs& a, cudaStream_t st) {
 
 __global__ void __launch_bounds__(256) gate_up_act_kernel(const float* __restrict__ gate_up, uint32_t T, uint32_t I, float limit, __nv_bfloat16* __restrict__ h) {
     const size_t n = (size_t)T * (I / 4);                   // four outputs to a thread
+    grid_dep_wait();
+    grid_dep_launch();
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
         const size_t t = i / (I / 4), f = i % (I / 4) * 4;
         const float4 g = *reinterpret_cast<const float4*>(gate_up + t * 2 * I + f), u = *reinterpret_cast<const float4*>(gate_up + t * 2 * I + I + f);
@@ -760,8 +760,7 @@ __global__ void __launch_bounds__(256) gate_up_act_kernel(const float* __restric
 }
 cudaError_t launch_gate_up_act(const float* gate_up, uint32_t T, uint32_t I, float limit, __nv_bfloat16* h, cudaStream_t st) {
     const size_t blocks = ((size_t)T * (I / 4) + 255) / 256;
-    gate_up_act_kernel<<<(uint32_t)(blocks < 2368 ? blocks : 2368), 256, 0, st>>>(gate_up, T, I, limit, h);
-    return cudaGetLastError();
+    return launch_dependent(true, gate_up_act_kernel, dim3((uint32_t)(blocks < 2368 ? blocks : 2368)), dim3(256), 0, st, gate_up, T, I, limit, h);
 }
 
 }  // namespace mlxs

@@ -569,6 +569,18 @@ def test_shared_expert_with_adapters_in_the_layer_call(T):
     torch.cuda.synchronize()
     assert m.stats().device_status == 0
 
+    # captured into a graph and replayed: the eager bits
+    eager = y.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        m.experts_adapted(0, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, full, aid.data_ptr(), y.data_ptr(),
+                          torch.cuda.current_stream().cuda_stream)
+    for _ in range(2):
+        y.fill_(SENTINEL)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
+
     def low_rank(v, a, b):
         out = torch.zeros(T, b.shape[1], dtype=torch.float64, device="cuda")
         for i in range(n):
