@@ -1,17 +1,19 @@
 // Low-rank adapters of many requests beside a shared projection: y[t] = base[t] + scale_a B_a (A_a x[t]), a = ids[t].
 //
-// Both factors are thin (rank <= 256 of thousands), so the work is bytes: x, base and y once, an adapter's A and B once per 64 tokens that
-// use it; the products themselves (2 R (K + N) per token) are small enough for mma.sync.
-//   * A cluster of C CTAs takes a tile of 64 tokens and, one after the other, the adapters that occur in it (its share of them where few tiles
-//     leave SMs free: the tile's distinct adapters are dealt out over `slots` clusters).  Nothing is sorted and no workspace is held: the
-//     cluster finds an adapter's rows in the tile's 64 ids.
-//   * Inner product u = A x: every CTA sums a C-th of the inputs; its warps split that share again.  The partial sums meet over distributed
-//     shared memory, warps first, then CTAs, always in the same order (no atomics: a call repeats itself).
-//   * u is kept as two 16-bit parts, hi = round(u), lo = round(u - hi): 16 (bf16) or 22 (f16) bits, so what is lost between the factors is far
+// Both factors are thin (rank <= 256 of thousands), so the work is bytes and, for few tokens, latency: x, base and y once, an adapter's A and B once per unit
+// of up to 64 tokens that use it.  A cluster of C CTAs takes a unit: every CTA sums a C-th of the inputs, the sums meet over distributed shared memory
+// (always in the same order, no atomics: a call repeats itself), every CTA then makes a C-th of the outputs.  C is as large as the units leave SMs for.
+//   * Up to 64 tokens, or 512 adapters and more: adapters_tile_kernel, a tile of 64 tokens, whose distinct adapters are dealt out over `slots` clusters.
+//   * More tokens: every CTA sorts the ids of a segment of 2048 tokens by itself, so that an adapter's tokens, wherever they lie, share its units (999
+//     mixed tokens of 24 adapters: 318 us by tiles, 145 sorted).  From 16 tokens per unit on, and ranks to 128, adapters_tensor_kernel (tcgen05);
+//     otherwise adapters_sorted_kernel (mma.sync).
+//   * u = A x is kept as two 16-bit parts, hi = round(u), lo = round(u - hi): 16 (bf16) or 22 (f16) bits, so what is lost between the factors is far
 //     inside an output's rounding.  f16 parts are scaled by the row's largest power of two, since A x may pass f16's range where y does not.
-//   * Outer product y = base + u B^T: every CTA a C-th of the outputs, base added in f32, one rounding.
-// Operands come straight from global memory as mma fragments, 16 bytes per lane: a lane's eight consecutive inputs stand for the k positions
-// 2t, 2t+1, 2t+8, 2t+9 of two products, the same for both operands.
+//   * base is added in f32, one rounding.
+// Measured (GPU time, other inputs every call): one token of rank 16, 5120 -> 2304: 6.7 us, a chain of two cluster barriers and three cold loads; 64 tokens of 48
+// adapters, rank 32: 13 us (floor 2.6); 8192 tokens of six, rank 64, 4096 -> 2048: 52 us (floor 21); 999 of 24, rank 128, f32: 36 us (floor 14).
+// The mma.sync kernels take operands straight from global memory as fragments, 16 bytes per lane: a lane's eight consecutive inputs stand for the k
+// positions 2t, 2t+1, 2t+8, 2t+9 of two products, the same for both operands.
 #include <type_traits>
 
 #include "common.cuh"
@@ -594,9 +596,9 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const A
     }
 }
 
-// More tokens: every CTA sorts the ids of a segment of up to 1024 tokens in its own shared memory (stable, so that all CTAs have the same order),
+// More tokens: every CTA sorts the ids of a segment of up to 2048 tokens in its own shared memory (stable, so that all CTAs have the same order),
 // then the segment's clusters take units of one adapter and up to 64 of its tokens, wherever they lie.
-constexpr uint32_t AD_SEG = 1024, AD_PLACES = 512;                   // tokens of a segment; adapters that are counted, and none
+constexpr uint32_t AD_SEG = 2048, AD_PLACES = 512;                   // tokens of a segment; adapters that are counted, and none
 struct AdSort {                          // dynamic shared memory behind AdSmem
     uint32_t first[AD_PLACES + 1];       // first token in the order (low half), first unit (high half)
     uint16_t cursor[AD_WARPS][AD_PLACES];
@@ -728,9 +730,13 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
 // the adapter's rank).  A warp to a ring slot, one that issues the products, eight that read accumulators: inner sums -> shared memory -> the cluster's fold ->
 // parts of u as operand rows; outputs -> turned through shared memory -> + base -> y.  The fold's steps are joined by mbarriers between the CTAs, so the
 // ring runs on underneath.  Every wait is bounded: a give-up sets the status word, and everybody still meets at the end.
+// 8192 tokens of six adapters, rank 64, 4096 -> 2048, in cycles: sort 8,500, start 3,500, inner 35,000 (the issuer: 400 for a stage's four small MMAs), fold
+// 7,000, outer 40,000 (16 blocks of 128 outputs; each a chain of tensor-memory read, turn, base and store over eight warps): 52 us against 71 with
+// mma.sync.  Measured and not kept: base through the ring (52 -> 51 us, rank 128 with f32 outputs 36 -> 51), prefetches of x and base into L2 (their issue
+// takes what they save), 64-byte pieces of base one block further ahead.
 // The inner product's accumulator truncates (see the grouped products): its inputs are dealt out in order to up to six accumulators, added in f32.
 constexpr uint32_t AB_CHAIN = 8, AB_CHAINS = 6, AB_D2 = AB_CHAINS * 64;   // stages, accumulators of 64 columns, the outputs' first column
-constexpr uint32_t AB_MOST_SLOTS = 9, AB_MAX_R = 128, AB_MIN_ROWS = 16;   // from so many tokens per unit on
+constexpr uint32_t AB_MOST_SLOTS = 9, AB_MAX_R = 128, AB_MIN_ROWS = 16, AB_MIN_R = 40;   // from so many tokens per unit, and ranks, on
 constexpr uint32_t AB_U_BYTES = 64 * 128;                            // one part of 64 rank columns of the unit's tokens
 constexpr uint32_t AB_TURN = 16 * 32 * 4;                            // an epilogue warp's turn of 16 tokens x 32 outputs
 struct AbSmem {
@@ -799,9 +805,9 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         mbar_fence_init();
         tma_prefetch_map(&P.a);
     }
-    if (warp == AD_WARPS) tmem_alloc(&s_tmem, 512);                   // the issuer's warp
-    grid_dep_wait();
+    grid_dep_wait();                                                  // before tensor memory is taken, see the grouped products
     grid_dep_launch();
+    if (warp == AD_WARPS) tmem_alloc(&s_tmem, 512);                   // the issuer's warp
     ad_sort(a, so, reinterpret_cast<uint16_t*>(ring_p), s_scan, t0, n_tok, cl % P.per_seg == 0 && rank == 0);
     fence_async_smem();                                               // the sort's scratch was where copies land
     tc_fence_before();
@@ -1068,6 +1074,24 @@ static cudaError_t ad_launch(void (*kernel)(Params...), uint32_t C, uint32_t clu
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     return e == cudaSuccess ? launch_dependent_clusters(kernel, C, clusters, threads, smem, st, args...) : e;
 }
+// clusters of 1, 2, 4, 8 CTAs of the tensor-core kernel that the device holds at once
+struct AbClusters { uint32_t n[9]; };
+static AbClusters ab_clusters(const void* kernel, int sm_count) {
+    AbClusters c{};
+    const AbSmem L = ab_smem(AB_MAX_R);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L.bytes);
+    for (uint32_t C = 1; C <= 8; C *= 2) {
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = C; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(C * 148); cfg.blockDim = dim3(L.threads()); cfg.dynamicSmemBytes = L.bytes; cfg.attrs = &attr; cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = sm_count / (int)C; }
+        c.n[C] = n > 0 ? (uint32_t)n : 1u;
+    }
+    return c;
+}
 template <class T, class O>
 static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     const AdSmem L = ad_smem(a.R, a.T);
@@ -1084,14 +1108,18 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     const uint32_t segs = (a.T + AD_SEG - 1) / AD_SEG, tokens = a.T < AD_SEG ? a.T : AD_SEG;
     // a segment's units: about as many as it has adapters, or 64 tokens
     const uint32_t units = tokens / AD_TT > a.n_adapters ? tokens / AD_TT : a.n_adapters < tokens ? a.n_adapters : tokens;
-    if (a.R <= AB_MAX_R && tokens >= AB_MIN_ROWS * units) {
+    // 5120 -> 2304, mma.sync against tensor cores: rank 32: 256 tokens of 16 adapters 15.2 and 19.5 us, 1000 of 32 26 and 24, 4000 of 8 61 and 59, 8192 of
+    // 6 94 and 101; rank 64: 19.4 and 20.0, 34 and 25, 84 and 60, 128 and 101; rank 128: 35 and 22, 59 and 29, 145 and 65, 224 and 112.  Eight tokens per
+    // unit, rank 32: 16 and 22 (256 of 32), 64 and 93 (4000 of 64).
+    if (a.R >= AB_MIN_R && a.R <= AB_MAX_R && tokens >= AB_MIN_ROWS * units) {
         AbParams P;
         P.p = a;
         cudaError_t e = encode_map<3>(&P.a, a.dtype, a.a, {a.K, a.R, a.n_adapters}, {a.K, a.a_stride}, {64, a.R, 1});
         if (e != cudaSuccess) return e;
-        P.C = spread((uint64_t)units * segs, sms, 1);
-        while (P.C > (a.K + 63) / 64) P.C /= 2;                     // every CTA has inputs to sum
-        P.per_seg = sms / (P.C * segs);
+        static const AbClusters room1 = ab_clusters(reinterpret_cast<const void*>(adapters_tensor_kernel<T, O>), a.sm_count);   // an SM holds one CTA
+        P.C = 8;
+        while (P.C > 1 && ((uint64_t)units * segs > room1.n[P.C] || P.C > (a.K + 63) / 64)) P.C /= 2;   // every CTA has inputs to sum
+        P.per_seg = room1.n[P.C] / segs;
         P.per_seg = P.per_seg < 1 ? 1 : P.per_seg > units + tokens / AD_TT + 1 ? units + tokens / AD_TT + 1 : P.per_seg;
         return ad_launch(adapters_tensor_kernel<T, O>, P.C, P.per_seg * segs, ab_smem(a.R).threads(), ab_smem(a.R).bytes, st, P);
     }

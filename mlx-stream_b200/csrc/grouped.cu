@@ -1,12 +1,16 @@
-// Products grouped by expert over 16-bit weights: y[p] = W_g x[p] for offsets[g] <= p < offsets[g + 1], or SwiGLU of a
-// gate and an up product of the same rows.
+// Products grouped by expert over 16-bit weights: y[p] = W_g x[p] for offsets[g] <= p < offsets[g + 1], or SwiGLU of a gate and an up product of the
+// same rows.  Weights row-major, outputs or inputs first, nothing laid out anew; rows may be gathered and scattered on the way.  Two kernels, by
+// the call's rows alone (the groups' sizes are on the device):
+//   * up to 16 rows: grouped_few_kernel streams the weights through mma.sync (bound: HBM);
+//   * more: grouped_tile_kernel, tcgen05 tiles over CTA pairs.  Many rows per group are bound by the tensor pipe under the power cap, few by HBM:
+//     512 rows over 256 groups (K 2304, N 5120, f32) 0.75 ms = 6.7 TB/s, 1.02 of the measured copy rate, with the same tiles.
+// 17 rows over 64 groups (K 5120, 2 x 2304 outputs): 121 us with the tiles (5.9 TB/s); 16 rows: 105 us streamed (6.3 TB/s) against 126 with the tiles.
 #include "common.cuh"
 #include "kernels.h"
 #include "tensor_map.cuh"
 #include "umma_pair.cuh"
 
 namespace mlxs {
-
 
 // EXACT: the exponential's own function (f32 outputs); without it the product with log2(e) rounds once more, 2^-24 of the exponent,
 // far inside a 16-bit output's half step
@@ -34,6 +38,8 @@ __device__ __forceinline__ bool gp_range(const GroupedArgs& a, uint32_t g, uint3
 // Calls of up to 16 rows (a token's or two tokens' experts): the weights' bytes are everything, and tiles of 512 outputs would leave most SMs
 // without work.  A CTA takes 32 rows of a group's matrix (inputs first: 64) and all the group's rows; its eight warps split the inputs and stream
 // the weights from memory straight into mma fragments, 16 bytes per lane, four blocks ahead.  The warps' sums meet in shared memory, in order.
+// Bound by HBM: one token's eight experts (K 5120, gate and up of 2304) 63 us = 6.0 TB/s, 0.92 of the measured copy rate (82 with the tiles);
+// inputs first 66 us (64-byte runs of a row per warp instead of 64 bytes of eight rows).  One row alone: 14.7 us, latency.
 constexpr uint32_t GN_ROWS = 16, GN_WARPS = 8, GN_AHEAD = 4;
 
 __device__ __forceinline__ uint4 gn_stream16(const void* p) {
@@ -226,6 +232,19 @@ static cudaError_t few_launch(const GroupedArgs& a, cudaStream_t st) {
 // ------------------------------------------------------------------------------------------------------------
 // tensor-core tiles
 // ------------------------------------------------------------------------------------------------------------
+// An item is 512 outputs (activation: 256 and their gates) of up to 256 rows of a group, D[outputs][rows] = W x^T: the weights are the MMA's A operand, so
+// that a ragged last tile pads rows only to 32.  Two CTAs share it (cta_group::2, M = 256): each holds half of the outputs, as two accumulators of 128, and half
+// of the rows' operand.  Per stage of 64 inputs a CTA takes in 48 KB for eight MMAs of 128 cycles: 48 bytes a cycle, where 256 outputs would take 64 and
+// came out 6 % slower at K 8192.  Copies are few and large (one box of weights, one of rows): a stage in six boxes took 398 ns without any MMA, in two 284.
+//   * gate and up are one accumulator each, so a thread has both of an output; the weights' box is gate rows behind up rows (a four-dimensional map);
+//   * weights with the inputs first are M-major operands: boxes of 64 outputs x 64 inputs, the same stage;
+//   * gathered rows come by cp.async, two warps to a ring slot.  Tensor-map gathers (four rows to a copy) take 97 cycles each: 32768 rows 3.0 ms against
+//     1.05 now; one arrival per copying thread on the slot's barrier took longer than the stage (2400 rows 720 us against 400);
+//   * the epilogue packs two rows to a word and turns 16 x 32 outputs through shared memory: 8-byte stores, 64 bytes of a row per warp.
+// Sorted rows, 64 groups of 512, K 4096, gate and up of 2048: 0.86 - 0.94 ms = 1,170 - 1,280 TFLOP/s, the tensor pipe busy 81 - 84 % of the cycles at 1.57 GHz (power
+// cap); one product of 8192^3 0.73 - 0.83 ms where the library's took 0.68 - 0.70.  What is left: a 256-row item has no second accumulator buffer (512 columns are full),
+// so its epilogue (2 - 5 us of 60) stands alone, and 512 rows of a group are often three tiles of 192.
+// Every wait is bounded; on a give-up the CTA sets the status word and still meets the others at the end.
 constexpr uint32_t GT_KS = 64;                                   // inputs per stage: 128 bytes, one swizzle row
 constexpr uint32_t GT_STAGES = 4;
 constexpr uint32_t GT_A_HALF = 128 * GT_KS * 2;                  // 128 outputs of a stage
@@ -250,7 +269,7 @@ struct TileParams {
     CUtensorMap w, x[GT_BOXES];   // x by box height
     GroupedArgs a;
     uint32_t n_ft, n_ks;          // output tiles of a row tile, stages
-    uint32_t cap;                 // most rows of a tile: 128, 160, 192 or 256
+    uint32_t cap;                 // most rows of a tile: 64 (f32 outputs), 128, 160, 192 or 256
     uint32_t w_loads;             // copies that a stage of weights takes
     uint32_t fmt;
     uint32_t parts;               // parts of the reduction, a CTA pair of the item's cluster to each (1: no cluster, pairs walk the items)
@@ -338,10 +357,11 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
         mbar_fence_init();
         tma_prefetch_map(&P.w);
     }
-    if (warp == 1) tmem_alloc_pair(&s_tmem, 512);
-    // what came before on the stream is complete from here on; what follows may start its own beginning
+    // What came before on the stream is complete from here on; what follows may start its own beginning.  Tensor memory is taken only now: a CTA that
+    // held it while it waited could keep it from the grid that it waits for.
     grid_dep_wait();
     grid_dep_launch();
+    if (warp == 1) tmem_alloc_pair(&s_tmem, 512);
     // the groups' positions and row tiles
     for (uint32_t g = threadIdx.x; g < a.G; g += blockDim.x) {
         uint32_t r0, r1;
@@ -680,7 +700,7 @@ static GtClusters gt_clusters(const void* kernel, int sm_count) {
     return c;
 }
 // How a call is cut: rows of a tile at most (128: two accumulator buffers; more: one; the parts' sums fit where the ring was up to 192) and parts of
-// the reduction.  The groups' sizes are on the
+// the reduction (777 rows of one group, K 5120, N 2304: 54 us in one part, 28 in two; 64 rows 29 and 16).  The groups' sizes are on the
 // device; the estimate takes them as equal.  A stage costs its products (4 cycles a row) or its bytes (55 a cycle), whichever is longer; joining parts costs
 // as much as eight stages.  Returns the row tiles that the call can have at most.
 static uint32_t gt_cut(const GroupedArgs& a, uint32_t n_ft, uint32_t n_ks, const GtClusters& room, uint32_t* cap, uint32_t* parts) {
