@@ -700,9 +700,10 @@ static GtClusters gt_clusters(const void* kernel, int sm_count) {
     return c;
 }
 // How a call is cut: rows of a tile at most (128: two accumulator buffers; more: one; the parts' sums fit where the ring was up to 192) and parts of
-// the reduction (777 rows of one group, K 5120, N 2304: 54 us in one part, 28 in two; 64 rows 29 and 16).  The groups' sizes are on the
-// device; the estimate takes them as equal.  A stage costs its products (4 cycles a row) or its bytes (55 a cycle), whichever is longer; joining parts costs
-// as much as eight stages.  Returns the row tiles that the call can have at most.
+// the reduction (one group, K 5120, N 2304: 300 rows 31 us in one part, 22 in two, 18 in four; 777 rows in tiles of 160 38 and 28; 1500 rows in tiles
+// of 128 35 and 45).  The groups' sizes are on the device; the estimate takes them as equal.  A stage costs its products (4.4 cycles a row) or its
+// bytes (62 a cycle), whichever is longer; joining parts costs 50 cycles a row, and what has parts starts anew with each wave of clusters.  Returns the
+// row tiles that the call can have at most.
 static uint32_t gt_cut(const GroupedArgs& a, uint32_t n_ft, uint32_t n_ks, const GtClusters& room, uint32_t* cap, uint32_t* parts) {
     const bool sums = a.out_dtype == DT_F32;          // f32 outputs: 64 rows and two buffers, or 128 and one that the products wait for
     const uint32_t groups = a.G < a.rows ? a.G : a.rows, per = (a.rows + groups - 1) / groups;
@@ -712,8 +713,9 @@ static uint32_t gt_cut(const GroupedArgs& a, uint32_t n_ft, uint32_t n_ks, const
             if (sums ? c > 128 : c == 64) continue;
             const uint32_t tiles = (per + c - 1) / c, n = ((per + tiles - 1) / tiles + 31) / 32 * 32;
             const uint64_t items = (uint64_t)groups * tiles * n_ft, waves = (items + room.n[s] - 1) / room.n[s];
-            const double stage = 4.0 * n > (32768 + n * 64) / 55.0 ? 4.0 * n : (32768 + n * 64) / 55.0;
-            const double t = (double)waves * ((n_ks + s - 1) / s * stage * (sums && c == 128 ? 1.2 : 1.0) + (s > 1 ? 8 * stage : 0) + (s == 1 && c > 128 ? 3000 : 0));
+            const double stage = 4.4 * n > (32768 + n * 64) / 62.0 ? 4.4 * n : (32768 + n * 64) / 62.0;
+            const double wave = (n_ks + s - 1) / s * stage * (sums && c == 128 ? 1.2 : 1.0) + (s > 1 ? 50.0 * n : c > 128 ? 3000 : 0);
+            const double t = waves * wave + (s > 1 ? (waves - 1) * 6000.0 : 0);
             if (best == 0 || t < best) { best = t; *cap = c; *parts = s; }
         }
     return a.rows / *cap + groups;
