@@ -6,6 +6,10 @@ its type is off by half a step more (eps / 2 of its value).  Every element is he
 random walk with a drift: at most n / 16 truncations (one for every 16 inputs that a matrix instruction takes) and sqrt(n) roundings of 2^-23 of the
 result, which is what the relative 2-norm is held to, beside the outputs' half step.
 """
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -380,10 +384,10 @@ def test_adapters_against_64_bits(moe, T, kind):
         c.check((dtype, out))
 
 
-@pytest.mark.parametrize("n, T", [(511, 700), (512, 700), (3, 4096), (3, 4097), (511, 9000), (600, 130), (2, 65)])
+@pytest.mark.parametrize("n, T", [(511, 700), (512, 700), (3, 2048), (3, 2049), (3, 4096), (3, 4097), (511, 9000), (600, 130), (2, 65)])
 @pytest.mark.parametrize("kind", ["mixed", "runs", "same"])
 def test_adapters_many_tokens_and_many_adapters(moe, n, T, kind):
-    """Around the sorting form's limits: 511 adapters, segments of 4096 tokens, units of 64."""
+    """Around the sorting form's limits: 511 adapters, segments of 2048 tokens, units of 64."""
     c = Adapters(some_ids(T, n, kind), n, 8, 40, 24, "bf16", "f32", pad=8)
     c.call(moe)
     c.check()
@@ -600,3 +604,43 @@ def test_shared_expert_with_adapters_in_the_layer_call(T):
     assert float((y.double() - plain.double()).norm() / plain.double().norm()) > 0.05     # the adapters do something
     bare = aid < 0
     assert float((y[bare].double() - none[bare].double()).abs().max() if bare.any() else 0.0) == 0.0
+
+
+FIRST_CALLS = """
+import sys, torch
+from __graft_entry__ import load_package
+pkg = load_package()
+moe = pkg.MoE(pkg.make_config(128, 128, 4, 1, max_tokens=4))
+rows, T = int(sys.argv[1]), int(sys.argv[2])
+x = torch.randn(rows, 256, device="cuda").bfloat16()
+w = torch.randn(2, 136, 256, device="cuda").bfloat16()
+offsets = torch.tensor([0, rows // 2, rows], device="cuda", dtype=torch.int32)
+y = torch.zeros(rows, 136, device="cuda", dtype=torch.bfloat16)
+a, b = torch.randn(2, 64, 256, device="cuda").bfloat16(), torch.randn(2, 136, 64, device="cuda").bfloat16()
+ids = (torch.arange(T, device="cuda") % 2).to(torch.int32)
+z = torch.zeros(T, 136, device="cuda", dtype=torch.bfloat16)
+def calls():
+    s = torch.cuda.current_stream().cuda_stream
+    moe.grouped(x.data_ptr(), w.data_ptr(), offsets.data_ptr(), y.data_ptr(), rows, 2, 256, 136, stream=s)
+    moe.adapters(x.data_ptr(), T, a.data_ptr(), b.data_ptr(), ids.data_ptr(), z.data_ptr(), 256, 136, 64, 2, stream=s)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    calls()
+assert not y.any() and not z.any()
+g.replay()
+torch.cuda.synchronize()
+first = y.clone(), z.clone()
+y.zero_(); z.zero_()
+calls()
+torch.cuda.synchronize()
+assert torch.equal(first[0], y) and torch.equal(first[1], z) and y.any() and z.any()
+assert moe.stats().device_status == 0
+"""
+
+
+@pytest.mark.parametrize("rows, T", [(9, 5), (200, 130), (300, 70)])
+def test_a_process_whose_first_calls_are_captured(rows, T):
+    """Each kernel's set-up (limits, what fits at once, tensor maps) happens inside the capture."""
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(rows), str(T)], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
