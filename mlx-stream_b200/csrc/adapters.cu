@@ -4,14 +4,14 @@
 // of up to 64 tokens that use it.  A cluster of C CTAs takes a unit: every CTA sums a C-th of the inputs, the sums meet over distributed shared memory
 // (always in the same order, no atomics: a call repeats itself), every CTA then makes a C-th of the outputs.  C is as large as the units leave SMs for.
 //   * Up to 64 tokens, or 512 adapters and more: adapters_tile_kernel, a tile of 64 tokens, whose distinct adapters are dealt out over `slots` clusters.
-//   * More tokens: every CTA sorts the ids of a segment of 2048 tokens by itself, so that an adapter's tokens, wherever they lie, share its units (999
-//     mixed tokens of 24 adapters: 318 us by tiles, 145 sorted).  From 16 tokens per unit on, and ranks to 128, adapters_tensor_kernel (tcgen05);
-//     otherwise adapters_sorted_kernel (mma.sync).
+//   * More tokens (or more than 16 that have 14 per adapter): every CTA sorts the ids of a segment of up to 2048 tokens by itself, so that an adapter's
+//     tokens, wherever they lie, share its units (999 mixed tokens of 24 adapters: 318 us by tiles, 145 sorted).  From 16 tokens per unit on, and ranks
+//     40 to 128, adapters_tensor_kernel (tcgen05); otherwise adapters_sorted_kernel (mma.sync).
 //   * u = A x is kept as two 16-bit parts, hi = round(u), lo = round(u - hi): 16 (bf16) or 22 (f16) bits, so what is lost between the factors is far
 //     inside an output's rounding.  f16 parts are scaled by the row's largest power of two, since A x may pass f16's range where y does not.
 //   * base is added in f32, one rounding.
 // Measured (GPU time, other inputs every call): one token of rank 16, 5120 -> 2304: 6.7 us, a chain of two cluster barriers and three cold loads; 64 tokens of 48
-// adapters, rank 32: 13 us (floor 2.6); 8192 tokens of six, rank 64, 4096 -> 2048: 52 us (floor 21); 999 of 24, rank 128, f32: 36 us (floor 14).
+// adapters, rank 32: 13 us (floor 2.6); 4000 of eight, rank 32: 38 us (floor 12.5); 8192 tokens of six, rank 64, 4096 -> 2048: 55 us (floor 21); 999 of 24, rank 128, f32: 36 us (floor 14).
 // The mma.sync kernels take operands straight from global memory as fragments, 16 bytes per lane: a lane's eight consecutive inputs stand for the k
 // positions 2t, 2t+1, 2t+8, 2t+9 of two products, the same for both operands.
 #include <type_traits>
@@ -518,8 +518,12 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
         ad_outer<T, O, 1>(a, B, R, fb0 + warp, fb1, sh.rows, n_rows, t0, base_s + L.u_hi, base_s + L.u_lo, L.pitch, sh.scale);
     else
         for (uint32_t h = 0; h < n_rows; h += 32)
-            ad_outer<T, O, 2>(a, B, R, fb0 + warp, fb1, sh.rows + h, min(n_rows - h, 32u), t0, base_s + L.u_hi + h * L.pitch, base_s + L.u_lo + h * L.pitch,
-                              L.pitch, sh.scale + h);
+            if (n_rows - h <= 16)
+                ad_outer<T, O, 1>(a, B, R, fb0 + warp, fb1, sh.rows + h, n_rows - h, t0, base_s + L.u_hi + h * L.pitch, base_s + L.u_lo + h * L.pitch, L.pitch,
+                                  sh.scale + h);
+            else
+                ad_outer<T, O, 2>(a, B, R, fb0 + warp, fb1, sh.rows + h, min(n_rows - h, 32u), t0, base_s + L.u_hi + h * L.pitch, base_s + L.u_lo + h * L.pitch,
+                                  L.pitch, sh.scale + h);
     __syncthreads();
 }
 
@@ -615,7 +619,7 @@ __device__ __forceinline__ uint32_t ad_same(uint32_t place, uint32_t bits, bool 
     return same;
 }
 // `scratch`: 2 x AD_SEG x 2 bytes, free again afterwards.  All threads of the CTA (AD_WARPS warps or more; the first AD_WARPS work).
-__device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint16_t* scratch, uint32_t* s_scan, uint32_t t0, uint32_t n_tok, bool report) {
+__device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint16_t* scratch, uint32_t* s_scan, uint32_t t0, uint32_t n_tok, uint32_t tt, bool report) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     // a warp counts the places of its run of tokens, then the runs of a place follow one another
     const uint32_t run_len = (n_tok + AD_WARPS * 32 - 1) / (AD_WARPS * 32) * 32, run0 = warp < AD_WARPS ? warp * run_len : n_tok, run1 = min(run0 + run_len, n_tok);
@@ -639,7 +643,7 @@ __device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint1
         __syncwarp();
     }
     __syncthreads();
-    // two places to a thread: counts and units (64 tokens) summed side by side
+    // two places to a thread: counts and units (up to tt tokens) summed side by side
     uint32_t v[2] = {0, 0}, sum = 0, run = 0;
     if (warp < AD_WARPS) {
 #pragma unroll
@@ -647,7 +651,7 @@ __device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint1
             const uint32_t p = tid * 2 + j;
             uint32_t n = 0;
             for (uint32_t w = 0; w < AD_WARPS; ++w) n += so.cursor[w][p];
-            v[j] = n | ((n + AD_TT - 1) / AD_TT) << 16;
+            v[j] = n | ((n + tt - 1) / tt) << 16;
             sum += v[j];
         }
         run = sum;
@@ -678,13 +682,13 @@ __device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint1
 }
 // unit u of the sorted segment: its place (n_adapters: no adapter), its tokens so.order[at .. at + rows), and the most tokens that a unit of its place has
 struct AdUnit { uint32_t place, at, rows, per; };
-__device__ __forceinline__ AdUnit ad_find(const AdSort& so, uint32_t n_places, uint32_t u) {
+__device__ __forceinline__ AdUnit ad_find(const AdSort& so, uint32_t n_places, uint32_t tt, uint32_t u) {
     uint32_t lo = 0, hi = n_places;
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
         if (so.first[mid] >> 16 <= u) lo = mid; else hi = mid;
     }
-    const uint32_t at = so.first[lo] & 0xFFFFu, n = (so.first[lo + 1] & 0xFFFFu) - at, n_chunks = (n + AD_TT - 1) / AD_TT;
+    const uint32_t at = so.first[lo] & 0xFFFFu, n = (so.first[lo + 1] & 0xFFFFu) - at, n_chunks = (n + tt - 1) / tt;
     AdUnit r;
     r.place = lo;
     r.per = (n + n_chunks - 1) / n_chunks;
@@ -695,20 +699,20 @@ __device__ __forceinline__ AdUnit ad_find(const AdSort& so, uint32_t n_places, u
 }
 
 template <class T, class O>
-__global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const AdaptersArgs a, const uint32_t C, const uint32_t per_seg) {
+__global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const AdaptersArgs a, const uint32_t C, const uint32_t per_seg, const uint32_t seg_len, const uint32_t tt) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ AdShared sh;
     __shared__ uint32_t s_scan[AD_WARPS];
     const AdSmem L = ad_smem(a.R, a.T);
     const uint32_t tid = threadIdx.x, rank = cluster_rank();
-    const uint32_t cl = blockIdx.x / C, seg = cl / per_seg, t0 = seg * AD_SEG, n_tok = min(AD_SEG, a.T - t0), n_places = a.n_adapters + 1;
+    const uint32_t cl = blockIdx.x / C, seg = cl / per_seg, t0 = seg * seg_len, n_tok = min(seg_len, a.T - t0), n_places = a.n_adapters + 1;
     AdSort& so = *reinterpret_cast<AdSort*>(smem + L.bytes);
     grid_dep_wait();
     grid_dep_launch();
-    ad_sort(a, so, reinterpret_cast<uint16_t*>(smem), s_scan, t0, n_tok, cl % per_seg == 0 && rank == 0);
+    ad_sort(a, so, reinterpret_cast<uint16_t*>(smem), s_scan, t0, n_tok, tt, cl % per_seg == 0 && rank == 0);
     const uint32_t n_units = so.first[n_places] >> 16;
     for (uint32_t u = cl % per_seg; u < n_units; u += per_seg) {
-        const AdUnit un = ad_find(so, n_places, u);
+        const AdUnit un = ad_find(so, n_places, tt, u);
         if (tid < un.rows) sh.rows[tid] = so.order[un.at + tid];
         __syncthreads();
         if (un.place == a.n_adapters) {
@@ -731,7 +735,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
 // parts of u as operand rows; outputs -> turned through shared memory -> + base -> y.  The fold's steps are joined by mbarriers between the CTAs, so the
 // ring runs on underneath.  Every wait is bounded: a give-up sets the status word, and everybody still meets at the end.
 // 8192 tokens of six adapters, rank 64, 4096 -> 2048, in cycles: sort 8,500, start 3,500, inner 35,000 (the issuer: 400 for a stage's four small MMAs), fold
-// 7,000, outer 40,000 (16 blocks of 128 outputs; each a chain of tensor-memory read, turn, base and store over eight warps): 52 us against 71 with
+// 7,000, outer 40,000 (16 blocks of 128 outputs; each a chain of tensor-memory read, turn, base and store over eight warps): 55 us against 71 with
 // mma.sync.  Measured and not kept: base through the ring (52 -> 51 us, rank 128 with f32 outputs 36 -> 51), prefetches of x and base into L2 (their issue
 // takes what they save), 64-byte pieces of base one block further ahead.
 // The inner product's accumulator truncates (see the grouped products): its inputs are dealt out in order to up to six accumulators, added in f32.
@@ -767,7 +771,7 @@ struct AbParts {
 struct AbParams {
     CUtensorMap a;                       // [n_adapters][R][K], boxes of R rows x 64 inputs
     AdaptersArgs p;
-    uint32_t C, per_seg;
+    uint32_t C, per_seg, seg_len;
 };
 __device__ __forceinline__ void ab_tma_3d(uint32_t dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(c0),
@@ -794,7 +798,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
     const uint32_t ring = (smem_u32(smem_any) + 1023u) & ~1023u;
     uint8_t* const ring_p = smem_any + (ring - smem_u32(smem_any));
     const AbSmem L = ab_smem(a.R);
-    const uint32_t cl = blockIdx.x / C, seg = cl / P.per_seg, t0 = seg * AD_SEG, n_tok = min(AD_SEG, a.T - t0), n_places = a.n_adapters + 1;
+    const uint32_t cl = blockIdx.x / C, seg = cl / P.per_seg, t0 = seg * P.seg_len, n_tok = min(P.seg_len, a.T - t0), n_places = a.n_adapters + 1;
     AdSort& so = *reinterpret_cast<AdSort*>(ring_p + L.sort);
     if (tid == 0) {
         for (uint32_t s = 0; s < L.slots; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
@@ -808,7 +812,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
     grid_dep_wait();                                                  // before tensor memory is taken, see the grouped products
     grid_dep_launch();
     if (warp == AD_WARPS) tmem_alloc(&s_tmem, 512);                   // the issuer's warp
-    ad_sort(a, so, reinterpret_cast<uint16_t*>(ring_p), s_scan, t0, n_tok, cl % P.per_seg == 0 && rank == 0);
+    ad_sort(a, so, reinterpret_cast<uint16_t*>(ring_p), s_scan, t0, n_tok, AD_TT, cl % P.per_seg == 0 && rank == 0);
     fence_async_smem();                                               // the sort's scratch was where copies land
     tc_fence_before();
     cluster_sync_all();
@@ -830,7 +834,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         uint32_t ph = 0, base = 0;                                    // stages of the units before, modulo the ring
         bool ok = true;
         for (uint32_t u = cl % P.per_seg; u < n_units && ok; u += P.per_seg) {
-            const AdUnit un = ad_find(so, n_places, u);
+            const AdUnit un = ad_find(so, n_places, AD_TT, u);
             if (un.place == a.n_adapters) continue;
             const uint32_t R = rank_of(un.place), chunks = (R + 63) / 64, n_in = R ? ks1 - ks0 : 0, n_st = n_in + (fb1 - fb0) * chunks;
             const T* const B = static_cast<const T*>(a.b) + (size_t)un.place * a.b_stride;
@@ -882,7 +886,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         };
         auto next = [&]() { if (++s == L.slots) { s = 0; ph ^= 1u; } };
         for (uint32_t u = cl % P.per_seg; u < n_units && ok; u += P.per_seg) {
-            const AdUnit un = ad_find(so, n_places, u);
+            const AdUnit un = ad_find(so, n_places, AD_TT, u);
             if (un.place == a.n_adapters) continue;
             const uint32_t R = rank_of(un.place), chunks = (R + 63) / 64;
             if (R) {
@@ -953,7 +957,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
             return ok;
         };
         for (uint32_t u = cl % P.per_seg; u < n_units && ok; u += P.per_seg) {
-            const AdUnit un = ad_find(so, n_places, u);
+            const AdUnit un = ad_find(so, n_places, AD_TT, u);
             if (un.place == a.n_adapters) { ad_copy<O>(a, so.order + un.at, un.rows, t0, C, rank); continue; }
             const uint32_t R = rank_of(un.place);
             if (!R) {   // outputs are base
@@ -1098,18 +1102,19 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     const uint32_t sms = (uint32_t)a.sm_count, room = 2 * sms;     // CTAs of the mma.sync kernels that run at once
     // a cluster is as large as the units leave SMs for
     const auto spread = [](uint64_t units, uint32_t ctas, uint32_t least) { uint32_t C = 8; while (C > least && units * C > ctas) C /= 2; return C; };
-    if (a.T <= AD_TT || a.n_adapters >= AD_PLACES) {
+    // 5120 -> 2304, tiles against sorted: 64 tokens, rank 16 or 32: of one adapter 15.3 and 9.1 us, of four 11.1 and 9.6, of 16 8.3 and 10.6; 40 of three 9.1 both
+    if (a.T <= 16 || (a.T <= AD_TT && a.T < 14 * (uint64_t)a.n_adapters) || a.n_adapters >= AD_PLACES) {
         const uint32_t tiles = (a.T + AD_TT - 1) / AD_TT, most = a.T < a.n_adapters ? a.T : a.n_adapters, distinct = most < AD_TT ? most : AD_TT;
         const uint32_t C = spread((uint64_t)tiles * distinct, room, 2);
         uint32_t slots = room / (C * tiles);
         slots = slots < 1 ? 1 : slots > distinct ? distinct : slots;
         return ad_launch(adapters_tile_kernel<T, O>, C, slots * tiles, AD_WARPS * 32, L.bytes, st, a, C, slots);
     }
-    const uint32_t segs = (a.T + AD_SEG - 1) / AD_SEG, tokens = a.T < AD_SEG ? a.T : AD_SEG;
+    const uint32_t segs = (a.T + AD_SEG - 1) / AD_SEG, tokens = (a.T + segs - 1) / segs;   // segments all alike
     // a segment's units: about as many as it has adapters, or 64 tokens
     const uint32_t units = tokens / AD_TT > a.n_adapters ? tokens / AD_TT : a.n_adapters < tokens ? a.n_adapters : tokens;
-    // 5120 -> 2304, mma.sync against tensor cores: rank 32: 256 tokens of 16 adapters 15.2 and 19.5 us, 1000 of 32 26 and 24, 4000 of 8 61 and 59, 8192 of
-    // 6 94 and 101; rank 64: 19.4 and 20.0, 34 and 25, 84 and 60, 128 and 101; rank 128: 35 and 22, 59 and 29, 145 and 65, 224 and 112.  Eight tokens per
+    // 5120 -> 2304, mma.sync against tensor cores: rank 32: 256 tokens of 16 adapters 13.0 and 19.5 us, 1000 of 32 26 and 24, 4000 of 8 38 and 59, 8192 of
+    // 6 68 and 101; rank 64: 19.4 and 20.0, 34 and 25, 84 and 60, 128 and 101; rank 128: 35 and 22, 59 and 29, 145 and 65, 224 and 112.  Eight tokens per
     // unit, rank 32: 16 and 22 (256 of 32), 64 and 93 (4000 of 64).
     if (a.R >= AB_MIN_R && a.R <= AB_MAX_R && tokens >= AB_MIN_ROWS * units) {
         AbParams P;
@@ -1118,15 +1123,34 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         static const AbClusters room1 = ab_clusters(reinterpret_cast<const void*>(adapters_tensor_kernel<T, O>), a.sm_count);   // an SM holds one CTA
         P.C = 8;
+        P.seg_len = tokens;
         while (P.C > 1 && ((uint64_t)units * segs > room1.n[P.C] || P.C > (a.K + 63) / 64)) P.C /= 2;   // every CTA has inputs to sum
         P.per_seg = room1.n[P.C] / segs;
         P.per_seg = P.per_seg < 1 ? 1 : P.per_seg > units + tokens / AD_TT + 1 ? units + tokens / AD_TT + 1 : P.per_seg;
         return ad_launch(adapters_tensor_kernel<T, O>, P.C, P.per_seg * segs, ab_smem(a.R).threads(), ab_smem(a.R).bytes, st, P);
     }
-    const uint32_t C = spread((uint64_t)units * segs, room, 2);
+    // Tokens of a unit at most, and CTAs of its cluster.  Ranks to 32: by waves of clusters, each a start (us: 6, or 9 with the ring) and the unit's outputs and
+    // inputs over its CTAs; a unit of up to 16 tokens takes about as long per token as a larger one, and more of them fill the SMs (rank 8 or 32, units
+    // of 64 against the choice: 431 tokens of one adapter, 872 -> 5120, 20 and 12.6 us; 648 of four, 4096 -> 5120, 28 and 19; 4465 of 58, 2304 -> 5120, 92 and 79;
+    // 4000 of eight, 5120 -> 2304, 48 and 38; 4000 of 64 stays at 64: 55, with 16 62).  Larger ranks: an adapter's rows, read once per unit, outweigh 16 tokens.
+    uint32_t tt = AD_TT, C = spread((uint64_t)units * segs, room, 2), cut = units;
+    if (a.R <= 32) {
+        const uint32_t n = a.n_adapters < tokens ? a.n_adapters : tokens;
+        const double one = (3.0 * a.K + 28.0 * a.N) / 5120;
+        double best = 0;
+        for (const uint32_t t : {16u, 32u, 64u}) {
+            const uint32_t most = tokens / t + n / 2 > n ? tokens / t + n / 2 : n;
+            const double rows = (double)tokens / most;
+            for (uint32_t c = 1; c <= 8; c *= 2) {
+                const uint32_t at_once = room / (c * segs) < 1 ? 1 : room / (c * segs);
+                const double us = (most + at_once - 1) / at_once * ((t > 16 && rows > 8 ? 9 : 6) + one * (rows > 16 ? rows / 13 : 1.0) / c);
+                if (best == 0 || us < best) { best = us; tt = t; C = c; cut = most; }
+            }
+        }
+    }
     uint32_t per_seg = room / (C * segs);
-    per_seg = per_seg < 1 ? 1 : per_seg > units + tokens / AD_TT + 1 ? units + tokens / AD_TT + 1 : per_seg;
-    return ad_launch(adapters_sorted_kernel<T, O>, C, per_seg * segs, AD_WARPS * 32, L.bytes + sizeof(AdSort), st, a, C, per_seg);
+    per_seg = per_seg < 1 ? 1 : per_seg > cut + tokens / tt + 1 ? cut + tokens / tt + 1 : per_seg;
+    return ad_launch(adapters_sorted_kernel<T, O>, C, per_seg * segs, AD_WARPS * 32, L.bytes + sizeof(AdSort), st, a, C, per_seg, tokens, tt);
 }
 cudaError_t launch_adapters(const AdaptersArgs& a, cudaStream_t st) {
     if (a.dtype == DT_BF16) return a.out_dtype == DT_F32 ? adapters_launch<__nv_bfloat16, float>(a, st) : adapters_launch<__nv_bfloat16, __nv_bfloat16>(a, st);
