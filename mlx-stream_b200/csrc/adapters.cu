@@ -6,7 +6,7 @@
 //   * Up to 64 tokens, or 512 adapters and more: adapters_tile_kernel, a tile of 64 tokens, whose distinct adapters are dealt out over `slots` clusters.
 //   * More tokens (or more than 16 that have 14 per adapter): every CTA sorts the ids of a segment of up to 2048 tokens by itself, so that an adapter's
 //     tokens, wherever they lie, share its units (999 mixed tokens of 24 adapters: 318 us by tiles, 145 sorted).  From 16 tokens per unit on, and ranks
-//     40 to 128, adapters_tensor_kernel (tcgen05); otherwise adapters_sorted_kernel (mma.sync).
+//     40 to 128 where there is enough work, adapters_tensor_kernel (tcgen05); otherwise adapters_sorted_kernel (mma.sync).
 //   * u = A x is kept as two 16-bit parts, hi = round(u), lo = round(u - hi): 16 (bf16) or 22 (f16) bits, so what is lost between the factors is far
 //     inside an output's rounding.  f16 parts are scaled by the row's largest power of two, since A x may pass f16's range where y does not.
 //   * base is added in f32, one rounding.
@@ -740,7 +740,8 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
 // takes what they save), 64-byte pieces of base one block further ahead.
 // The inner product's accumulator truncates (see the grouped products): its inputs are dealt out in order to up to six accumulators, added in f32.
 constexpr uint32_t AB_CHAIN = 8, AB_CHAINS = 6, AB_D2 = AB_CHAINS * 64;   // stages, accumulators of 64 columns, the outputs' first column
-constexpr uint32_t AB_MOST_SLOTS = 9, AB_MAX_R = 128, AB_MIN_ROWS = 16, AB_MIN_R = 40;   // from so many tokens per unit, and ranks, on
+constexpr uint32_t AB_MOST_SLOTS = 9, AB_MAX_R = 128, AB_MIN_ROWS = 16;   // ranks to, tokens per unit from
+constexpr uint32_t AB_LITTLE = 12000;                                // tokens x rank that mma.sync does sooner
 constexpr uint32_t AB_U_BYTES = 64 * 128;                            // one part of 64 rank columns of the unit's tokens
 constexpr uint32_t AB_TURN = 16 * 32 * 4;                            // an epilogue warp's turn of 16 tokens x 32 outputs
 struct AbSmem {
@@ -1099,7 +1100,10 @@ static AbClusters ab_clusters(const void* kernel, int sm_count) {
 template <class T, class O>
 static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     const AdSmem L = ad_smem(a.R, a.T);
-    const uint32_t sms = (uint32_t)a.sm_count, room = 2 * sms;     // CTAs of the mma.sync kernels that run at once
+    const uint32_t sms = (uint32_t)a.sm_count;
+    // CTAs of the mma.sync kernels that run at once: two to an SM (ranks to 128) where their shared memory and the 1 KB
+    // that each costs besides fit twice into 228 KB
+    const uint32_t room = L.bytes + sizeof(AdSort) + sizeof(AdShared) + 1024 + 64 <= 114 * 1024 ? 2 * sms : sms;
     // a cluster is as large as the units leave SMs for
     const auto spread = [](uint64_t units, uint32_t ctas, uint32_t least) { uint32_t C = 8; while (C > least && units * C > ctas) C /= 2; return C; };
     // 5120 -> 2304, tiles against sorted: 64 tokens, rank 16 or 32: of one adapter 15.3 and 9.1 us, of four 11.1 and 9.6, of 16 8.3 and 10.6; 40 of three 9.1 both
@@ -1113,10 +1117,10 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     const uint32_t segs = (a.T + AD_SEG - 1) / AD_SEG, tokens = (a.T + segs - 1) / segs;   // segments all alike
     // a segment's units: about as many as it has adapters, or 64 tokens
     const uint32_t units = tokens / AD_TT > a.n_adapters ? tokens / AD_TT : a.n_adapters < tokens ? a.n_adapters : tokens;
-    // 5120 -> 2304, mma.sync against tensor cores: rank 32: 256 tokens of 16 adapters 13.0 and 19.5 us, 1000 of 32 26 and 24, 4000 of 8 38 and 59, 8192 of
-    // 6 68 and 101; rank 64: 19.4 and 20.0, 34 and 25, 84 and 60, 128 and 101; rank 128: 35 and 22, 59 and 29, 145 and 65, 224 and 112.  Eight tokens per
-    // unit, rank 32: 16 and 22 (256 of 32), 64 and 93 (4000 of 64).
-    if (a.R >= AB_MIN_R && a.R <= AB_MAX_R && tokens >= AB_MIN_ROWS * units) {
+    // mma.sync against tensor cores, 5120 -> 2304: rank 32: 1000 tokens of 32 adapters 27 and 24 us, 4000 of 8 38 and 39; rank 64: 1000 of 32 34 and 25, 4000
+    // of 8 57 and 39; rank 128: 56 and 29, 115 and 42.  Eight tokens per unit, rank 32: 16 and 22 (256 of 32), 55 and 93 (4000 of 64).  Little work: 105 tokens
+    // of three, 2048 -> 4584: rank 64 12.3 and 14.9, rank 96 15.9 and 17.0, rank 128 19.0 and 17.0; 256 of four, rank 64, 15.1 and 15.9, rank 96 24 and 18.
+    if (a.R > 32 && (uint64_t)a.T * a.R > AB_LITTLE && a.R <= AB_MAX_R && tokens >= AB_MIN_ROWS * units) {
         AbParams P;
         P.p = a;
         cudaError_t e = encode_map<3>(&P.a, a.dtype, a.a, {a.K, a.R, a.n_adapters}, {a.K, a.a_stride}, {64, a.R, 1});
@@ -1129,23 +1133,22 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
         P.per_seg = P.per_seg < 1 ? 1 : P.per_seg > units + tokens / AD_TT + 1 ? units + tokens / AD_TT + 1 : P.per_seg;
         return ad_launch(adapters_tensor_kernel<T, O>, P.C, P.per_seg * segs, ab_smem(a.R).threads(), ab_smem(a.R).bytes, st, P);
     }
-    // Tokens of a unit at most, and CTAs of its cluster.  Ranks to 32: by waves of clusters, each a start (us: 6, or 9 with the ring) and the unit's outputs and
-    // inputs over its CTAs; a unit of up to 16 tokens takes about as long per token as a larger one, and more of them fill the SMs (rank 8 or 32, units
-    // of 64 against the choice: 431 tokens of one adapter, 872 -> 5120, 20 and 12.6 us; 648 of four, 4096 -> 5120, 28 and 19; 4465 of 58, 2304 -> 5120, 92 and 79;
-    // 4000 of eight, 5120 -> 2304, 48 and 38; 4000 of 64 stays at 64: 55, with 16 62).  Larger ranks: an adapter's rows, read once per unit, outweigh 16 tokens.
-    uint32_t tt = AD_TT, C = spread((uint64_t)units * segs, room, 2), cut = units;
-    if (a.R <= 32) {
-        const uint32_t n = a.n_adapters < tokens ? a.n_adapters : tokens;
-        const double one = (3.0 * a.K + 28.0 * a.N) / 5120;
-        double best = 0;
-        for (const uint32_t t : {16u, 32u, 64u}) {
-            const uint32_t most = tokens / t + n / 2 > n ? tokens / t + n / 2 : n;
-            const double rows = (double)tokens / most;
-            for (uint32_t c = 1; c <= 8; c *= 2) {
-                const uint32_t at_once = room / (c * segs) < 1 ? 1 : room / (c * segs);
-                const double us = (most + at_once - 1) / at_once * ((t > 16 && rows > 8 ? 9 : 6) + one * (rows > 16 ? rows / 13 : 1.0) / c);
-                if (best == 0 || us < best) { best = us; tt = t; C = c; cut = most; }
-            }
+    // Tokens of a unit at most, and CTAs of its cluster: by waves of clusters, each a start (us: 6, or 9 with the ring) and the unit's outputs and
+    // inputs over its CTAs; a unit of up to 16 tokens takes about as long per token as a larger one (at high ranks more: its A and B are read once), and more of them fill the SMs (units of 64
+    // against the choice: 431 tokens of one adapter, rank 8, 872 -> 5120, 20 and 12.6 us; 648 of four, rank 8, 4096 -> 5120, 28 and 19; 4465 of 58, rank 8,
+    // 2304 -> 5120, 92 and 79; 4000 of eight, rank 32, 5120 -> 2304, 48 and 38; 4000 of 64 stays at 64: 55, with 16 62;
+    // rank 256: 200 of two, 4096 -> 4096, 72 and 32).
+    uint32_t tt = AD_TT, C = 8, cut = units;
+    const uint32_t n = a.n_adapters < tokens ? a.n_adapters : tokens;
+    const double one = (3.0 * a.K + 28.0 * a.N) / 5120;
+    double best = 0;
+    for (const uint32_t t : {16u, 32u, 64u}) {
+        const uint32_t most = tokens / t + n / 2 > n ? tokens / t + n / 2 : n;
+        const double rows = (double)tokens / most;
+        for (uint32_t c = 1; c <= 8; c *= 2) {
+            const uint32_t at_once = room / (c * segs) < 1 ? 1 : room / (c * segs);
+            const double us = (most + at_once - 1) / at_once * ((t > 16 && rows > 8 ? 9 : 6) + one * (rows > 16 ? rows / (13 + a.R / 32.0) : 1.0) / c);
+            if (best == 0 || us < best) { best = us; tt = t; C = c; cut = most; }
         }
     }
     uint32_t per_seg = room / (C * segs);
