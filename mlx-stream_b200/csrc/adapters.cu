@@ -1134,8 +1134,8 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
         return ad_launch(adapters_tensor_kernel<T, O>, P.C, P.per_seg * segs, ab_smem(a.R).threads(), ab_smem(a.R).bytes, st, P);
     }
     // Tokens of a unit at most, and CTAs of its cluster: by waves of clusters, each a start (us: 6, or 9 with the ring) and the unit's outputs and
-    // inputs over its CTAs; a unit of up to 16 tokens takes about as long per token as a larger one (at high ranks more: its A and B are read once), and more of them fill the SMs (units of 64
-    // against the choice: 431 tokens of one adapter, rank 8, 872 -> 5120, 20 and 12.6 us; 648 of four, rank 8, 4096 -> 5120, 28 and 19; 4465 of 58, rank 8,
+    // inputs over its CTAs; a unit of up to 16 tokens takes about as long per token as a larger one (longer at high ranks: A and B are read once per
+    // unit), and more of them fill the SMs (units of 64 against the choice: 431 tokens of one adapter, rank 8, 872 -> 5120, 20 and 12.6 us; 648 of four, rank 8, 4096 -> 5120, 28 and 19; 4465 of 58, rank 8,
     // 2304 -> 5120, 92 and 79; 4000 of eight, rank 32, 5120 -> 2304, 48 and 38; 4000 of 64 stays at 64: 55, with 16 62;
     // rank 256: 200 of two, 4096 -> 4096, 72 and 32).
     uint32_t tt = AD_TT, C = 8, cut = units;
@@ -1146,8 +1146,9 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
         const uint32_t most = tokens / t + n / 2 > n ? tokens / t + n / 2 : n;
         const double rows = (double)tokens / most;
         for (uint32_t c = 1; c <= 8; c *= 2) {
-            const uint32_t at_once = room / (c * segs) < 1 ? 1 : room / (c * segs);
-            const double us = (most + at_once - 1) / at_once * ((t > 16 && rows > 8 ? 9 : 6) + one * (rows > 16 ? rows / (13 + a.R / 32.0) : 1.0) / c);
+            const uint32_t at_once = room / (c * segs);              // of a segment's clusters
+            const double waves = at_once ? (most + at_once - 1) / at_once : (double)most * c * segs / room;
+            const double us = waves * ((t > 16 && rows > 8 ? 9 : 6) + one * (rows > 16 ? rows / (13 + a.R / 32.0) : 1.0) / c);
             if (best == 0 || us < best) { best = us; tt = t; C = c; cut = most; }
         }
     }
