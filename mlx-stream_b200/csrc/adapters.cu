@@ -3,7 +3,8 @@
 // Both factors are thin (rank <= 256 of thousands), so the work is bytes and, for few tokens, latency: x, base and y once, an adapter's A and B once per unit
 // of up to 64 tokens that use it.  A cluster of C CTAs takes a unit: every CTA sums a C-th of the inputs, the sums meet over distributed shared memory
 // (always in the same order, no atomics: a call repeats itself), every CTA then makes a C-th of the outputs.  C is as large as the units leave SMs for.
-//   * Up to 64 tokens, or 512 adapters and more: adapters_tile_kernel, a tile of 64 tokens, whose distinct adapters are dealt out over `slots` clusters.
+//   * Up to 64 tokens (of 512 adapters and more: up to 511), or 2048 adapters and more: adapters_tile_kernel, a tile of 64 tokens, whose distinct adapters
+//     are dealt out over `slots` clusters.
 //   * More tokens (or more than 16 that have 14 per adapter): every CTA sorts the ids of a segment of up to 2048 tokens by itself, so that an adapter's
 //     tokens, wherever they lie, share its units (999 mixed tokens of 24 adapters: 318 us by tiles, 145 sorted).  From 16 tokens per unit on, and ranks
 //     40 to 128 where there is enough work, adapters_tensor_kernel (tcgen05); otherwise adapters_sorted_kernel (mma.sync).
@@ -602,10 +603,11 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const A
 
 // More tokens: every CTA sorts the ids of a segment of up to 2048 tokens in its own shared memory (stable, so that all CTAs have the same order),
 // then the segment's clusters take units of one adapter and up to 64 of its tokens, wherever they lie.
-constexpr uint32_t AD_SEG = 2048, AD_PLACES = 512;                   // tokens of a segment; adapters that are counted, and none
+constexpr uint32_t AD_SEG = 2048, AD_FEW = 512, AD_MANY = 2048;      // tokens of a segment; adapters that are counted, and none
+template <uint32_t PLACES>
 struct AdSort {                          // dynamic shared memory behind AdSmem
-    uint32_t first[AD_PLACES + 1];       // first token in the order (low half), first unit (high half)
-    uint16_t cursor[AD_WARPS][AD_PLACES];
+    uint32_t first[PLACES + 1];          // first token in the order (low half), first unit (high half)
+    uint16_t cursor[AD_WARPS][PLACES];
     uint16_t order[AD_SEG];
 };
 // the lanes that hold the same place, by one ballot per bit of the largest (a match of whole words took 700 cycles)
@@ -619,11 +621,12 @@ __device__ __forceinline__ uint32_t ad_same(uint32_t place, uint32_t bits, bool 
     return same;
 }
 // `scratch`: 2 x AD_SEG x 2 bytes, free again afterwards.  All threads of the CTA (AD_WARPS warps or more; the first AD_WARPS work).
-__device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint16_t* scratch, uint32_t* s_scan, uint32_t t0, uint32_t n_tok, uint32_t tt, bool report) {
+template <uint32_t PLACES>
+__device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort<PLACES>& so, uint16_t* scratch, uint32_t* s_scan, uint32_t t0, uint32_t n_tok, uint32_t tt, bool report) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     // a warp counts the places of its run of tokens, then the runs of a place follow one another
     const uint32_t run_len = (n_tok + AD_WARPS * 32 - 1) / (AD_WARPS * 32) * 32, run0 = warp < AD_WARPS ? warp * run_len : n_tok, run1 = min(run0 + run_len, n_tok);
-    for (uint32_t i = tid; i < AD_WARPS * AD_PLACES / 2; i += blockDim.x) reinterpret_cast<uint32_t*>(so.cursor)[i] = 0;
+    for (uint32_t i = tid; i < AD_WARPS * PLACES / 2; i += blockDim.x) reinterpret_cast<uint32_t*>(so.cursor)[i] = 0;
     __syncthreads();
     // a token's place, and its number among the run's tokens of that place
     uint16_t* const place_of = scratch;
@@ -643,12 +646,13 @@ __device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint1
         __syncwarp();
     }
     __syncthreads();
-    // two places to a thread: counts and units (up to tt tokens) summed side by side
-    uint32_t v[2] = {0, 0}, sum = 0, run = 0;
+    // a run of places to a thread: counts and units (up to tt tokens) summed side by side
+    constexpr uint32_t MINE = PLACES / (AD_WARPS * 32);
+    uint32_t v[MINE] = {}, sum = 0, run = 0;
     if (warp < AD_WARPS) {
 #pragma unroll
-        for (uint32_t j = 0; j < 2; ++j) {
-            const uint32_t p = tid * 2 + j;
+        for (uint32_t j = 0; j < MINE; ++j) {
+            const uint32_t p = tid * MINE + j;
             uint32_t n = 0;
             for (uint32_t w = 0; w < AD_WARPS; ++w) n += so.cursor[w][p];
             v[j] = n | ((n + tt - 1) / tt) << 16;
@@ -663,8 +667,8 @@ __device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint1
         uint32_t at = run - sum;
         for (uint32_t w = 0; w < warp; ++w) at += s_scan[w];
 #pragma unroll
-        for (uint32_t j = 0; j < 2; ++j) {
-            const uint32_t p = tid * 2 + j;
+        for (uint32_t j = 0; j < MINE; ++j) {
+            const uint32_t p = tid * MINE + j;
             so.first[p] = at;
             uint32_t pos = at & 0xFFFFu;
             for (uint32_t w = 0; w < AD_WARPS; ++w) {
@@ -673,7 +677,7 @@ __device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint1
                 pos += n;
             }
             at += v[j];
-            if (p == AD_PLACES - 1) so.first[AD_PLACES] = at;
+            if (p == PLACES - 1) so.first[PLACES] = at;
         }
     }
     __syncthreads();
@@ -682,7 +686,8 @@ __device__ __forceinline__ void ad_sort(const AdaptersArgs& a, AdSort& so, uint1
 }
 // unit u of the sorted segment: its place (n_adapters: no adapter), its tokens so.order[at .. at + rows), and the most tokens that a unit of its place has
 struct AdUnit { uint32_t place, at, rows, per; };
-__device__ __forceinline__ AdUnit ad_find(const AdSort& so, uint32_t n_places, uint32_t tt, uint32_t u) {
+template <uint32_t PLACES>
+__device__ __forceinline__ AdUnit ad_find(const AdSort<PLACES>& so, uint32_t n_places, uint32_t tt, uint32_t u) {
     uint32_t lo = 0, hi = n_places;
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
@@ -698,7 +703,7 @@ __device__ __forceinline__ AdUnit ad_find(const AdSort& so, uint32_t n_places, u
     return r;
 }
 
-template <class T, class O>
+template <class T, class O, uint32_t PLACES>
 __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const AdaptersArgs a, const uint32_t C, const uint32_t per_seg, const uint32_t seg_len, const uint32_t tt) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ AdShared sh;
@@ -706,7 +711,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
     const AdSmem L = ad_smem(a.R, a.T);
     const uint32_t tid = threadIdx.x, rank = cluster_rank();
     const uint32_t cl = blockIdx.x / C, seg = cl / per_seg, t0 = seg * seg_len, n_tok = min(seg_len, a.T - t0), n_places = a.n_adapters + 1;
-    AdSort& so = *reinterpret_cast<AdSort*>(smem + L.bytes);
+    AdSort<PLACES>& so = *reinterpret_cast<AdSort<PLACES>*>(smem + L.bytes);
     grid_dep_wait();
     grid_dep_launch();
     ad_sort(a, so, reinterpret_cast<uint16_t*>(smem), s_scan, t0, n_tok, tt, cl % per_seg == 0 && rank == 0);
@@ -759,7 +764,7 @@ __host__ __device__ inline AbSmem ab_smem(uint32_t R) {
     s.part = s.u + chunks * 2 * AB_U_BYTES;
     s.turn = s.part + (R + 15) / 16 * 16 * 64 * 4;
     s.sort = s.turn + AD_WARPS * AB_TURN;
-    s.bytes = s.sort + (uint32_t)sizeof(AdSort) + 1024;
+    s.bytes = s.sort + (uint32_t)sizeof(AdSort<AD_FEW>) + 1024;
     return s;
 }
 // operand rows of 64 rank columns, 128 bytes, 16-byte chunks swizzled by the row: [64-column chunk][part][64 tokens]
@@ -800,7 +805,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
     uint8_t* const ring_p = smem_any + (ring - smem_u32(smem_any));
     const AbSmem L = ab_smem(a.R);
     const uint32_t cl = blockIdx.x / C, seg = cl / P.per_seg, t0 = seg * P.seg_len, n_tok = min(P.seg_len, a.T - t0), n_places = a.n_adapters + 1;
-    AdSort& so = *reinterpret_cast<AdSort*>(ring_p + L.sort);
+    AdSort<AD_FEW>& so = *reinterpret_cast<AdSort<AD_FEW>*>(ring_p + L.sort);
     if (tid == 0) {
         for (uint32_t s = 0; s < L.slots; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         mbar_init(&d1_full, 1); mbar_init(&d1_empty, AD_WARPS);
@@ -1103,11 +1108,14 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     const uint32_t sms = (uint32_t)a.sm_count;
     // CTAs of the mma.sync kernels that run at once: two to an SM (ranks to 128) where their shared memory and the 1 KB
     // that each costs besides fit twice into 228 KB
-    const uint32_t room = L.bytes + sizeof(AdSort) + sizeof(AdShared) + 1024 + 64 <= 114 * 1024 ? 2 * sms : sms;
+    const bool few = a.n_adapters < AD_FEW;
+    const uint32_t sort = few ? sizeof(AdSort<AD_FEW>) : sizeof(AdSort<AD_MANY>);
+    const uint32_t room = L.bytes + sort + sizeof(AdShared) + 1024 + 64 <= 114 * 1024 ? 2 * sms : sms;
     // a cluster is as large as the units leave SMs for
     const auto spread = [](uint64_t units, uint32_t ctas, uint32_t least) { uint32_t C = 8; while (C > least && units * C > ctas) C /= 2; return C; };
-    // 5120 -> 2304, tiles against sorted: 64 tokens, rank 16 or 32: of one adapter 15.3 and 9.1 us, of four 11.1 and 9.6, of 16 8.3 and 10.6; 40 of three 9.1 both
-    if (a.T <= 16 || (a.T <= AD_TT && a.T < 14 * (uint64_t)a.n_adapters) || a.n_adapters >= AD_PLACES) {
+    // 5120 -> 2304, tiles against sorted: 64 tokens, rank 16 or 32: of one adapter 15.3 and 9.1 us, of four 11.1 and 9.6, of 16 8.3 and 10.6; 40 of three 9.1 both.
+    // 600 adapters, 4096 -> 2048: 200 tokens, rank 16, 24 and 29, rank 64 46 and 65; 999: 86 and 59, 158 and 144; 8192: 720 and 181, 1320 and 488
+    if (a.T <= 16 || (a.T <= AD_TT && a.T < 14 * (uint64_t)a.n_adapters) || (!few && a.T < 512) || a.n_adapters >= AD_MANY) {
         const uint32_t tiles = (a.T + AD_TT - 1) / AD_TT, most = a.T < a.n_adapters ? a.T : a.n_adapters, distinct = most < AD_TT ? most : AD_TT;
         const uint32_t C = spread((uint64_t)tiles * distinct, room, 2);
         uint32_t slots = room / (C * tiles);
@@ -1120,7 +1128,7 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     // mma.sync against tensor cores, 5120 -> 2304: rank 32: 1000 tokens of 32 adapters 27 and 24 us, 4000 of 8 38 and 39; rank 64: 1000 of 32 34 and 25, 4000
     // of 8 57 and 39; rank 128: 56 and 29, 115 and 42.  Eight tokens per unit, rank 32: 16 and 22 (256 of 32), 55 and 93 (4000 of 64).  Little work: 105 tokens
     // of three, 2048 -> 4584: rank 64 12.3 and 14.9, rank 96 15.9 and 17.0, rank 128 19.0 and 17.0; 256 of four, rank 64, 15.1 and 15.9, rank 96 24 and 18.
-    if (a.R > 32 && (uint64_t)a.T * a.R > AB_LITTLE && a.R <= AB_MAX_R && tokens >= AB_MIN_ROWS * units) {
+    if (a.R > 32 && (uint64_t)a.T * a.R > AB_LITTLE && a.R <= AB_MAX_R && tokens >= AB_MIN_ROWS * units && few) {
         AbParams P;
         P.p = a;
         cudaError_t e = encode_map<3>(&P.a, a.dtype, a.a, {a.K, a.R, a.n_adapters}, {a.K, a.a_stride}, {64, a.R, 1});
@@ -1154,7 +1162,8 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     }
     uint32_t per_seg = room / (C * segs);
     per_seg = per_seg < 1 ? 1 : per_seg > cut + tokens / tt + 1 ? cut + tokens / tt + 1 : per_seg;
-    return ad_launch(adapters_sorted_kernel<T, O>, C, per_seg * segs, AD_WARPS * 32, L.bytes + sizeof(AdSort), st, a, C, per_seg, tokens, tt);
+    return ad_launch(few ? adapters_sorted_kernel<T, O, AD_FEW> : adapters_sorted_kernel<T, O, AD_MANY>, C, per_seg * segs, AD_WARPS * 32, L.bytes + sort, st, a, C,
+                     per_seg, tokens, tt);
 }
 cudaError_t launch_adapters(const AdaptersArgs& a, cudaStream_t st) {
     if (a.dtype == DT_BF16) return a.out_dtype == DT_F32 ? adapters_launch<__nv_bfloat16, float>(a, st) : adapters_launch<__nv_bfloat16, __nv_bfloat16>(a, st);

@@ -384,10 +384,10 @@ def test_adapters_against_64_bits(moe, T, kind):
         c.check((dtype, out))
 
 
-@pytest.mark.parametrize("n, T", [(511, 700), (512, 700), (3, 2048), (3, 2049), (3, 4096), (3, 4097), (511, 9000), (600, 130), (2, 65), (1, 17), (1, 64), (4, 56), (4, 55), (3, 33), (1, 431), (58, 4465), (8, 4000), (5, 300000)])
+@pytest.mark.parametrize("n, T", [(511, 700), (512, 700), (3, 2048), (3, 2049), (3, 4096), (3, 4097), (511, 9000), (600, 130), (2, 65), (1, 17), (1, 64), (4, 56), (4, 55), (3, 33), (1, 431), (58, 4465), (8, 4000), (5, 300000), (600, 511), (600, 512), (600, 5000), (2047, 3000), (2048, 3000)])
 @pytest.mark.parametrize("kind", ["mixed", "runs", "same"])
 def test_adapters_many_tokens_and_many_adapters(moe, n, T, kind):
-    """Around the sorting form's limits: 511 adapters, segments of 2048 tokens, units of 64, 32 or 16; up to 64 tokens: 14 per adapter."""
+    """Around the sorting form's limits: 511 and 2047 adapters, segments of 2048 tokens, units of 64, 32 or 16; up to 64 tokens: 14 per adapter."""
     c = Adapters(some_ids(T, n, kind), n, 8, 40, 24, "bf16", "f32", pad=8)
     c.call(moe)
     c.check()
