@@ -238,7 +238,7 @@ static cudaError_t few_launch(const GroupedArgs& a, cudaStream_t st) {
 // came out 6 % slower at K 8192.  Copies are few and large (one box of weights, one of rows): a stage in six boxes took 398 ns without any MMA, in two 284.
 //   * gate and up are one accumulator each, so a thread has both of an output; the weights' box is gate rows behind up rows (a four-dimensional map);
 //   * weights with the inputs first are M-major operands: boxes of 64 outputs x 64 inputs, the same stage;
-//   * gathered rows come by cp.async, two warps to a ring slot.  Tensor-map gathers (four rows to a copy) take 97 cycles each: 32768 rows 3.0 ms against
+//   * gathered rows come by cp.async into a ring of their own, two warps to a stage.  Tensor-map gathers (four rows to a copy) take 97 cycles each: 32768 rows 3.0 ms against
 //     1.05 now; one arrival per copying thread on the slot's barrier took longer than the stage (2400 rows 720 us against 400);
 //   * the epilogue packs two rows to a word and turns 16 x 32 outputs through shared memory: 8-byte stores, 64 bytes of a row per warp.
 // Sorted rows, 64 groups of 512, K 4096, gate and up of 2048: 0.86 - 0.94 ms = 1,170 - 1,280 TFLOP/s, the tensor pipe busy 81 - 84 % of the cycles at 1.57 GHz (power
@@ -252,7 +252,9 @@ constexpr uint32_t GT_A_BYTES = 2 * GT_A_HALF;                   // a CTA's outp
 constexpr uint32_t GT_B_BYTES = 128 * GT_KS * 2;                 // at most: a CTA's half of 256 rows
 constexpr uint32_t GT_STAGE = GT_A_BYTES + GT_B_BYTES;
 constexpr uint32_t GT_MAX_G = 1024;
-constexpr uint32_t GT_EPI_WARPS = 8, GT_SLOT_WARPS = 2, GT_GATHER_WARPS = GT_SLOT_WARPS * GT_STAGES;   // gathered rows: two warps to a ring slot
+constexpr uint32_t GT_EPI_WARPS = 8, GT_SLOT_WARPS = 2, GT_GATHER_WARPS = GT_SLOT_WARPS * GT_STAGES;   // gathered rows: two warps to a stage, four stages at once
+constexpr uint32_t GT_X_SLOTS = 8;                                // at most: gathered rows have a ring of their own
+constexpr uint32_t GT_X = GT_STAGES * GT_A_BYTES;                // the rows' operand, behind the weights' ring
 constexpr uint32_t GT_THREADS = 64 + (GT_EPI_WARPS + GT_GATHER_WARPS) * 32;
 constexpr uint32_t GT_TURN = 8 * 32 * 4;                         // an epilogue warp's turn of 16 rows x 32 outputs, two rows to a word
 constexpr uint32_t GT_SMEM = GT_STAGES * GT_STAGE + GT_EPI_WARPS * 2 * GT_TURN + 1024;
@@ -341,7 +343,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
 template <bool SWIGLU, class O>
 __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __grid_constant__ TileParams P) {
     extern __shared__ uint8_t smem_any[];
-    __shared__ __align__(8) uint64_t full_bar[GT_STAGES], empty_bar[GT_STAGES], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) uint64_t full_bar[GT_STAGES], empty_bar[GT_STAGES], acc_full[2], acc_empty[2], x_full[GT_X_SLOTS], x_empty[GT_X_SLOTS];
     __shared__ uint32_t s_tmem, s_off[2 * GT_MAX_G], s_tiles[GT_MAX_G + 1], s_row[GT_GATHER_WARPS][128 / GT_SLOT_WARPS];
     __shared__ volatile int s_abort;
     const GroupedArgs& a = P.a;
@@ -351,7 +353,8 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
     const uint16_t pair_mask = (uint16_t)(3u << leader);
     const uint32_t ring = (smem_u32(smem_any) + 1023u) & ~1023u;
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < GT_STAGES; ++s) { mbar_init(&full_bar[s], a.gather ? 1 + 2 * GT_SLOT_WARPS : 1); mbar_init(&empty_bar[s], 1); }
+        for (uint32_t s = 0; s < GT_STAGES; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        for (uint32_t s = 0; s < GT_X_SLOTS; ++s) { mbar_init(&x_full[s], 2 * GT_SLOT_WARPS); mbar_init(&x_empty[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 2 * GT_EPI_WARPS); }
         s_abort = 0;
         mbar_fence_init();
@@ -392,6 +395,8 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
     const uint32_t n_buf = (SUMS ? 128 : 256) / P.cap, n_chains = SUMS ? (ks1 - ks0 + GT_CHAIN - 1) / GT_CHAIN : 1;
     auto give_up = [&](uint32_t code) { if (!s_abort) atomicMax(a.status, code); s_abort = 1; };
     GtWalk walk{s_off, s_tiles, a.G};
+    // gathered rows: as many slots as tiles of at most cap rows leave room for
+    const uint32_t x_slot = P.cap * 64, x_slots = min(GT_STAGES * GT_B_BYTES / x_slot, GT_X_SLOTS);
 
     if (warp == 0) {
         // ---------------- producer: this CTA's outputs' weights, and its half of the tile's rows where they lie in order ----------------
@@ -406,7 +411,7 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
             for (uint32_t ks = ks0; ks < ks1; ++ks) {
                 if (!mbar_wait_warp_at(smem_u32(&empty_bar[s]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
                 if (lane == 0) {
-                    const uint32_t full = map_to_rank(smem_u32(&full_bar[s]), leader), sa = ring + s * GT_STAGE;
+                    const uint32_t full = map_to_rank(smem_u32(&full_bar[s]), leader), sa = ring + s * GT_A_BYTES;
                     const int32_t k = (int32_t)(ks * GT_KS);
                     if (rank == 0) mbar_expect_tx(&full_bar[s], bytes);
                     if (!a.in_out) {
@@ -421,7 +426,7 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
 #pragma unroll
                         for (int j = 0; j < 4; ++j) tma_load_4d(sa + j * (GT_A_HALF / 2), &P.w, f0 + j * 64, k, 0, g, full);
                     }
-                    if (!gather) tma_load_2d(sa + GT_A_BYTES, &P.x[bi], k, (int32_t)b0, full);
+                    if (!gather) tma_load_2d(ring + GT_X + s * GT_B_BYTES, &P.x[bi], k, (int32_t)b0, full);
                 }
                 __syncwarp();
                 if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
     } else if (warp == 1) {
         // ---------------- MMA issuer: the even CTA's, for both ----------------
         if (rank == 0) {
-            uint32_t s = 0, ph = 0, n_done = 0;
+            uint32_t s = 0, ph = 0, xs = 0, x_ph = 0, n_done = 0;
             bool ok = true;
             // K-major: 16 inputs are 32 bytes of every row; M-major: 16 rows of 128 bytes.  M-major 64-output tiles of one accumulator:
             // 8 KB apart, but for the activation's boxes (gate and up of 64 outputs) 16 KB
@@ -448,9 +453,10 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                     tc_fence_after();
                     for (uint32_t ks = k0; ks < k1; ++ks) {
                         ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&full_bar[s]), ph, &s_abort));
+                        if (ok && a.gather) ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&x_full[xs]), x_ph, &s_abort));
                         if (!ok) { give_up(ST_WAIT_FULL); break; }
                         tc_fence_after();
-                        const uint32_t sa = ring + s * GT_STAGE, sb = sa + GT_A_BYTES;
+                        const uint32_t sa = ring + s * GT_A_BYTES, sb = ring + GT_X + (a.gather ? xs * x_slot : s * GT_B_BYTES);
                         if (elect_one()) {
 #pragma unroll
                             for (uint32_t h = 0; h < 2; ++h)
@@ -459,9 +465,11 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                                     umma_f16_pair(acc + h * P.cap, umma_desc_sw128(sa + h * a_next + j * a_step, a_lbo, 1024),
                                                   umma_desc_sw128(sb + j * 32, 16, 1024), idesc, ks != k0 || j ? 1u : 0u);
                             umma_commit_pair(smem_u32(&empty_bar[s]), pair_mask);
+                            if (a.gather) umma_commit_pair(smem_u32(&x_empty[xs]), pair_mask);
                         }
                         __syncwarp();
                         if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
+                        if (++xs == x_slots) { xs = 0; x_ph ^= 1u; }
                     }
                     if (!ok) break;
                     if (elect_one()) umma_commit_pair(smem_u32(&acc_full[buf]), pair_mask);
@@ -587,11 +595,13 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
             if (!ok) break;
         }
     } else if (a.gather) {
-        // ---------------- gathered rows: two warps to a ring slot, so that waiting for its copies keeps nobody; eight lanes copy 128 bytes of a row ----------------
-        // (one arrival per warp and stage: with one per thread, posted by the copies themselves, the arrivals took longer than the stage)
-        const uint32_t gw = warp - 2 - GT_EPI_WARPS, slot = gw % GT_STAGES, share = gw / GT_STAGES, r_in = lane >> 3, chunk = lane & 7u;
-        const uint32_t sb = ring + slot * GT_STAGE + GT_A_BYTES, full = map_to_rank(smem_u32(&full_bar[slot]), leader);
-        uint32_t ph = 0, base = 0;                                // stages of the items before, modulo the ring
+        // ---------------- gathered rows: two warps to every fourth stage, so that waiting for its copies keeps nobody; eight lanes copy 128 bytes of a row ----------------
+        // (one arrival per warp and stage: with one per thread, posted by the copies themselves, the arrivals took longer than the stage).  Their ring is
+        // their own and as deep as the tile's rows allow, so that they are there before the weights: a weights slot that waited for its rows
+        // stood idle meanwhile (K 4096, 2 x 2048 outputs: 2400 Zipf rows of 64
+        // groups 377 us with the rows in the weights' slots, 360 now, 338 in sorted order; 512 rows of 64, K 5120, 490 and 462).
+        const uint32_t gw = warp - 2 - GT_EPI_WARPS, turn = gw % GT_STAGES, share = gw / GT_STAGES, r_in = lane >> 3, chunk = lane & 7u;
+        uint32_t slot = turn, ph = 0, base = 0;                   // base: stages of the items before, modulo the turns
         bool ok = true;
         // this CTA's rows of an item's tile (what the columns behind the tile's last row hold is not stored), and how many of them are this warp's: every second
         const auto rows_of = [&](uint32_t i, uint32_t& p0) {
@@ -620,8 +630,9 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
             }
             __syncwarp();
             n_next = ask_rows(i + n_pairs);
-            for (uint32_t ks = ks0 + (slot + GT_STAGES - base) % GT_STAGES; ks < ks1; ks += GT_STAGES) {
-                if (!mbar_wait_warp_at(smem_u32(&empty_bar[slot]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
+            for (uint32_t ks = ks0 + (turn + GT_STAGES - base) % GT_STAGES; ks < ks1; ks += GT_STAGES) {
+                const uint32_t sb = ring + GT_X + slot * x_slot;
+                if (!mbar_wait_warp_at(smem_u32(&x_empty[slot]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
                 const uint32_t k = ks * GT_KS + chunk * 8;
                 const bool there = k < a.K;                       // K is a multiple of 8
                 const uint16_t* x = static_cast<const uint16_t*>(a.x) + (there ? k : 0);
@@ -633,8 +644,9 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(full);
-                ph ^= 1u;
+                if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&x_full[slot]), leader));
+                slot += GT_STAGES;                                // at most as many as the ring has
+                if (slot >= x_slots) { slot -= x_slots; ph ^= 1u; }
             }
             base = (base + ks1 - ks0) % GT_STAGES;
         }

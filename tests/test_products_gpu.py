@@ -164,6 +164,22 @@ def test_grouped_many_or_one_group(moe, G, rows):
     c.check()
 
 
+@pytest.mark.parametrize("rows, G, K, N", [(320, 2, 4096, 1024), (320, 2, 4096, 4096), (777, 1, 5120, 2304), (1216, 8, 4096, 4096), (3000, 16, 2304, 2048),
+                                           (2400, 16, 1032, 4096), (4000, 30, 328, 4096), (6000, 8, 1032, 4096)])
+def test_grouped_gathered_tiles_of_every_height(moe, rows, G, K, N):
+    """Tiles of 128 to 256 rows, one item of a pair or several, parts of the reduction: rings of gathered rows of every depth."""
+    rng = np.random.default_rng(rows)
+    sizes = np.bincount(rng.integers(0, G, rows), minlength=G).tolist()
+    for out, scatter in (("bf16", True), ("f32", False)):
+        c = Grouped(sizes, K, N, "bf16", out, gather=True, scatter=scatter, x_div=4)
+        c.call(moe)
+        first = c.y_all.clone()
+        c.check(out)
+        c.call(moe)
+        torch.cuda.synchronize()
+        assert torch.equal(c.y_all, first)
+
+
 @pytest.mark.parametrize("rows", [1, 16, 17, 200])
 def test_grouped_one_group_without_offsets(moe, rows):
     c = Grouped([rows], 264, 136)
