@@ -271,7 +271,8 @@ typedef struct {
     uint32_t out_dtype;           /* of y: the same type or MLXS_DTYPE_F32 */
     uint32_t layout;
     uint32_t act;
-    float act_limit;              /* SWIGLU: > 0 cuts the gate from above and the up row from both sides; 0: no limit */
+    float act_limit;              /* SWIGLU: > 0 cuts the gate from above and the up row from both sides; 0: no limit.  PLAIN: 0, a limit
+                                   * without an activation is refused */
     uint32_t n_groups;            /* 1..1024 */
     uint32_t n_in, n_out;         /* multiples of 8, up to 262,144; SWIGLU: a group's matrix has 2 n_out outputs, the gate's first */
     uint32_t rows;                /* sorted positions of the call, up to 2^22; offsets_dev[n_groups] <= rows */

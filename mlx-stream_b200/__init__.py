@@ -360,8 +360,10 @@ class MoE:
                 ld_x=0, ld_y=0, ld_w=0, w_stride=0, stream=None):
         """Products grouped by expert over 16-bit weights: y[p] = W_g x[p] (or SwiGLU of gate and up) for offsets[g] <= p < offsets[g + 1].
         order, offsets: as sort_rows writes them; gather reads row order[p] // x_div of x, scatter writes row order[p] of y.
-        y has the type of x unless out_dtype names another."""
-        d = GroupedDesc(C.sizeof(GroupedDesc), dtype, dtype if out_dtype is None else out_dtype, layout, act, act_limit, n_groups, n_in,
+        y has the type of x unless out_dtype names another.  act_limit is the activation's: without one it says nothing and is not passed on,
+        so a layer's one limit serves its gate-and-up and its down call."""
+        d = GroupedDesc(C.sizeof(GroupedDesc), dtype, dtype if out_dtype is None else out_dtype, layout, act,
+                        act_limit if act != GROUPED_PLAIN else 0.0, n_groups, n_in,
                         n_out, rows, (ROWS_GATHER if gather else 0) | (ROWS_SCATTER if scatter else 0), x_div,
                         rows if x_rows is None else x_rows, rows if y_rows is None else y_rows, ld_x, ld_y, ld_w, w_stride)
         _check(lib().mlxs_moe_grouped(self._h, C.byref(d), x, w, offsets, order, y, stream))

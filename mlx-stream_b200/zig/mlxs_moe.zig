@@ -134,7 +134,7 @@ pub const GroupedDesc = extern struct {
     out_dtype: u32,
     layout: u32,
     act: u32,
-    act_limit: f32 = 0,
+    act_limit: f32 = 0, // of the activation: 0 with .plain
     n_groups: u32,
     n_in: u32,
     n_out: u32,
