@@ -222,8 +222,7 @@ def run(s):
         moe.grouped(s["x"].data_ptr(), s["w"].data_ptr(), s["offsets"].data_ptr(), s["y"].data_ptr(), rows=c["rows"], n_groups=c["groups"],
                     n_in=c["n_in"], n_out=c["n_out"], dtype=kinds[c["dtype"]], out_dtype=kinds[c["out"]],
                     layout=pkg.LAYOUT_OUT_IN if c["layout"] == "out_in" else pkg.LAYOUT_IN_OUT,
-                    act=pkg.GROUPED_SWIGLU if c["act"] == "swiglu" else pkg.GROUPED_PLAIN,
-                    act_limit=c["limit"] if c["act"] == "swiglu" else 0.0,
+                    act=pkg.GROUPED_SWIGLU if c["act"] == "swiglu" else pkg.GROUPED_PLAIN, act_limit=c["limit"],
                     order=s["order"].data_ptr() if c["gather"] or c["scatter"] else None, gather=c["gather"], scatter=c["scatter"],
                     x_div=c["top_k"], x_rows=s["x"].shape[0], y_rows=c["rows"], stream=s["stream"])
     else:
