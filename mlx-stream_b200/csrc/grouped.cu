@@ -38,9 +38,11 @@ __device__ __forceinline__ bool gp_range(const GroupedArgs& a, uint32_t g, uint3
 // Calls of up to 16 rows (a token's or two tokens' experts): the weights' bytes are everything, and tiles of 512 outputs would leave most SMs
 // without work.  A CTA takes 32 rows of a group's matrix (inputs first: 64) and all the group's rows; its eight warps split the inputs and stream
 // the weights from memory straight into mma fragments, 16 bytes per lane, four blocks ahead.  The warps' sums meet in shared memory, in order.
+// The matrix instruction truncates where it adds to its accumulator, so after GN_CHAIN products a warp's accumulators move on to f32 sums in shared memory
+// (f32 outputs against 64 bits with one chain to a warp: K 5120 6.0e-7, gate and up 1.2e-6, 65,536 same-signed inputs 2.5e-5).
 // Bound by HBM: one token's eight experts (K 5120, gate and up of 2304) 63 us = 6.0 TB/s, 0.92 of the measured copy rate (82 with the tiles);
 // inputs first 66 us (64-byte runs of a row per warp instead of 64 bytes of eight rows).  One row alone: 14.7 us, latency.
-constexpr uint32_t GN_ROWS = 16, GN_WARPS = 8, GN_AHEAD = 4;
+constexpr uint32_t GN_ROWS = 16, GN_WARPS = 8, GN_AHEAD = 4, GN_CHAIN = 16;
 
 __device__ __forceinline__ uint4 gn_stream16(const void* p) {
     uint4 v;
@@ -62,6 +64,24 @@ __device__ __forceinline__ void gn_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
     const uint32_t a[4] = {a0, a1, a2, a3};
     if (BF16) mma_bf16(d, a, b0, b1);
     else mma_f16(d, a, b0, b1);
+}
+
+// the accumulators to the warp's sums, row(m, h) and column n of them; they begin anew
+template <int MT, int NT, class Row>
+__device__ __forceinline__ void gn_move(float (&acc)[MT][NT][4], float* out, bool first, Row row) {
+    const uint32_t t = threadIdx.x & 3u;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float2* const o = reinterpret_cast<float2*>(out + row(m, h) * GN_ROWS + n * 8 + 2 * t);
+                float2 v = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
+                if (!first) { const float2 s = *o; v.x += s.x; v.y += s.y; }
+                *o = v;
+                acc[m][n][2 * h] = acc[m][n][2 * h + 1] = 0.f;
+            }
 }
 
 // Outputs first.  W row r of the CTA's 32 (r < 16: m-tile 0) is w + row_of(r) ld_w.  A lane's eight consecutive inputs stand for the k positions 2t,
@@ -87,8 +107,14 @@ __device__ __forceinline__ void gn_out_in(const GroupedArgs& a, const uint16_t* 
     };
 #pragma unroll
     for (uint32_t i = 0; i < GN_AHEAD; ++i) ask(b[i], warp + i * GN_WARPS);
+    // [row of W][row of x], eight columns to a fragment
+    const auto row = [&](int m, int h) { return m * 16 + h * 8 + g; };
+    uint32_t chain = 0;
+    bool first = true;
 #pragma unroll 1
     for (uint32_t kb = warp; kb < n_kb; kb += GN_AHEAD * GN_WARPS) {
+        if (chain == GN_CHAIN) { gn_move<2, NT>(acc, out, first, row); first = false; chain = 0; }
+        chain += 2 * GN_AHEAD;
 #pragma unroll
         for (uint32_t i = 0; i < GN_AHEAD; ++i) {
 #pragma unroll
@@ -102,14 +128,7 @@ __device__ __forceinline__ void gn_out_in(const GroupedArgs& a, const uint16_t* 
             ask(b[i], kb + (GN_AHEAD + i) * GN_WARPS);
         }
     }
-    // [row of W][row of x], eight columns to a fragment
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                *reinterpret_cast<float2*>(out + (m * 16 + h * 8 + g) * GN_ROWS + n * 8 + 2 * t) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
+    gn_move<2, NT>(acc, out, first, row);
 }
 
 // Inputs first: a lane takes eight outputs (lane / 4) of the inputs 4t .. 4t + 3 of a block of 16, which stand for the k positions 2t, 2t+1, 2t+8,
@@ -134,8 +153,13 @@ __device__ __forceinline__ void gn_in_out(const GroupedArgs& a, const uint16_t* 
     };
 #pragma unroll
     for (uint32_t i = 0; i < GN_AHEAD; ++i) ask(b[i], warp + i * GN_WARPS);
+    const auto row = [&](int m, int h) { return g * 8 + 2 * m + h; };
+    uint32_t chain = 0;
+    bool first = true;
 #pragma unroll 1
     for (uint32_t kb = warp; kb < n_kb; kb += GN_AHEAD * GN_WARPS) {
+        if (chain == GN_CHAIN) { gn_move<4, NT>(acc, out, first, row); first = false; chain = 0; }
+        chain += GN_AHEAD;
 #pragma unroll
         for (uint32_t i = 0; i < GN_AHEAD; ++i) {
             const uint32_t r0[4] = {b[i].w[0].x, b[i].w[0].y, b[i].w[0].z, b[i].w[0].w}, r1[4] = {b[i].w[1].x, b[i].w[1].y, b[i].w[1].z, b[i].w[1].w};
@@ -149,13 +173,7 @@ __device__ __forceinline__ void gn_in_out(const GroupedArgs& a, const uint16_t* 
             ask(b[i], kb + (GN_AHEAD + i) * GN_WARPS);
         }
     }
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                *reinterpret_cast<float2*>(out + (g * 8 + 2 * m + h) * GN_ROWS + n * 8 + 2 * t) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
+    gn_move<4, NT>(acc, out, first, row);
 }
 
 __device__ __forceinline__ void gn_put(float v, __nv_bfloat16* o) { *o = __float2bfloat16_rn(v); }

@@ -1,0 +1,96 @@
+"""Products over 16-bit weights on the GPU: precision of long sums and of f32 outputs, paths that the other file's sizes do not take.
+
+Tolerances, from the arithmetic alone.
+  * A matrix instruction truncates where it adds: up to four times for 16 inputs (sums of four products each), by a step of 2^-23 of what its accumulator
+    holds.  With inputs of one sign an accumulator that moves on after 16 instructions holds half of its last value on average, so its value is off by
+    32 steps at most; what has moved on is added with rounding, half a step for each addition, in no one direction.
+  * f32 outputs of products of random signs are held to what f32 sums give: 2^-20 of the result in the 2-norm (eight steps: 16 instructions' truncations over an
+    accumulator that holds half of its last value on average), or one and a half times the error of the same product in 32 bits, where that is more.
+"""
+import pytest
+import torch
+
+from __graft_entry__ import load_package
+from test_products_gpu import CODE, DT, STEP, half_step
+
+pytestmark = pytest.mark.gpu
+pkg = load_package()
+
+
+@pytest.fixture(scope="module")
+def moe():
+    return pkg.MoE(pkg.make_config(128, 128, 4, 1, max_tokens=4))
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def norm_off(y, exact):
+    return float((y.double() - exact).norm() / exact.norm())
+
+
+def as_f32(off, off32):
+    """The bound of f32 outputs: `off32` is what the same product in 32 bits is off."""
+    return off <= max(2.0 ** -20, 1.5 * off32)
+
+
+def one_sign_bound(terms):
+    """`terms` chains of 16 instructions, or values as exact as those, added one after the other"""
+    return (32 + terms ** 0.5) * STEP
+
+
+def one_sign(gen, *shape, dtype):
+    return (torch.rand(*shape, device="cuda", generator=gen) + 0.5).to(dtype)
+
+
+def dense(moe, x, w, out, layout="out_in", act=False, gather=False):
+    """x w^T (w [outputs, inputs]) by the grouped product of one group"""
+    rows, K = x.shape
+    N = w.shape[0] // (2 if act else 1)
+    laid = w if layout == "out_in" else w.T.contiguous()
+    y = torch.empty(rows, N, device="cuda", dtype=out)
+    order = torch.arange(rows, device="cuda", dtype=torch.int32)
+    code = {v: CODE[k] for k, v in DT.items()}
+    moe.grouped(x.data_ptr(), laid.data_ptr(), None, y.data_ptr(), rows, 1, K, N, dtype=code[x.dtype], out_dtype=code[out],
+                layout=pkg.LAYOUT_OUT_IN if layout == "out_in" else pkg.LAYOUT_IN_OUT, act=pkg.GROUPED_SWIGLU if act else pkg.GROUPED_PLAIN,
+                order=order.data_ptr() if gather else None, gather=gather, stream=stream())
+    torch.cuda.synchronize()
+    return y
+
+
+def activated(z):
+    gate, up = z.chunk(2, dim=1)
+    return gate * torch.sigmoid(gate) * up
+
+
+# ------------------------------------------------------------------------------------------------------------
+# up to 16 rows
+# ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("layout", ["out_in", "in_out"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [3, 16])
+def test_few_rows_f32_outputs_are_as_exact_as_f32_sums(moe, rows, dtype, layout):
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    for K in (512, 2304, 6144):
+        for act in (False, True):
+            x = torch.randn(rows, K, device="cuda", generator=gen).to(DT[dtype])
+            w = (torch.randn(512, K, device="cuda", generator=gen) * K ** -0.5).to(DT[dtype])
+            z, z32 = x.double() @ w.double().T, x.float() @ w.float().T
+            if act:
+                z, z32 = activated(z), activated(z32)
+            off, off32 = norm_off(dense(moe, x, w, torch.float32, layout, act), z), norm_off(z32, z)
+            assert as_f32(off, off32), (K, act, off, off32)
+
+
+@pytest.mark.parametrize("layout", ["out_in", "in_out"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [3, 16])
+def test_few_rows_long_sums_of_one_sign(moe, rows, dtype, layout):
+    """A truncated sum of one sign drifts towards zero with its length."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    for K in (6144, 65536, 262144):
+        x = one_sign(gen, rows, K, dtype=DT[dtype])
+        w = (one_sign(gen, 64, K, dtype=torch.float32) * (1 + torch.rand(64, 1, device="cuda", generator=gen)) / K).to(DT[dtype])
+        z = x.double() @ w.double().T
+        assert norm_off(dense(moe, x, w, torch.float32, layout), z) <= one_sign_bound(K / 256), K
