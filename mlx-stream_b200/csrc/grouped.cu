@@ -278,9 +278,11 @@ constexpr uint32_t GT_TURN = 8 * 32 * 4;                         // an epilogue 
 constexpr uint32_t GT_SMEM = GT_STAGES * GT_STAGE + GT_EPI_WARPS * 2 * GT_TURN + 1024;
 
 constexpr uint32_t GT_PARTS = 4;                                  // most parts of a reduction: a cluster of eight CTAs
-// f32 outputs: the accumulator's additions truncate (1.7e-8 of the sum for each product of 16 inputs: 2.4e-6 after 2304 inputs), so after as many stages
-// as this the sums move on: the epilogue warps add them, rounding, to running sums in the tensor memory's second half
-constexpr uint32_t GT_CHAIN = 8;
+// The accumulator's additions truncate (1.7e-8 of the sum for each product of 16 inputs: 2.4e-6 after 2304 inputs), so for f32 outputs the sums move on
+// after as many stages as this: the epilogue warps add them, rounding, to running sums in the tensor memory's second half
+// (bf16; products of f16 have 22 bits, of which more is cut: about one and a half times the error).  f32 outputs, K 512 to 6144, gate and up, random signs:
+// bf16 9.6e-7 off 64 bits with eight stages, f16 1.3e-6, 6.9e-7 with four.  16384 rows of 32 groups, 2048 -> 6144: 569 us with eight, 677 with four.
+constexpr uint32_t GT_CHAIN_BF16 = 7, GT_CHAIN_F16 = 4;
 constexpr uint32_t GT_RUN = 256;                                 // first column of the running sums
 constexpr uint32_t GT_BOXES = 5;
 __host__ __device__ constexpr uint32_t gt_box_rows(uint32_t i) { return i < 3 ? 16u << i : 32 * i; }   // 16 32 64 96 128
@@ -289,10 +291,11 @@ struct TileParams {
     CUtensorMap w, x[GT_BOXES];   // x by box height
     GroupedArgs a;
     uint32_t n_ft, n_ks;          // output tiles of a row tile, stages
-    uint32_t cap;                 // most rows of a tile: 64 (f32 outputs), 128, 160, 192 or 256
+    uint32_t cap;                 // most rows of a tile: 64 (running sums), 128, 160, 192 or 256
     uint32_t w_loads;             // copies that a stage of weights takes
     uint32_t fmt;
     uint32_t parts;               // parts of the reduction, a CTA pair of the item's cluster to each (1: no cluster, pairs walk the items)
+    uint32_t chain;               // running sums: stages after which an accumulator moves on
 };
 
 struct GtItem { uint32_t g, p0, rows, n; };   // group, first position, rows, MMA N (a multiple of 32)
@@ -358,7 +361,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <bool SWIGLU, class O>
+template <bool SWIGLU, class O, bool SUMS>
 __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __grid_constant__ TileParams P) {
     extern __shared__ uint8_t smem_any[];
     __shared__ __align__(8) uint64_t full_bar[GT_STAGES], empty_bar[GT_STAGES], acc_full[2], acc_empty[2], x_full[GT_X_SLOTS], x_empty[GT_X_SLOTS];
@@ -408,9 +411,8 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
     const uint32_t n_pairs = P.parts == 1 ? gridDim.x / 2 : max(n_items, 1u);
     const uint32_t ks0 = part * P.n_ks / P.parts, ks1 = (part + 1) * P.n_ks / P.parts;
     constexpr uint32_t FT = SWIGLU ? 256 : 512;                  // outputs of an item: half of them this CTA's
-    // tensor memory: buffers of two accumulators of `cap` columns (f32 outputs: in the first half, with running sums in the second)
-    constexpr bool SUMS = sizeof(O) == 4;
-    const uint32_t n_buf = (SUMS ? 128 : 256) / P.cap, n_chains = SUMS ? (ks1 - ks0 + GT_CHAIN - 1) / GT_CHAIN : 1;
+    // tensor memory: buffers of two accumulators of `cap` columns (with running sums: in the first half, those in the second)
+    const uint32_t n_buf = (SUMS ? 128 : 256) / P.cap, n_chains = SUMS ? (ks1 - ks0 + P.chain - 1) / P.chain : 1;
     auto give_up = [&](uint32_t code) { if (!s_abort) atomicMax(a.status, code); s_abort = 1; };
     GtWalk walk{s_off, s_tiles, a.G};
     // gathered rows: as many slots as tiles of at most cap rows leave room for
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                 const uint32_t idesc = umma_idesc_pair(P.fmt, it.n, a.in_out);
                 for (uint32_t chain = 0; chain < n_chains && ok; ++chain) {
                     const uint32_t buf = n_done % n_buf, acc = tmem + buf * 2 * P.cap;
-                    const uint32_t k0 = SUMS ? ks0 + chain * GT_CHAIN : ks0, k1 = SUMS ? min(k0 + GT_CHAIN, ks1) : ks1;
+                    const uint32_t k0 = SUMS ? ks0 + chain * P.chain : ks0, k1 = SUMS ? min(k0 + P.chain, ks1) : ks1;
                     ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_empty[buf]), (n_done / n_buf & 1u) ^ 1u, &s_abort));
                     if (!ok) { give_up(ST_WAIT_EMPTY); break; }
                     tc_fence_after();
@@ -734,8 +736,8 @@ static GtClusters gt_clusters(const void* kernel, int sm_count) {
 // of 128 35 and 45).  The groups' sizes are on the device; the estimate takes them as equal.  A stage costs its products (4.4 cycles a row) or its
 // bytes (62 a cycle), whichever is longer; joining parts costs 50 cycles a row, and what has parts starts anew with each wave of clusters.  Returns the
 // row tiles that the call can have at most.
-static uint32_t gt_cut(const GroupedArgs& a, uint32_t n_ft, uint32_t n_ks, const GtClusters& room, uint32_t* cap, uint32_t* parts) {
-    const bool sums = a.out_dtype == DT_F32;          // f32 outputs: 64 rows and two buffers, or 128 and one that the products wait for
+// sums: 64 rows and two buffers beside the running sums, or 128 and one that the products wait for
+static uint32_t gt_cut(const GroupedArgs& a, bool sums, uint32_t n_ft, uint32_t n_ks, const GtClusters& room, uint32_t* cap, uint32_t* parts) {
     const uint32_t groups = a.G < a.rows ? a.G : a.rows, per = (a.rows + groups - 1) / groups;
     double best = 0;
     for (const uint32_t c : {64u, 128u, 160u, 192u, 256u})
@@ -751,7 +753,7 @@ static uint32_t gt_cut(const GroupedArgs& a, uint32_t n_ft, uint32_t n_ks, const
     return a.rows / *cap + groups;
 }
 
-template <bool SWIGLU, class O>
+template <bool SWIGLU, class O, bool SUMS>
 static cudaError_t tile_launch(const GroupedArgs& a, cudaStream_t st) {
     TileParams P;
     P.a = a;
@@ -759,11 +761,15 @@ static cudaError_t tile_launch(const GroupedArgs& a, cudaStream_t st) {
     P.n_ks = (a.K + GT_KS - 1) / GT_KS;
     P.fmt = a.dtype == DT_BF16 ? UMMA_BF16 : UMMA_F16;
     P.w_loads = 1;
-    const auto kernel = grouped_tile_kernel<SWIGLU, O>;
+    const auto kernel = grouped_tile_kernel<SWIGLU, O, SUMS>;
     cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GT_SMEM);
     if (set != cudaSuccess) return set;
     static const GtClusters room = gt_clusters(reinterpret_cast<const void*>(kernel), a.sm_count);
-    const uint32_t most_tiles = gt_cut(a, P.n_ft, P.n_ks, room, &P.cap, &P.parts);
+    const uint32_t most_tiles = gt_cut(a, SUMS, P.n_ft, P.n_ks, room, &P.cap, &P.parts);
+    // a part's stages in as few chains as hold them, all alike
+    const uint32_t part_ks = (P.n_ks + P.parts - 1) / P.parts, most_chain = a.dtype == DT_BF16 ? GT_CHAIN_BF16 : GT_CHAIN_F16;
+    const uint32_t chains = (part_ks + most_chain - 1) / most_chain;
+    P.chain = (part_ks + chains - 1) / chains;
     cudaError_t e;
     const uint64_t N = a.N, K = a.K, G = a.G, ld = a.ld_w, gs = a.w_stride;
     // A box is one CTA's weights of a stage.  Activation: gate rows, then up rows (outputs first), or 64 outputs' gate and up
@@ -791,7 +797,7 @@ static cudaError_t grouped_out(const GroupedArgs& a, cudaStream_t st) {
         if (a.in_out) return a.swiglu ? few_launch<BF16, true, true, O>(a, st) : few_launch<BF16, true, false, O>(a, st);
         return a.swiglu ? few_launch<BF16, false, true, O>(a, st) : few_launch<BF16, false, false, O>(a, st);
     }
-    return a.swiglu ? tile_launch<true, O>(a, st) : tile_launch<false, O>(a, st);
+    return a.swiglu ? tile_launch<true, O, sizeof(O) == 4>(a, st) : tile_launch<false, O, sizeof(O) == 4>(a, st);
 }
 cudaError_t launch_grouped(const GroupedArgs& a, cudaStream_t st) {
     if (a.dtype == DT_BF16) return a.out_dtype == DT_F32 ? grouped_out<true, float>(a, st) : grouped_out<true, __nv_bfloat16>(a, st);

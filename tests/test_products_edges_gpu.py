@@ -94,3 +94,22 @@ def test_few_rows_long_sums_of_one_sign(moe, rows, dtype, layout):
         w = (one_sign(gen, 64, K, dtype=torch.float32) * (1 + torch.rand(64, 1, device="cuda", generator=gen)) / K).to(DT[dtype])
         z = x.double() @ w.double().T
         assert norm_off(dense(moe, x, w, torch.float32, layout), z) <= one_sign_bound(K / 256), K
+
+
+# ------------------------------------------------------------------------------------------------------------
+# tensor-core tiles
+# ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("layout", ["out_in", "in_out"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [17, 64, 777])
+def test_tiles_f32_outputs_are_as_exact_as_f32_sums(moe, rows, dtype, layout):
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    for K in (512, 2304, 6144):
+        for act in (False, True):
+            x = torch.randn(rows, K, device="cuda", generator=gen).to(DT[dtype])
+            w = (torch.randn(1024, K, device="cuda", generator=gen) * K ** -0.5).to(DT[dtype])
+            z, z32 = x.double() @ w.double().T, x.float() @ w.float().T
+            if act:
+                z, z32 = activated(z), activated(z32)
+            off, off32 = norm_off(dense(moe, x, w, torch.float32, layout, act, gather=K == 2304), z), norm_off(z32, z)
+            assert as_f32(off, off32), (K, act, off, off32)
