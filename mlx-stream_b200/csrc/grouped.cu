@@ -278,11 +278,14 @@ constexpr uint32_t GT_TURN = 8 * 32 * 4;                         // an epilogue 
 constexpr uint32_t GT_SMEM = GT_STAGES * GT_STAGE + GT_EPI_WARPS * 2 * GT_TURN + 1024;
 
 constexpr uint32_t GT_PARTS = 4;                                  // most parts of a reduction: a cluster of eight CTAs
-// The accumulator's additions truncate (1.7e-8 of the sum for each product of 16 inputs: 2.4e-6 after 2304 inputs), so for f32 outputs the sums move on
-// after as many stages as this: the epilogue warps add them, rounding, to running sums in the tensor memory's second half
+// The accumulator's additions truncate (1.7e-8 of the sum for each product of 16 inputs: 2.4e-6 after 2304 inputs; inputs of one sign, 65,536 of them
+// in f16: 1e-4, near f16's half step), so for f32 outputs and for long sums of 16-bit ones the sums move on after as many stages as this: the epilogue
+// warps add them, rounding, to running sums in the tensor memory's second half
 // (bf16; products of f16 have 22 bits, of which more is cut: about one and a half times the error).  f32 outputs, K 512 to 6144, gate and up, random signs:
 // bf16 9.6e-7 off 64 bits with eight stages, f16 1.3e-6, 6.9e-7 with four.  16384 rows of 32 groups, 2048 -> 6144: 569 us with eight, 677 with four.
 constexpr uint32_t GT_CHAIN_BF16 = 7, GT_CHAIN_F16 = 4;
+// 16-bit outputs: inputs from which on their sums move on, where a sum of one sign may drift by a sixteenth of the type's half step
+constexpr uint32_t GT_LONG_F16 = 8192, GT_LONG_BF16 = 65536;
 constexpr uint32_t GT_RUN = 256;                                 // first column of the running sums
 constexpr uint32_t GT_BOXES = 5;
 __host__ __device__ constexpr uint32_t gt_box_rows(uint32_t i) { return i < 3 ? 16u << i : 32 * i; }   // 16 32 64 96 128
@@ -797,6 +800,7 @@ static cudaError_t grouped_out(const GroupedArgs& a, cudaStream_t st) {
         if (a.in_out) return a.swiglu ? few_launch<BF16, true, true, O>(a, st) : few_launch<BF16, true, false, O>(a, st);
         return a.swiglu ? few_launch<BF16, false, true, O>(a, st) : few_launch<BF16, false, false, O>(a, st);
     }
+    if (sizeof(O) == 4 || a.K > (BF16 ? GT_LONG_BF16 : GT_LONG_F16)) return a.swiglu ? tile_launch<true, O, true>(a, st) : tile_launch<false, O, true>(a, st);
     return a.swiglu ? tile_launch<true, O, sizeof(O) == 4>(a, st) : tile_launch<false, O, sizeof(O) == 4>(a, st);
 }
 cudaError_t launch_grouped(const GroupedArgs& a, cudaStream_t st) {

@@ -113,3 +113,26 @@ def test_tiles_f32_outputs_are_as_exact_as_f32_sums(moe, rows, dtype, layout):
                 z, z32 = activated(z), activated(z32)
             off, off32 = norm_off(dense(moe, x, w, torch.float32, layout, act, gather=K == 2304), z), norm_off(z32, z)
             assert as_f32(off, off32), (K, act, off, off32)
+
+
+@pytest.mark.parametrize("layout, act, gather", [("out_in", False, True), ("in_out", False, False), ("out_in", True, False), ("in_out", True, True)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [17, 300])
+def test_tiles_long_sums_of_one_sign(moe, rows, dtype, layout, act, gather):
+    """A truncated sum of one sign drifts towards zero with its length: f32 outputs, and 16-bit outputs of more inputs than one chain may take."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    N = 64
+    for K, out in ((65536 + 72, "f32"), (65536 + 72, dtype), (262144, dtype)):
+        x = (one_sign(gen, rows, K, dtype=torch.float32) * (1 + torch.rand(rows, 1, device="cuda", generator=gen))).to(DT[dtype])
+        w = (one_sign(gen, N * (2 if act else 1), K, dtype=torch.float32) * (1 + torch.rand(N * (2 if act else 1), 1, device="cuda", generator=gen)) / K).to(DT[dtype])
+        z = x.double() @ w.double().T
+        z = activated(z) if act else z
+        y = dense(moe, x, w, DT[out], layout, act, gather)
+        # gate and up: two sums' drifts, the gate's through a slope of at most 1.1 of a value that is at least 0.73 of it
+        bound = one_sign_bound(K / 1024) * (2.6 if act else 1.0)
+        if out == "f32":
+            assert norm_off(y, z) <= bound, (K, out)
+        else:
+            # an output rounds by up to half a step in no one direction: the mean of n such roundings is a drift of four of its deviations at most
+            drift = float(((y.double() - z) / z).mean())
+            assert abs(drift) <= bound + 4 * half_step(y.dtype) / (3 * y.numel()) ** 0.5, (K, out, drift)
