@@ -305,8 +305,8 @@ typedef struct {
 /* y[t] = base[t] + scale_a (x[t] A_a^T) B_a^T with a = ids_dev[t]; a token with a negative id has no adapter: y[t] = base[t].
  * a_dev [n_adapters, rank, n_in], b_dev [n_adapters, n_out, rank]; scales_dev f32 [n_adapters] or NULL (1); ranks_dev
  * i32 [n_adapters] or NULL: how many of an adapter's rank rows count (the others are not looked at).  base_dev NULL: zeros; base_dev == y_dev with
- * the same row stride: in place, otherwise they do not overlap; y overlaps neither x, a nor b.  The inner product is kept in f32 and as two 16-bit parts (16 bits of precision or more) between
- * the two factors; one rounding to y's type.  An id >= n_adapters counts as none and sets the status word. */
+ * the same row stride: in place, otherwise they do not overlap; y overlaps neither x, a nor b.  The inner product is kept in f32 and as 16-bit parts between the
+ * two factors: 16 bits for bf16 outputs, 22 for f16 inputs, 24 for bf16 inputs and f32 outputs; one rounding to y's type.  An id >= n_adapters counts as none and sets the status word. */
 int mlxs_moe_adapters(mlxs_moe *h, const mlxs_adapters_desc *desc, const void *x_dev, const void *a_dev, const void *b_dev,
                       const int32_t *ids_dev, const float *scales_dev, const int32_t *ranks_dev, const void *base_dev,
                       void *y_dev, void *stream);

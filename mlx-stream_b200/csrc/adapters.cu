@@ -8,8 +8,9 @@
 //   * More tokens (or more than 16 that have 14 per adapter): every CTA sorts the ids of a segment of up to 2048 tokens by itself, so that an adapter's
 //     tokens, wherever they lie, share its units (999 mixed tokens of 24 adapters: 318 us by tiles, 145 sorted).  From 16 tokens per unit on, and ranks
 //     40 to 128 where there is enough work, adapters_tensor_kernel (tcgen05); otherwise adapters_sorted_kernel (mma.sync).
-//   * u = A x is kept as two 16-bit parts, hi = round(u), lo = round(u - hi): 16 (bf16) or 22 (f16) bits, so what is lost between the factors is far
-//     inside an output's rounding.  f16 parts are scaled by the row's largest power of two, since A x may pass f16's range where y does not.
+//   * u = A x is kept as 16-bit parts, each the rounding of what the ones before it leave: two, 16 (bf16) or 22 (f16) bits, so that what is lost between the
+//     factors is far inside an output's rounding; three of bf16, 24 bits, where outputs are f32 (rank 64, 5120 inputs, no base: two parts 2.5e-6 off 64 bits,
+//     f32 2.3e-7).  f16 parts are scaled by the row's largest power of two, since A x may pass f16's range where y does not.
 //   * base is added in f32, one rounding.
 // Measured (GPU time, other inputs every call): one token of rank 16, 5120 -> 2304: 6.7 us, a chain of two cluster barriers and three cold loads; 64 tokens of 48
 // adapters, rank 32: 13 us (floor 2.6); 4000 of eight, rank 32: 38 us (floor 12.5); 8192 tokens of six, rank 64, 4096 -> 2048: 55 us (floor 21); 999 of 24, rank 128, f32: 36 us (floor 14).
@@ -51,16 +52,21 @@ __device__ __forceinline__ float ad_f32(float v) { return v; }
 __device__ __forceinline__ void ad_round(float v, float& o) { o = v; }
 __device__ __forceinline__ void ad_round(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void ad_round(float v, __half& o) { o = __float2half_rn(v); }
-// two values as two 16-bit parts each, packed
-template <class T>
-__device__ __forceinline__ void ad_split(float x, float y, uint32_t& hi, uint32_t& lo) {
-    T h[2], l[2];
-    ad_round(x, h[0]); ad_round(y, h[1]);
-    // an infinity has no remainder
-    const float dx = x - ad_f32(h[0]), dy = y - ad_f32(h[1]);
-    ad_round(isinf(ad_f32(h[0])) ? 0.f : dx, l[0]); ad_round(isinf(ad_f32(h[1])) ? 0.f : dy, l[1]);
-    hi = *reinterpret_cast<uint32_t*>(h);
-    lo = *reinterpret_cast<uint32_t*>(l);
+// 16-bit parts of the inner product
+template <class T, class O>
+constexpr int AD_PARTS = std::is_same<T, __nv_bfloat16>::value && sizeof(O) == 4 ? 3 : 2;
+// two values as NP 16-bit parts each, packed, the largest first
+template <class T, int NP>
+__device__ __forceinline__ void ad_split(float x, float y, uint32_t (&parts)[NP]) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        T h[2];
+        ad_round(x, h[0]); ad_round(y, h[1]);
+        parts[p] = *reinterpret_cast<uint32_t*>(h);
+        // an infinity has no remainder
+        x = isinf(ad_f32(h[0])) ? 0.f : x - ad_f32(h[0]);
+        y = isinf(ad_f32(h[1])) ? 0.f : y - ad_f32(h[1]);
+    }
 }
 // eight 16-bit values of which the first n count
 __device__ __forceinline__ uint4 ad_first(uint4 v, int n) {
@@ -77,21 +83,21 @@ __device__ __forceinline__ float2 ad_ld_cluster2(uint32_t addr) {
 __device__ __forceinline__ void ad_st_cluster(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 
 struct AdSmem {                          // dynamic shared memory, byte offsets
-    // rp: rank rows that a pass writes; pitch: bytes of a token's parts, 64 modulo 128 (rows on other banks)
-    uint32_t part, u_hi, u_lo, bytes, r16, rp, pitch, stage;
+    // rp: rank rows that a pass writes; u: the 16-bit parts, u_part bytes each; pitch: bytes of a token in one, 64 modulo 128 (rows on other banks)
+    uint32_t part, u, u_part, bytes, r16, rp, pitch, stage;
 };
-__host__ __device__ inline AdSmem ad_smem(uint32_t R, uint32_t tokens) {
+__host__ __device__ inline AdSmem ad_smem(uint32_t R, uint32_t tokens, uint32_t n_parts) {
     AdSmem s;
     s.r16 = (R + 15) / 16 * 16;
     s.rp = R <= 16 ? 16 : R <= 32 ? 32 : AD_MR;
     s.pitch = (R + 31) / 32 * 64;
     if (s.pitch % 128 == 0) s.pitch += 64;
     // one after the other: the ring of operands, the warps' sums, the 16-bit parts
-    s.u_hi = 0;
-    s.u_lo = AD_TT * s.pitch;
+    s.u = 0;
+    s.u_part = AD_TT * s.pitch;
     s.stage = (AD_TT + s.rp) * AD_ROW;
     const uint32_t warps = AD_WARPS * 16 * (s.rp + 4) * 4, ring = tokens > 16 ? AD_STAGES * s.stage : 0;
-    s.part = 2 * s.u_lo > warps ? 2 * s.u_lo : warps;
+    s.part = n_parts * s.u_part > warps ? n_parts * s.u_part : warps;
     if (ring > s.part) s.part = ring;
     s.bytes = s.part + s.r16 * AD_TT * 4;
     return s;
@@ -246,7 +252,7 @@ __device__ __forceinline__ uint32_t ad_pack(float x, float y, __half) {
 // the last hold zeros.
 template <class T, class O, int MT>
 __device__ __forceinline__ void ad_outer(const AdaptersArgs& a, const T* B, uint32_t R, uint32_t fb, uint32_t fb_end, const uint32_t* rows, uint32_t n_rows,
-                                         uint32_t t0, uint32_t u_hi, uint32_t u_lo, uint32_t pitch, const float* row_scale) {
+                                         uint32_t t0, uint32_t u, uint32_t u_part, uint32_t pitch, const float* row_scale) {
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     const uint4 zero = make_uint4(0, 0, 0, 0);
     constexpr int V = sizeof(O) / 2;                      // 16-byte words of eight outputs
@@ -268,7 +274,7 @@ __device__ __forceinline__ void ad_outer(const AdaptersArgs& a, const T* B, uint
                 if (std::is_same<T, __half>::value) scale[m][h] = row_scale[i];
             }
         }
-    const uint32_t u0 = u_hi + g * pitch + t * 16, k_end = (R + 31) / 32 * 32;
+    const uint32_t u0 = u + g * pitch + t * 16, k_end = (R + 31) / 32 * 32;
     uint4 bv[2][4], bs[MT][2][V];
     auto ask = [&](uint4 (&b)[4], uint32_t block, uint32_t k) {
         // outputs behind the last read the last one's row (their products go nowhere), rank columns behind the last are zeros
@@ -300,10 +306,10 @@ __device__ __forceinline__ void ad_outer(const AdaptersArgs& a, const T* B, uint
         float acc[MT][4][4] = {};
         auto multiply = [&](const uint4 (&b)[4], uint32_t k) {
 #pragma unroll
-            for (int part = 0; part < 2; ++part)
+            for (int part = 0; part < AD_PARTS<T, O>; ++part)
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    const uint32_t at = u0 + (part ? u_lo - u_hi : 0) + m * 16 * pitch + k * 2;
+                    const uint32_t at = u0 + part * u_part + m * 16 * pitch + k * 2;
                     const uint4 lo = ad_lds16(at), hi = ad_lds16(at + 8 * pitch);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -390,14 +396,13 @@ __device__ __forceinline__ void ad_copy(const AdaptersArgs& a, const Row* rows, 
 
 // where the 16-bit parts of rank columns r, r + 1 (r even) of a token go
 struct AdParts {                         // rows of `pitch` bytes
-    uint32_t hi_, lo_, pitch;
-    __device__ uint32_t hi(uint32_t i, uint32_t r) const { return hi_ + i * pitch + r * 2; }
-    __device__ uint32_t lo(uint32_t i, uint32_t r) const { return lo_ + i * pitch + r * 2; }
+    uint32_t u, u_part, pitch;
+    __device__ uint32_t at(uint32_t p, uint32_t i, uint32_t r) const { return u + p * u_part + i * pitch + r * 2; }
 };
 // The CTAs' sums in order (part: f32 [tokens][r16], in every CTA at the same place), a warp to a token; the parts, and a power of two that the outputs
 // are multiplied by, go to every CTA.  Eight warps.
 // NJ: 64 rank columns at most, NI: tokens of a warp whose reads are under way together.
-template <class T, int NJ, int NI, class Parts>
+template <class T, int NP, int NJ, int NI, class Parts>
 __device__ __forceinline__ void ad_fold(const AdaptersArgs& a, uint32_t C, uint32_t rank, int32_t id, uint32_t R, uint32_t n_rows, uint32_t warp,
                                         uint32_t part, uint32_t r16, uint32_t scales, const Parts& parts) {
     const uint32_t lane = threadIdx.x & 31u, step = C * AD_WARPS;
@@ -441,12 +446,11 @@ __device__ __forceinline__ void ad_fold(const AdaptersArgs& a, uint32_t C, uint3
             for (int j = 0; j < NJ; ++j) {
                 const uint32_t r = j * 64 + lane * 2;
                 if (r >= (R + 31) / 32 * 32) continue;               // zeros behind the last rank column
-                uint32_t hi, lo;
-                ad_split<T>(v[n][j][0] * down, v[n][j][1] * down, hi, lo);
-                for (uint32_t c = 0; c < C; ++c) {
-                    ad_st_cluster(map_to_rank(parts.hi(i, r), c), hi);
-                    ad_st_cluster(map_to_rank(parts.lo(i, r), c), lo);
-                }
+                uint32_t split[NP];
+                ad_split<T, NP>(v[n][j][0] * down, v[n][j][1] * down, split);
+                for (uint32_t c = 0; c < C; ++c)
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) ad_st_cluster(map_to_rank(parts.at(p, i, r), c), split[p]);
             }
             if (std::is_same<T, __half>::value && lane < C) ad_st_cluster(map_to_rank(scales + i * 4, lane), __float_as_uint(up));
         }
@@ -511,20 +515,19 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
         __syncthreads();
     }
     cluster_sync_all();
-    const AdParts parts{base_s + L.u_hi, base_s + L.u_lo, L.pitch};
-    ad_fold<T, 4, 1>(a, C, rank, id, R, n_rows, warp, base_s + L.part, L.r16, smem_u32(sh.scale), parts);
+    const AdParts parts{base_s + L.u, L.u_part, L.pitch};
+    ad_fold<T, AD_PARTS<T, O>, 4, 1>(a, C, rank, id, R, n_rows, warp, base_s + L.part, L.r16, smem_u32(sh.scale), parts);
     cluster_sync_all();
     // ---- outer product: this CTA's outputs ----
     if (n_rows <= 16)
-        ad_outer<T, O, 1>(a, B, R, fb0 + warp, fb1, sh.rows, n_rows, t0, base_s + L.u_hi, base_s + L.u_lo, L.pitch, sh.scale);
+        ad_outer<T, O, 1>(a, B, R, fb0 + warp, fb1, sh.rows, n_rows, t0, base_s + L.u, L.u_part, L.pitch, sh.scale);
     else
         for (uint32_t h = 0; h < n_rows; h += 32)
             if (n_rows - h <= 16)
-                ad_outer<T, O, 1>(a, B, R, fb0 + warp, fb1, sh.rows + h, n_rows - h, t0, base_s + L.u_hi + h * L.pitch, base_s + L.u_lo + h * L.pitch, L.pitch,
-                                  sh.scale + h);
+                ad_outer<T, O, 1>(a, B, R, fb0 + warp, fb1, sh.rows + h, n_rows - h, t0, base_s + L.u + h * L.pitch, L.u_part, L.pitch, sh.scale + h);
             else
-                ad_outer<T, O, 2>(a, B, R, fb0 + warp, fb1, sh.rows + h, min(n_rows - h, 32u), t0, base_s + L.u_hi + h * L.pitch, base_s + L.u_lo + h * L.pitch,
-                                  L.pitch, sh.scale + h);
+                ad_outer<T, O, 2>(a, B, R, fb0 + warp, fb1, sh.rows + h, min(n_rows - h, 32u), t0, base_s + L.u + h * L.pitch, L.u_part, L.pitch,
+                                  sh.scale + h);
     __syncthreads();
 }
 
@@ -540,7 +543,7 @@ template <class T, class O>
 __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const AdaptersArgs a, const uint32_t C, const uint32_t slots) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ AdShared sh;
-    const AdSmem L = ad_smem(a.R, a.T);
+    const AdSmem L = ad_smem(a.R, a.T, AD_PARTS<T, O>);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = cluster_rank();
     const uint32_t unit = blockIdx.x / C, tile = unit / slots, slot = unit % slots, t0 = tile * AD_TT;
 
@@ -708,7 +711,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ AdShared sh;
     __shared__ uint32_t s_scan[AD_WARPS];
-    const AdSmem L = ad_smem(a.R, a.T);
+    const AdSmem L = ad_smem(a.R, a.T, AD_PARTS<T, O>);
     const uint32_t tid = threadIdx.x, rank = cluster_rank();
     const uint32_t cl = blockIdx.x / C, seg = cl / per_seg, t0 = seg * seg_len, n_tok = min(seg_len, a.T - t0), n_places = a.n_adapters + 1;
     AdSort<PLACES>& so = *reinterpret_cast<AdSort<PLACES>*>(smem + L.bytes);
@@ -733,7 +736,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
 // many tokens per adapter: the same cut, both products on the tensor cores
 // ------------------------------------------------------------------------------------------------------------
 // For units of 16 tokens and more mma.sync's operands, read from shared memory by every warp again, take longer than the bytes.  Here a
-// unit's inner product is D1[rank 128][tokens 64] = A x^T and its outer product, per block of 128 outputs, D2[outputs 128][tokens 64] = B u^T (both parts of u, one after
+// unit's inner product is D1[rank 128][tokens 64] = A x^T and its outer product, per block of 128 outputs, D2[outputs 128][tokens 64] = B u^T (the parts of u, one after
 // the other, into one accumulator): tcgen05.mma with M = 128, N = 64, accumulators in tensor memory.  A ring of stages: 64 inputs of A (a tensor-map copy)
 // and of the unit's x rows (asynchronous copies, eight lanes to a row), later 64 rank columns of a block of B (asynchronous copies, which zero what lies behind
 // the adapter's rank).  A warp to a ring slot, one that issues the products, eight that read accumulators: inner sums -> shared memory -> the cluster's fold ->
@@ -749,30 +752,34 @@ constexpr uint32_t AB_MOST_SLOTS = 9, AB_MAX_R = 128, AB_MIN_ROWS = 16;   // ran
 constexpr uint32_t AB_LITTLE = 12000;                                // tokens x rank that mma.sync does sooner
 constexpr uint32_t AB_U_BYTES = 64 * 128;                            // one part of 64 rank columns of the unit's tokens
 constexpr uint32_t AB_TURN = 16 * 32 * 4;                            // an epilogue warp's turn of 16 tokens x 32 outputs
+constexpr uint32_t AB_MOST_SMEM = 227 * 1024 - 512;                  // beside the barriers
 struct AbSmem {
     uint32_t slots, slot, x;                                         // ring slots, their bytes, x rows behind R rows of A (the products read 128: what is there)
     uint32_t u, part, turn, sort, bytes;                             // behind the ring, offsets from its 1024-byte boundary
     __host__ __device__ uint32_t threads() const { return (1 + AD_WARPS + slots) * 32; }
 };
-__host__ __device__ inline AbSmem ab_smem(uint32_t R) {
+__host__ __device__ inline AbSmem ab_smem(uint32_t R, uint32_t n_parts) {
     AbSmem s;
-    const uint32_t chunks = (R + 63) / 64;
+    const uint32_t u_bytes = (R + 63) / 64 * n_parts * AB_U_BYTES, part_bytes = (R + 15) / 16 * 16 * 64 * 4;
+    const uint32_t rest = u_bytes + part_bytes + AD_WARPS * AB_TURN + (uint32_t)sizeof(AdSort<AD_FEW>) + 1024;
     s.x = R * 128;                                                   // a multiple of 1024
     s.slot = R <= 64 ? 128 * 128 : s.x + 64 * 128;                   // a block of 128 outputs' B fits too
     s.slots = R <= 64 ? AB_MOST_SLOTS : 5;
+    if (s.slots * s.slot + rest > AB_MOST_SMEM) s.slots = 4;        // three parts at ranks above 120
     s.u = s.slots * s.slot;
-    s.part = s.u + chunks * 2 * AB_U_BYTES;
-    s.turn = s.part + (R + 15) / 16 * 16 * 64 * 4;
+    s.part = s.u + u_bytes;
+    s.turn = s.part + part_bytes;
     s.sort = s.turn + AD_WARPS * AB_TURN;
-    s.bytes = s.sort + (uint32_t)sizeof(AdSort<AD_FEW>) + 1024;
+    s.bytes = s.slots * s.slot + rest;
     return s;
 }
 // operand rows of 64 rank columns, 128 bytes, 16-byte chunks swizzled by the row: [64-column chunk][part][64 tokens]
+template <int NP>
 struct AbParts {
     uint32_t u;
-    __device__ uint32_t at(uint32_t i, uint32_t r) const { return u + (r >> 6) * (2 * AB_U_BYTES) + i * 128 + ((((r & 63u) >> 3) ^ (i & 7u)) << 4) + (r & 7u) * 2; }
-    __device__ uint32_t hi(uint32_t i, uint32_t r) const { return at(i, r); }
-    __device__ uint32_t lo(uint32_t i, uint32_t r) const { return at(i, r) + AB_U_BYTES; }
+    __device__ uint32_t at(uint32_t p, uint32_t i, uint32_t r) const {
+        return u + ((r >> 6) * NP + p) * AB_U_BYTES + i * 128 + ((((r & 63u) >> 3) ^ (i & 7u)) << 4) + (r & 7u) * 2;
+    }
 };
 struct AbParams {
     CUtensorMap a;                       // [n_adapters][R][K], boxes of R rows x 64 inputs
@@ -803,7 +810,8 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, rank = cluster_rank(), C = P.C;
     const uint32_t ring = (smem_u32(smem_any) + 1023u) & ~1023u;
     uint8_t* const ring_p = smem_any + (ring - smem_u32(smem_any));
-    const AbSmem L = ab_smem(a.R);
+    constexpr int NP = AD_PARTS<T, O>;
+    const AbSmem L = ab_smem(a.R, NP);
     const uint32_t cl = blockIdx.x / C, seg = cl / P.per_seg, t0 = seg * P.seg_len, n_tok = min(P.seg_len, a.T - t0), n_places = a.n_adapters + 1;
     AdSort<AD_FEW>& so = *reinterpret_cast<AdSort<AD_FEW>*>(ring_p + L.sort);
     if (tid == 0) {
@@ -924,10 +932,10 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
                     wait(&full_bar[s], ph, ST_WAIT_FULL);
                     if (!ok) break;
                     const uint32_t at = __shfl_sync(0xFFFFFFFFu, (ring + s * L.slot) >> 4, 0) | 1u << 16, steps = (min(R - c * 64, 64u) + 15) / 16;
-                    const uint32_t ua = __shfl_sync(0xFFFFFFFFu, (ring + L.u + c * 2 * AB_U_BYTES) >> 4, 0) | 1u << 16;
+                    const uint32_t ua = __shfl_sync(0xFFFFFFFFu, (ring + L.u + c * NP * AB_U_BYTES) >> 4, 0) | 1u << 16;
                     if (elect_one()) {
 #pragma unroll
-                        for (uint32_t part = 0; part < 2; ++part)
+                        for (uint32_t part = 0; part < NP; ++part)
 #pragma unroll
                             for (uint32_t j = 0; j < 4; ++j)
                                 if (j < steps) umma_f16_lo(acc, at + j * 2, ua + part * (AB_U_BYTES >> 4) + j * 2, UMMA_SW128_HI, idesc, c | part | j ? 1u : 0u);
@@ -947,7 +955,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         const uint32_t q = warp & 3u, half = warp >> 2, etid = tid;   // warps 0 .. 7
         float* const part = reinterpret_cast<float*>(ring_p + L.part);
         const uint32_t r16 = (a.R + 15) / 16 * 16, turn = ring + L.turn + warp * AB_TURN;
-        const AbParts parts{ring + L.u};
+        const AbParts<NP> parts{ring + L.u};
         uint32_t n_done = 0, n_blocks = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -993,7 +1001,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
             if (etid < C) mbar_arrive_cluster(map_to_rank(smem_u32(&part_ready), etid));
             wait(&part_ready, n_done & 1u);
             if (!together()) break;
-            ad_fold<T, AB_MAX_R / 64, 4>(a, C, rank, (int32_t)un.place, R, un.rows, warp, ring + L.part, r16, smem_u32(s_scale), parts);
+            ad_fold<T, NP, AB_MAX_R / 64, 4>(a, C, rank, (int32_t)un.place, R, un.rows, warp, ring + L.part, r16, smem_u32(s_scale), parts);
             together();
             if (etid < C) mbar_arrive_cluster(map_to_rank(smem_u32(&u_ready), etid));
             wait(&u_ready, n_done & 1u);
@@ -1086,9 +1094,9 @@ static cudaError_t ad_launch(void (*kernel)(Params...), uint32_t C, uint32_t clu
 }
 // clusters of 1, 2, 4, 8 CTAs of the tensor-core kernel that the device holds at once
 struct AbClusters { uint32_t n[9]; };
-static AbClusters ab_clusters(const void* kernel, int sm_count) {
+static AbClusters ab_clusters(const void* kernel, uint32_t n_parts, int sm_count) {
     AbClusters c{};
-    const AbSmem L = ab_smem(AB_MAX_R);
+    const AbSmem L = ab_smem(AB_MAX_R, n_parts);
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L.bytes);
     for (uint32_t C = 1; C <= 8; C *= 2) {
         cudaLaunchAttribute attr;
@@ -1104,7 +1112,7 @@ static AbClusters ab_clusters(const void* kernel, int sm_count) {
 }
 template <class T, class O>
 static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
-    const AdSmem L = ad_smem(a.R, a.T);
+    const AdSmem L = ad_smem(a.R, a.T, AD_PARTS<T, O>);
     const uint32_t sms = (uint32_t)a.sm_count;
     // CTAs of the mma.sync kernels that run at once: two to an SM (ranks to 128) where their shared memory and the 1 KB
     // that each costs besides fit twice into 228 KB
@@ -1133,13 +1141,14 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
         P.p = a;
         cudaError_t e = encode_map<3>(&P.a, a.dtype, a.a, {a.K, a.R, a.n_adapters}, {a.K, a.a_stride}, {64, a.R, 1});
         if (e != cudaSuccess) return e;
-        static const AbClusters room1 = ab_clusters(reinterpret_cast<const void*>(adapters_tensor_kernel<T, O>), a.sm_count);   // an SM holds one CTA
+        static const AbClusters room1 = ab_clusters(reinterpret_cast<const void*>(adapters_tensor_kernel<T, O>), AD_PARTS<T, O>, a.sm_count);   // an SM holds one CTA
         P.C = 8;
         P.seg_len = tokens;
         while (P.C > 1 && ((uint64_t)units * segs > room1.n[P.C] || P.C > (a.K + 63) / 64)) P.C /= 2;   // every CTA has inputs to sum
         P.per_seg = room1.n[P.C] / segs;
         P.per_seg = P.per_seg < 1 ? 1 : P.per_seg > units + tokens / AD_TT + 1 ? units + tokens / AD_TT + 1 : P.per_seg;
-        return ad_launch(adapters_tensor_kernel<T, O>, P.C, P.per_seg * segs, ab_smem(a.R).threads(), ab_smem(a.R).bytes, st, P);
+        const AbSmem S = ab_smem(a.R, AD_PARTS<T, O>);
+        return ad_launch(adapters_tensor_kernel<T, O>, P.C, P.per_seg * segs, S.threads(), S.bytes, st, P);
     }
     // Tokens of a unit at most, and CTAs of its cluster: by waves of clusters, each a start (us: 6, or 9 with the ring) and the unit's outputs and
     // inputs over its CTAs; a unit of up to 16 tokens takes about as long per token as a larger one (longer at high ranks: A and B are read once per

@@ -136,3 +136,58 @@ def test_tiles_long_sums_of_one_sign(moe, rows, dtype, layout, act, gather):
             # an output rounds by up to half a step in no one direction: the mean of n such roundings is a drift of four of its deviations at most
             drift = float(((y.double() - z) / z).mean())
             assert abs(drift) <= bound + 4 * half_step(y.dtype) / (3 * y.numel()) ** 0.5, (K, out, drift)
+
+
+# ------------------------------------------------------------------------------------------------------------
+# adapters
+# ------------------------------------------------------------------------------------------------------------
+# tokens, adapters, rank: tiles of up to 64 tokens (16 and fewer, and more to an adapter), sorted tokens by few and by many adapters, tensor cores at ranks
+# of one and two operand rows' widths, and the ranks whose rings have four slots
+PATHS = [(1, 1, 16), (3, 2, 256), (40, 20, 64), (64, 48, 32), (200, 2, 8), (200, 2, 256), (700, 600, 24), (1000, 8, 40), (1000, 8, 64), (600, 8, 72), (1000, 8, 128),
+         (4100, 3, 120)]
+
+
+def lora(moe, x, a, b, ids, out, base=None, scales=None, ranks=None, handle_stream=None, in_place=False):
+    (T, K), (n, R, _), N = x.shape, a.shape, b.shape[1]
+    code = {v: CODE[k] for k, v in DT.items()}
+    y = base.clone() if in_place else torch.empty(T, N, device="cuda", dtype=out)
+    given = y if in_place else base
+    moe.adapters(x.data_ptr(), T, a.data_ptr(), b.data_ptr(), ids.data_ptr(), y.data_ptr(), K, N, R, n, dtype=code[x.dtype], out_dtype=code[out],
+                 base=None if given is None else given.data_ptr(), scales=None if scales is None else scales.data_ptr(),
+                 ranks=None if ranks is None else ranks.data_ptr(), stream=handle_stream or stream())
+    torch.cuda.synchronize()
+    return y
+
+
+def lora_plain(x, a, b, ids, base, scales, wide):
+    y = torch.zeros(x.shape[0], b.shape[1], device="cuda", dtype=wide) if base is None else base.to(wide)
+    y = y.clone()
+    for i in range(a.shape[0]):
+        at = (ids == i).nonzero().squeeze(1)
+        if len(at):
+            s = 1.0 if scales is None else scales[i].to(wide)
+            y[at] += (x[at].to(wide) @ a[i].to(wide).T * s) @ b[i].to(wide).T
+    return y
+
+
+def adapters_off(moe, T, n, R, K, N, dtype, based, seed=0):
+    """(the call's error, that of the same products in 32 bits)"""
+    gen = torch.Generator(device="cuda").manual_seed(seed + T)
+    x = torch.randn(T, K, device="cuda", generator=gen).to(DT[dtype])
+    a = (torch.randn(n, R, K, device="cuda", generator=gen) * K ** -0.5).to(DT[dtype])
+    b = (torch.randn(n, N, R, device="cuda", generator=gen) * 0.1).to(DT[dtype])
+    ids = torch.randint(0, n, (T,), device="cuda", generator=gen).to(torch.int32)
+    scales = torch.rand(n, device="cuda", generator=gen) + 0.5
+    base = torch.randn(T, N, device="cuda", generator=gen) if based else None
+    y = lora(moe, x, a, b, ids, torch.float32, base, scales, in_place=based)
+    exact = lora_plain(x, a, b, ids, base, scales, torch.float64)
+    return norm_off(y, exact), norm_off(lora_plain(x, a, b, ids, base, scales, torch.float32), exact)
+
+
+@pytest.mark.parametrize("based", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T, n, R", PATHS)
+def test_adapters_f32_outputs_are_as_exact_as_f32_sums(moe, T, n, R, dtype, based):
+    """Few inputs: what is kept of the inner product decides."""
+    off, off32 = adapters_off(moe, T, n, R, 264, 136, dtype, based)
+    assert as_f32(off, off32), (off, off32)
