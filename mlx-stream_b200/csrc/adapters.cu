@@ -30,6 +30,14 @@ constexpr uint32_t AD_WARPS = 8;
 constexpr uint32_t AD_MR = 64;          // rank rows of a pass
 constexpr uint32_t AD_KS = 64, AD_STAGES = 4;   // inputs of a stage, stages of the ring (more than 16 tokens)
 constexpr uint32_t AD_ROW = AD_KS * 2;          // bytes of a row of a stage
+// The matrix instruction truncates where it adds.  How the sums are kept: in one accumulator; the inner product's in chains of ad_chain products of 16
+// inputs, added with rounding (f32 outputs: 4000 f16 tokens of rank 16, 5120 inputs, in one accumulator 9.0e-7 off 64 bits, of one sign 3.2e-6; f32 sums 3.9e-7);
+// the outer product's too, 32 rank columns by themselves (f32 outputs above rank 128: up to 48 products, 1.03e-6 in one accumulator).  Kernels of their
+// own: beside one another their registers cost every call.
+enum AdSums { AD_PLAIN, AD_CHAINED, AD_ROUNDED };
+template <class O, AdSums SUMS>
+constexpr uint32_t ad_chain = SUMS == AD_PLAIN ? 0 : sizeof(O) == 4 ? 16 : 64;
+constexpr uint32_t AD_LONG = 16384;              // 16-bit outputs: one accumulator to so many inputs (512 products at most)
 
 __device__ __forceinline__ uint4 ad_ld16(const void* p) {
     uint4 v;
@@ -103,22 +111,27 @@ __host__ __device__ inline AdSmem ad_smem(uint32_t R, uint32_t tokens, uint32_t 
     return s;
 }
 
-// The sums of a warp, one token's rank rows side by side, rows of rp + 4 floats: a fragment's stores and the reads along the rank meet no bank twice
+// The sums of a warp, one token's rank rows side by side, rows of rp + 4 floats: a fragment's stores and the reads along the rank meet no bank twice.
+// `more`: added to what is there.
 template <int MT, int NT>
-__device__ __forceinline__ void ad_put_sums(const float (&acc)[MT][NT][4], float* out, uint32_t rp, uint32_t m0) {
+__device__ __forceinline__ void ad_put_sums(const float (&acc)[MT][NT][4], float* out, uint32_t rp, uint32_t m0, bool more = false) {
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) out[(n * 8 + 2 * t + (e & 1)) * (rp + 4) + (m0 + m) * 16 + g + (e >> 1) * 8] = acc[m][n][e];
+            for (int e = 0; e < 4; ++e) {
+                float* const o = out + (n * 8 + 2 * t + (e & 1)) * (rp + 4) + (m0 + m) * 16 + g + (e >> 1) * 8;
+                *o = more ? *o + acc[m][n][e] : acc[m][n][e];
+            }
 }
 
 // One warp's share of the inner products of MT x 16 rank rows from r0 on and NT x 8 tokens: k blocks of 32 from kb on, every `step`-th.
 // The next block's operands are asked for before a block's products run.  Rows behind the last token, and rank rows behind the last, read the
 // first: what their products are is not looked at.
-template <class T, int MT, int NT>
+// CHAIN: products after which the accumulators move on to the warp's sums, or 0.
+template <class T, int MT, int NT, uint32_t CHAIN>
 __device__ __forceinline__ void ad_inner(const AdaptersArgs& a, const T* A, uint32_t R, uint32_t r0, const uint32_t* rows, uint32_t n_rows, uint32_t t0,
                                          uint32_t kb, uint32_t kb_end, uint32_t step, float* out, uint32_t rp) {
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
@@ -152,14 +165,23 @@ __device__ __forceinline__ void ad_inner(const AdaptersArgs& a, const T* A, uint
             }
     };
     ask(b0, kb);
+    uint32_t chain = 0;
+    bool more = false;
 #pragma unroll 1
     for (; kb < kb_end; kb += 2 * step) {
+        if (CHAIN && chain == CHAIN) {
+            ad_put_sums<MT, NT>(acc, out, rp, 0, more);
+#pragma unroll
+            for (int i = 0; i < MT * NT * 4; ++i) acc[i / (NT * 4)][i / 4 % NT][i % 4] = 0.f;
+            more = true; chain = 0;
+        }
+        chain += 4;
         ask(b1, kb + step);
         multiply(b0);
         ask(b0, kb + 2 * step);
         multiply(b1);
     }
-    ad_put_sums<MT, NT>(acc, out, rp, 0);
+    ad_put_sums<MT, NT>(acc, out, rp, 0, more);
 }
 
 __device__ __forceinline__ void ad_copy16(uint32_t dst, const void* src, bool there) {
@@ -173,8 +195,9 @@ __device__ __forceinline__ uint4 ad_lds16(uint32_t addr) {
 // 17 .. 64 tokens: the rows of x and A go through a ring of stages of 64 inputs in shared memory (fragment loads straight from memory keep too few
 // bytes in flight: 2 TB/s over the GPU).  In a stage 16-byte chunk c of row r lies at c ^ (4 (r odd)): the eight lanes of a load phase (two rows,
 // four chunks) meet no bank twice.  A warp takes 16 NH tokens from row n0 on, block kq of the stage's two blocks of 32 inputs, and MT of the pass'
-// m-tiles from m0 on.  Rows that were not copied give products that are not looked at.
-template <class T, int MT, int NT>
+// m-tiles from m0 on.  Rows that were not copied give products that are not looked at.  CHAIN: products after which the accumulators move on to
+// sums in registers, or 0.
+template <class T, int MT, int NT, uint32_t CHAIN>
 __device__ __forceinline__ void ad_inner_ring(const AdaptersArgs& a, const AdSmem& L, const T* A, uint32_t r0, uint32_t rr, const uint32_t* rows,
                                               uint32_t n_rows, uint32_t t0, uint32_t k0, uint32_t k1, uint32_t smem, uint32_t n0, uint32_t kq, uint32_t m0,
                                               float* out) {
@@ -188,8 +211,8 @@ __device__ __forceinline__ void ad_inner_ring(const AdaptersArgs& a, const AdSme
         xs[i] = r < n_rows ? static_cast<const T*>(a.x) + (size_t)(t0 + rows[r]) * a.ld_x + k0 + chunk * 8 : nullptr;
         as[i] = r < rr ? A + (size_t)(r0 + r) * a.K + k0 + chunk * 8 : nullptr;
     }
-    float acc[MT][NT][4] = {};
-    uint32_t ask_slot = 0, ask_st = 0;
+    float acc[MT][NT][4] = {}, sum[MT][NT][4] = {};
+    uint32_t ask_slot = 0, ask_st = 0, chain = 0;
     auto ask = [&]() {
         if (ask_st < n_st) {
             const uint32_t to = to0 + ask_slot * L.stage, k = ask_st * AD_KS;
@@ -229,10 +252,19 @@ __device__ __forceinline__ void ad_inner_ring(const AdaptersArgs& a, const AdSme
                 ad_mma<T>(acc[m][n], lo.z, hi.z, lo.w, hi.w, x[n].z, x[n].w);
             }
         }
+        if (CHAIN && ((chain += 2) == CHAIN || st + 1 == n_st)) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { sum[m][n][e] += acc[m][n][e]; acc[m][n][e] = 0.f; }
+            chain = 0;
+        }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();                                     // the warps' sums lie where the ring was
-    ad_put_sums<MT, NT>(acc, out, L.rp, m0);
+    ad_put_sums<MT, NT>(CHAIN ? sum : acc, out, L.rp, m0);
 }
 
 // two 16-bit values to f32
@@ -250,7 +282,8 @@ __device__ __forceinline__ uint32_t ad_pack(float x, float y, __half) {
 // (c / 2) 8 + 2 j + c % 2 of the block, so that a lane ends up with eight consecutive outputs of a token.  The next 32 rank columns of B are
 // asked for before a product, 16-bit bases a block ahead.  The parts' rows behind the last token hold anything, those of rank columns behind
 // the last hold zeros.
-template <class T, class O, int MT>
+// ROUNDED: 32 rank columns are summed by themselves, the small parts first, and added with rounding.
+template <class T, class O, int MT, bool ROUNDED>
 __device__ __forceinline__ void ad_outer(const AdaptersArgs& a, const T* B, uint32_t R, uint32_t fb, uint32_t fb_end, const uint32_t* rows, uint32_t n_rows,
                                          uint32_t t0, uint32_t u, uint32_t u_part, uint32_t pitch, const float* row_scale) {
     const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
@@ -305,8 +338,32 @@ __device__ __forceinline__ void ad_outer(const AdaptersArgs& a, const T* B, uint
     for (; fb < fb_end; fb += AD_WARPS) {
         float acc[MT][4][4] = {};
         auto multiply = [&](const uint4 (&b)[4], uint32_t k) {
+            constexpr int NP = AD_PARTS<T, O>;
+            if constexpr (ROUNDED) {
 #pragma unroll
-            for (int part = 0; part < AD_PARTS<T, O>; ++part)
+                for (int m = 0; m < MT; ++m) {
+                    uint4 lo[NP], hi[NP];
+#pragma unroll
+                    for (int part = 0; part < NP; ++part) {
+                        const uint32_t at = u0 + part * u_part + m * 16 * pitch + k * 2;
+                        lo[part] = ad_lds16(at); hi[part] = ad_lds16(at + 8 * pitch);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float s[4] = {};
+#pragma unroll
+                        for (int part = NP - 1; part >= 0; --part) {
+                            ad_mma<T>(s, lo[part].x, hi[part].x, lo[part].y, hi[part].y, b[j].x, b[j].y);
+                            ad_mma<T>(s, lo[part].z, hi[part].z, lo[part].w, hi[part].w, b[j].z, b[j].w);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[m][j][e] += s[e];
+                    }
+                }
+                return;
+            }
+#pragma unroll
+            for (int part = 0; part < NP; ++part)
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     const uint32_t at = u0 + part * u_part + m * 16 * pitch + k * 2;
@@ -458,7 +515,7 @@ __device__ __forceinline__ void ad_fold(const AdaptersArgs& a, uint32_t C, uint3
 }
 
 // One adapter's n_rows <= 16 n_q tokens t0 + sh.rows[..], by the whole cluster, n_q = 1, 2 or 4.
-template <class T, class O>
+template <class T, class O, AdSums SUMS>
 __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, uint8_t* smem, AdShared& sh, uint32_t C, uint32_t rank, int32_t id,
                                         uint32_t n_rows, uint32_t n_q, uint32_t t0) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, base_s = smem_u32(smem);
@@ -472,6 +529,7 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
     const T* B = static_cast<const T*>(a.b) + (size_t)id * a.b_stride;
 
     // ---- inner product: this CTA's inputs ----
+    constexpr uint32_t CHAIN = ad_chain<O, SUMS>;
     for (uint32_t r0 = 0; r0 < R; r0 += AD_MR) {
         const uint32_t rr = min(R - r0, AD_MR);                      // rank rows of the pass
         uint32_t n_sums;                                             // partial sums of a value, one after the other n_next floats apart
@@ -480,13 +538,13 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
             float* const mine = warp_part + warp * region;
             n_sums = AD_WARPS;
             if (n_rows <= 8) {
-                if (rr <= 16) ad_inner<T, 1, 1>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
-                else if (rr <= 32) ad_inner<T, 2, 1>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
-                else ad_inner<T, 4, 1>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                if (rr <= 16) ad_inner<T, 1, 1, CHAIN>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                else if (rr <= 32) ad_inner<T, 2, 1, CHAIN>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                else ad_inner<T, 4, 1, CHAIN>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
             } else {
-                if (rr <= 16) ad_inner<T, 1, 2>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
-                else if (rr <= 32) ad_inner<T, 2, 2>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
-                else ad_inner<T, 4, 2>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                if (rr <= 16) ad_inner<T, 1, 2, CHAIN>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                else if (rr <= 32) ad_inner<T, 2, 2, CHAIN>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
+                else ad_inner<T, 4, 2, CHAIN>(a, A, R, r0, sh.rows, n_rows, t0, kb0 + warp, kb1, AD_WARPS, mine, L.rp);
             }
         } else {
             // warp = (tokens, inputs, m-tiles): 4 x 2 x 1, or 2 x 2 x 2 (where there is one m-tile, both halves take it)
@@ -494,12 +552,12 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
             float* const mine = warp_part + (q * 2 + kq) * region;
             n_sums = 2;
             if (n_q == 4) {
-                if (L.rp == 16) ad_inner_ring<T, 1, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, 0, mine);
-                else if (L.rp == 32) ad_inner_ring<T, 2, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, 0, mine);
-                else ad_inner_ring<T, 4, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, 0, mine);
+                if (L.rp == 16) ad_inner_ring<T, 1, 2, CHAIN>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, 0, mine);
+                else if (L.rp == 32) ad_inner_ring<T, 2, 2, CHAIN>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, 0, mine);
+                else ad_inner_ring<T, 4, 2, CHAIN>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, 0, mine);
             } else {
-                if (L.rp <= 32) ad_inner_ring<T, 1, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, L.rp == 16 ? 0 : mh, mine);
-                else ad_inner_ring<T, 2, 2>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, mh * 2, mine);
+                if (L.rp <= 32) ad_inner_ring<T, 1, 2, CHAIN>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, L.rp == 16 ? 0 : mh, mine);
+                else ad_inner_ring<T, 2, 2, CHAIN>(a, L, A, r0, rr, sh.rows, n_rows, t0, kb0 * 32, k_end, base_s, q * 16, kq, mh * 2, mine);
             }
         }
         __syncthreads();
@@ -519,15 +577,16 @@ __device__ __forceinline__ void ad_unit(const AdaptersArgs& a, const AdSmem& L, 
     ad_fold<T, AD_PARTS<T, O>, 4, 1>(a, C, rank, id, R, n_rows, warp, base_s + L.part, L.r16, smem_u32(sh.scale), parts);
     cluster_sync_all();
     // ---- outer product: this CTA's outputs ----
+    constexpr bool ROUNDED = SUMS == AD_ROUNDED;
     if (n_rows <= 16)
-        ad_outer<T, O, 1>(a, B, R, fb0 + warp, fb1, sh.rows, n_rows, t0, base_s + L.u, L.u_part, L.pitch, sh.scale);
+        ad_outer<T, O, 1, ROUNDED>(a, B, R, fb0 + warp, fb1, sh.rows, n_rows, t0, base_s + L.u, L.u_part, L.pitch, sh.scale);
     else
         for (uint32_t h = 0; h < n_rows; h += 32)
             if (n_rows - h <= 16)
-                ad_outer<T, O, 1>(a, B, R, fb0 + warp, fb1, sh.rows + h, n_rows - h, t0, base_s + L.u + h * L.pitch, L.u_part, L.pitch, sh.scale + h);
+                ad_outer<T, O, 1, ROUNDED>(a, B, R, fb0 + warp, fb1, sh.rows + h, n_rows - h, t0, base_s + L.u + h * L.pitch, L.u_part, L.pitch, sh.scale + h);
             else
-                ad_outer<T, O, 2>(a, B, R, fb0 + warp, fb1, sh.rows + h, min(n_rows - h, 32u), t0, base_s + L.u + h * L.pitch, L.u_part, L.pitch,
-                                  sh.scale + h);
+                ad_outer<T, O, 2, ROUNDED>(a, B, R, fb0 + warp, fb1, sh.rows + h, min(n_rows - h, 32u), t0, base_s + L.u + h * L.pitch, L.u_part, L.pitch,
+                                           sh.scale + h);
     __syncthreads();
 }
 
@@ -539,7 +598,7 @@ __device__ __forceinline__ uint32_t ad_place(const AdaptersArgs& a, uint32_t t, 
 }
 
 // Up to 64 tokens, or more adapters than the sorting form counts: tile by tile
-template <class T, class O>
+template <class T, class O, AdSums SUMS>
 __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const AdaptersArgs a, const uint32_t C, const uint32_t slots) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ AdShared sh;
@@ -600,7 +659,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_tile_kernel(const A
             if (lane == 0) sh.n[1] = n;
         }
         __syncthreads();
-        ad_unit<T, O>(a, L, smem, sh, C, rank, id, sh.n[1], sh.n[1] <= 16 ? 1 : sh.n[1] <= 32 ? 2 : 4, t0);
+        ad_unit<T, O, SUMS>(a, L, smem, sh, C, rank, id, sh.n[1], sh.n[1] <= 16 ? 1 : sh.n[1] <= 32 ? 2 : 4, t0);
     }
 }
 
@@ -706,7 +765,7 @@ __device__ __forceinline__ AdUnit ad_find(const AdSort<PLACES>& so, uint32_t n_p
     return r;
 }
 
-template <class T, class O, uint32_t PLACES>
+template <class T, class O, AdSums SUMS, uint32_t PLACES>
 __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const AdaptersArgs a, const uint32_t C, const uint32_t per_seg, const uint32_t seg_len, const uint32_t tt) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ AdShared sh;
@@ -727,7 +786,7 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
             ad_copy<O>(a, sh.rows, un.rows, t0, C, rank);
             __syncthreads();
         } else {
-            ad_unit<T, O>(a, L, smem, sh, C, rank, (int32_t)un.place, un.rows, un.per <= 16 ? 1 : un.per <= 32 ? 2 : 4, t0);   // one split for all units of an adapter
+            ad_unit<T, O, SUMS>(a, L, smem, sh, C, rank, (int32_t)un.place, un.rows, un.per <= 16 ? 1 : un.per <= 32 ? 2 : 4, t0);   // one split for all units of an adapter
         }
     }
 }
@@ -1110,7 +1169,7 @@ static AbClusters ab_clusters(const void* kernel, uint32_t n_parts, int sm_count
     }
     return c;
 }
-template <class T, class O>
+template <class T, class O, AdSums SUMS>
 static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     const AdSmem L = ad_smem(a.R, a.T, AD_PARTS<T, O>);
     const uint32_t sms = (uint32_t)a.sm_count;
@@ -1128,7 +1187,7 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
         const uint32_t C = spread((uint64_t)tiles * distinct, room, 2);
         uint32_t slots = room / (C * tiles);
         slots = slots < 1 ? 1 : slots > distinct ? distinct : slots;
-        return ad_launch(adapters_tile_kernel<T, O>, C, slots * tiles, AD_WARPS * 32, L.bytes, st, a, C, slots);
+        return ad_launch(adapters_tile_kernel<T, O, SUMS>, C, slots * tiles, AD_WARPS * 32, L.bytes, st, a, C, slots);
     }
     const uint32_t segs = (a.T + AD_SEG - 1) / AD_SEG, tokens = (a.T + segs - 1) / segs;   // segments all alike
     // a segment's units: about as many as it has adapters, or 64 tokens
@@ -1171,12 +1230,16 @@ static cudaError_t adapters_launch(const AdaptersArgs& a, cudaStream_t st) {
     }
     uint32_t per_seg = room / (C * segs);
     per_seg = per_seg < 1 ? 1 : per_seg > cut + tokens / tt + 1 ? cut + tokens / tt + 1 : per_seg;
-    return ad_launch(few ? adapters_sorted_kernel<T, O, AD_FEW> : adapters_sorted_kernel<T, O, AD_MANY>, C, per_seg * segs, AD_WARPS * 32, L.bytes + sort, st, a, C,
+    return ad_launch(few ? adapters_sorted_kernel<T, O, SUMS, AD_FEW> : adapters_sorted_kernel<T, O, SUMS, AD_MANY>, C, per_seg * segs, AD_WARPS * 32, L.bytes + sort, st, a, C,
                      per_seg, tokens, tt);
 }
+template <class T>
+static cudaError_t adapters_out(const AdaptersArgs& a, cudaStream_t st) {
+    if (a.out_dtype == DT_F32) return a.R > 128 ? adapters_launch<T, float, AD_ROUNDED>(a, st) : adapters_launch<T, float, AD_CHAINED>(a, st);
+    return a.K > AD_LONG ? adapters_launch<T, T, AD_CHAINED>(a, st) : adapters_launch<T, T, AD_PLAIN>(a, st);
+}
 cudaError_t launch_adapters(const AdaptersArgs& a, cudaStream_t st) {
-    if (a.dtype == DT_BF16) return a.out_dtype == DT_F32 ? adapters_launch<__nv_bfloat16, float>(a, st) : adapters_launch<__nv_bfloat16, __nv_bfloat16>(a, st);
-    return a.out_dtype == DT_F32 ? adapters_launch<__half, float>(a, st) : adapters_launch<__half, __half>(a, st);
+    return a.dtype == DT_BF16 ? adapters_out<__nv_bfloat16>(a, st) : adapters_out<__half>(a, st);
 }
 
 }  // namespace mlxs

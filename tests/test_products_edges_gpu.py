@@ -191,3 +191,34 @@ def test_adapters_f32_outputs_are_as_exact_as_f32_sums(moe, T, n, R, dtype, base
     """Few inputs: what is kept of the inner product decides."""
     off, off32 = adapters_off(moe, T, n, R, 264, 136, dtype, based)
     assert as_f32(off, off32), (off, off32)
+
+
+SUMS = [(1, 1, 16, 5120, 2304), (16, 1, 16, 6144, 512), (40, 2, 64, 5120, 520), (64, 1, 32, 6144, 520), (300, 2, 256, 6144, 520), (4000, 8, 16, 5120, 2304), (3000, 600, 24, 4096, 520)]
+
+
+def check_sums(moe, T, n, R, K, N, dtype, based):
+    off, off32 = adapters_off(moe, T, n, R, K, N, dtype, based)
+    assert as_f32(off, off32), (off, off32)
+
+
+def check_one_sign(moe, T, n, R, K, dtype):
+    """Inner products of one sign drift together, and the outputs with them; 2^-20 beside it for the outer product."""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    x, a = one_sign(gen, T, K, dtype=DT[dtype]), (one_sign(gen, n, R, K, dtype=torch.float32) / K).to(DT[dtype])
+    b = torch.randn(n, 136, R, device="cuda", generator=gen).to(DT[dtype])
+    ids = torch.randint(0, n, (T,), device="cuda", generator=gen).to(torch.int32)
+    off = norm_off(lora(moe, x, a, b, ids, torch.float32), lora_plain(x, a, b, ids, None, None, torch.float64))
+    assert off <= one_sign_bound(K / 256) + 2.0 ** -20, off
+
+
+@pytest.mark.parametrize("based", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T, n, R, K, N", SUMS)
+def test_adapters_inner_sums(moe, T, n, R, K, N, dtype, based):
+    check_sums(moe, T, n, R, K, N, dtype, based)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T, n, R, K", [(1, 1, 16, 262144), (40, 1, 64, 262144), (300, 2, 200, 65536 + 8), (1000, 2, 16, 262144), (3000, 600, 8, 16384)])
+def test_adapters_long_inner_sums_of_one_sign(moe, T, n, R, K, dtype):
+    check_one_sign(moe, T, n, R, K, dtype)
