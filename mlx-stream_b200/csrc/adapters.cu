@@ -805,8 +805,13 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
 // 7,000, outer 40,000 (16 blocks of 128 outputs; each a chain of tensor-memory read, turn, base and store over eight warps): 55 us against 71 with
 // mma.sync.  Measured and not kept: base through the ring (52 -> 51 us, rank 128 with f32 outputs 36 -> 51), prefetches of x and base into L2 (their issue
 // takes what they save), 64-byte pieces of base one block further ahead.
-// The inner product's accumulator truncates (see the grouped products): its inputs are dealt out in order to up to six accumulators, added in f32.
-constexpr uint32_t AB_CHAIN = 8, AB_CHAINS = 6, AB_D2 = AB_CHAINS * 64;   // stages, accumulators of 64 columns, the outputs' first column
+// The accumulators truncate (see the grouped products).  The inner product's stages go in order to accumulators of a few stages each, three to a buffer of two;
+// the epilogue warps add a buffer's, rounding, to sums in shared memory while the next one fills, so an inner product of any length has chains of
+// ab_chain stages.  (Six accumulators that shared all of a CTA's stages: 8192 f16 tokens of six, rank 64, 5120 inputs, f32 outputs, 1.27e-6 off 64 bits; 9000
+// of two, 65,536 inputs of one sign, 6.8e-5.)  Of u's parts the small ones are multiplied first, under the large one's truncations.
+constexpr uint32_t AB_CHAINS = 3, AB_D2 = 2 * AB_CHAINS * 64;        // accumulators of 64 columns to a buffer, the outputs' first column
+template <class T, class O>
+constexpr uint32_t ab_chain = sizeof(O) == 2 ? 32 : std::is_same<T, __half>::value ? 4 : 8;   // stages: f16 products lose about twice as much
 constexpr uint32_t AB_MOST_SLOTS = 9, AB_MAX_R = 128, AB_MIN_ROWS = 16;   // ranks to, tokens per unit from
 constexpr uint32_t AB_LITTLE = 12000;                                // tokens x rank that mma.sync does sooner
 constexpr uint32_t AB_U_BYTES = 64 * 128;                            // one part of 64 rank columns of the unit's tokens
@@ -861,7 +866,7 @@ __device__ __forceinline__ void ab_copy(uint32_t dst, const void* src, uint32_t 
 template <class T, class O>
 __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapters_tensor_kernel(const __grid_constant__ AbParams P) {
     extern __shared__ uint8_t smem_any[];
-    __shared__ __align__(8) uint64_t full_bar[AB_MOST_SLOTS], empty_bar[AB_MOST_SLOTS], d1_full, d1_empty, d2_full[2], d2_empty[2], part_ready, u_ready, u_go;
+    __shared__ __align__(8) uint64_t full_bar[AB_MOST_SLOTS], empty_bar[AB_MOST_SLOTS], d1_full[2], d1_empty[2], d2_full[2], d2_empty[2], part_ready, u_ready, u_go;
     __shared__ uint32_t s_tmem, s_scan[AD_WARPS];
     __shared__ float s_scale[AD_TT];
     __shared__ volatile int s_abort;
@@ -875,8 +880,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
     AdSort<AD_FEW>& so = *reinterpret_cast<AdSort<AD_FEW>*>(ring_p + L.sort);
     if (tid == 0) {
         for (uint32_t s = 0; s < L.slots; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
-        mbar_init(&d1_full, 1); mbar_init(&d1_empty, AD_WARPS);
-        for (int b = 0; b < 2; ++b) { mbar_init(&d2_full[b], 1); mbar_init(&d2_empty[b], AD_WARPS); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&d1_full[b], 1); mbar_init(&d1_empty[b], AD_WARPS); mbar_init(&d2_full[b], 1); mbar_init(&d2_empty[b], AD_WARPS); }
         mbar_init(&part_ready, C); mbar_init(&u_ready, C); mbar_init(&u_go, 1);
         s_abort = 0;
         mbar_fence_init();
@@ -893,7 +897,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
     const uint32_t tmem = s_tmem, n_units = so.first[n_places] >> 16;
     const uint32_t n_ks = (a.K + 63) / 64, ks0 = rank * n_ks / C, ks1 = (rank + 1) * n_ks / C;
     const uint32_t n_fb = (a.N + 127) / 128, fb0 = rank * n_fb / C, fb1 = (rank + 1) * n_fb / C;
-    const uint32_t per_chain = max(AB_CHAIN, (ks1 - ks0 + AB_CHAINS - 1) / AB_CHAINS), n_chains = (ks1 - ks0 + per_chain - 1) / per_chain;
+    constexpr uint32_t CHAIN = ab_chain<T, O>, ROUND = AB_CHAINS * CHAIN;
     auto give_up = [&](uint32_t code) { if (!s_abort) atomicMax(a.status, code); s_abort = 1; };
     auto rank_of = [&](uint32_t place) {
         const int32_t given = a.ranks ? a.ranks[place] : (int32_t)a.R;
@@ -949,7 +953,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
     } else if (warp == AD_WARPS) {
         // ---------------- issuer ----------------
         const uint32_t fmt = std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16, idesc = umma_idesc(fmt, 64);
-        uint32_t s = 0, ph = 0, n_done = 0, n_blocks = 0;
+        uint32_t s = 0, ph = 0, n_done = 0, n_rounds = 0, n_blocks = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
             if (!ok) return;
@@ -962,45 +966,60 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
             const AdUnit un = ad_find(so, n_places, AD_TT, u);
             if (un.place == a.n_adapters) continue;
             const uint32_t R = rank_of(un.place), chunks = (R + 63) / 64;
-            if (R) {
-                wait(&d1_empty, (n_done & 1u) ^ 1u, ST_WAIT_EMPTY);
-                uint32_t d1 = tmem, in_chain = 0;
-                for (uint32_t ks = ks0; ks < ks1 && ok; ++ks) {
+            for (uint32_t k0 = ks0, chain = 0; k0 < ks1 && ok && R; k0 += CHAIN) {
+                const uint32_t buf = n_rounds & 1u, k1 = min(k0 + CHAIN, ks1);
+                if (chain == 0) wait(&d1_empty[buf], (n_rounds >> 1 & 1u) ^ 1u, ST_WAIT_EMPTY);
+                const uint32_t d1 = __shfl_sync(0xFFFFFFFFu, tmem + (buf * AB_CHAINS + chain) * 64, 0);
+                for (uint32_t ks = k0; ks < k1 && ok; ++ks) {
                     wait(&full_bar[s], ph, ST_WAIT_FULL);
                     if (!ok) break;
                     const uint32_t at = __shfl_sync(0xFFFFFFFFu, (ring + s * L.slot) >> 4, 0) | 1u << 16, x_at = at + (L.x >> 4);
                     if (elect_one()) {
 #pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) umma_f16_lo(d1, at + j * 2, x_at + j * 2, UMMA_SW128_HI, idesc, in_chain | j ? 1u : 0u);
+                        for (uint32_t j = 0; j < 4; ++j) umma_f16_lo(d1, at + j * 2, x_at + j * 2, UMMA_SW128_HI, idesc, ks != k0 || j ? 1u : 0u);
                         umma_commit(&empty_bar[s]);
                     }
                     __syncwarp();
                     next();
-                    if (++in_chain == per_chain) { in_chain = 0; d1 += 64; }
                 }
                 if (!ok) break;
-                if (elect_one()) umma_commit(&d1_full);
-                __syncwarp();
+                if (++chain == AB_CHAINS || k1 == ks1) {
+                    if (elect_one()) umma_commit(&d1_full[buf]);
+                    __syncwarp();
+                    chain = 0;
+                    ++n_rounds;
+                }
             }
+            if (!ok) break;
             // the parts of u are there (a unit without a rank has none: its outputs are base)
             if (R) wait(&u_go, n_done & 1u, ST_WAIT_FULL);
             for (uint32_t fb = fb0; fb < fb1 && ok && R; ++fb, ++n_blocks) {
                 const uint32_t buf = n_blocks & 1u, acc = tmem + AB_D2 + buf * 64;
                 wait(&d2_empty[buf], (n_blocks >> 1 & 1u) ^ 1u, ST_WAIT_EMPTY);
+                uint32_t first = 0, first_b = 0;                       // of two chunks the first one's slot, whose large part comes last
+                const uint32_t u_at = __shfl_sync(0xFFFFFFFFu, (ring + L.u) >> 4, 0) | 1u << 16;
+                const auto multiply = [&](uint32_t at, uint32_t c, uint32_t part) {
+                    const uint32_t ua = u_at + (c * NP + part) * (AB_U_BYTES >> 4), steps = (min(R - c * 64, 64u) + 15) / 16;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j)
+                        if (j < steps) umma_f16_lo(acc, at + j * 2, ua + j * 2, UMMA_SW128_HI, idesc, c || part + 1 < NP || j ? 1u : 0u);
+                };
                 for (uint32_t c = 0; c < chunks && ok; ++c) {
                     wait(&full_bar[s], ph, ST_WAIT_FULL);
                     if (!ok) break;
-                    const uint32_t at = __shfl_sync(0xFFFFFFFFu, (ring + s * L.slot) >> 4, 0) | 1u << 16, steps = (min(R - c * 64, 64u) + 15) / 16;
-                    const uint32_t ua = __shfl_sync(0xFFFFFFFFu, (ring + L.u + c * NP * AB_U_BYTES) >> 4, 0) | 1u << 16;
+                    const uint32_t at = __shfl_sync(0xFFFFFFFFu, (ring + s * L.slot) >> 4, 0) | 1u << 16;
+                    const bool last = c + 1 == chunks;
                     if (elect_one()) {
 #pragma unroll
-                        for (uint32_t part = 0; part < NP; ++part)
-#pragma unroll
-                            for (uint32_t j = 0; j < 4; ++j)
-                                if (j < steps) umma_f16_lo(acc, at + j * 2, ua + part * (AB_U_BYTES >> 4) + j * 2, UMMA_SW128_HI, idesc, c | part | j ? 1u : 0u);
-                        umma_commit(&empty_bar[s]);
+                        for (uint32_t part = NP - 1; part; --part) multiply(at, c, part);
+                        if (last) {
+                            multiply(at, c, 0);
+                            umma_commit(&empty_bar[s]);
+                            if (c) { multiply(first_b, 0, 0); umma_commit(&empty_bar[first]); }
+                        }
                     }
                     __syncwarp();
+                    first = s; first_b = at;
                     next();
                 }
                 if (!ok) break;
@@ -1015,7 +1034,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         float* const part = reinterpret_cast<float*>(ring_p + L.part);
         const uint32_t r16 = (a.R + 15) / 16 * 16, turn = ring + L.turn + warp * AB_TURN;
         const AbParts<NP> parts{ring + L.u};
-        uint32_t n_done = 0, n_blocks = 0;
+        uint32_t n_done = 0, n_rounds = 0, n_blocks = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(bar), parity, &s_abort));
@@ -1037,25 +1056,33 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
                 ad_copy<O>(a, so.order + un.at, un.rows, t0, C, rank);
                 continue;
             }
-            // inner sums of this CTA's inputs
-            wait(&d1_full, n_done & 1u);
-            tc_fence_after();
-            if (ok && q * 32 < R)
-                for (uint32_t c = half * 32; c < half * 32 + 32 && c < un.rows; c += 16) {
-                    float sum[16];
-                    for (uint32_t chain = 0; chain < n_chains; ++chain) {
-                        uint32_t v[16];
-                        tmem_ld16(tmem + chain * 64 + c + ((q * 32u) << 16), v);
+            // inner sums of this CTA's inputs, a buffer of accumulators at a time
+            for (uint32_t k0 = ks0; k0 < ks1; k0 += ROUND, ++n_rounds) {
+                const uint32_t buf = n_rounds & 1u, n_chains = (min(ROUND, ks1 - k0) + CHAIN - 1) / CHAIN;
+                if (!wait(&d1_full[buf], n_rounds >> 1 & 1u)) break;
+                tc_fence_after();
+                if (q * 32 < R)
+                    for (uint32_t c = half * 32; c < half * 32 + 32 && c < un.rows; c += 16) {
+                        float sum[16];
+                        const bool mine = q * 32 + lane < r16;
+                        float* const o = part + c * r16 + q * 32 + lane;
+                        if (k0 != ks0 && mine)                       // all on their way before the accumulators are read
 #pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j) sum[j] = chain ? sum[j] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
+                            for (uint32_t j = 0; j < 16; ++j) sum[j] = o[j * r16];
+                        for (uint32_t chain = 0; chain < n_chains; ++chain) {
+                            uint32_t v[16];
+                            tmem_ld16(tmem + (buf * AB_CHAINS + chain) * 64 + c + ((q * 32u) << 16), v);
+#pragma unroll
+                            for (uint32_t j = 0; j < 16; ++j) sum[j] = chain || k0 != ks0 ? sum[j] + __uint_as_float(v[j]) : __uint_as_float(v[j]);
+                        }
+                        if (mine)
+#pragma unroll
+                            for (uint32_t j = 0; j < 16; ++j) o[j * r16] = sum[j];
                     }
-                    if (q * 32 + lane < r16)
-#pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j) part[(c + j) * r16 + q * 32 + lane] = sum[j];
-                }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&d1_empty);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d1_empty[buf]);
+            }
             if (!together()) break;
             if (etid < C) mbar_arrive_cluster(map_to_rank(smem_u32(&part_ready), etid));
             wait(&part_ready, n_done & 1u);

@@ -194,6 +194,7 @@ def test_adapters_f32_outputs_are_as_exact_as_f32_sums(moe, T, n, R, dtype, base
 
 
 SUMS = [(1, 1, 16, 5120, 2304), (16, 1, 16, 6144, 512), (40, 2, 64, 5120, 520), (64, 1, 32, 6144, 520), (300, 2, 256, 6144, 520), (4000, 8, 16, 5120, 2304), (3000, 600, 24, 4096, 520)]
+SUMS_TENSOR = [(1000, 8, 64, 5120, 2304), (1000, 8, 72, 6144, 264), (4100, 3, 120, 1024, 520), (1000, 8, 128, 5120, 520), (8192, 6, 64, 5120, 520), (4100, 300, 40, 2304, 264)]
 
 
 def check_sums(moe, T, n, R, K, N, dtype, based):
@@ -221,4 +222,17 @@ def test_adapters_inner_sums(moe, T, n, R, K, N, dtype, based):
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("T, n, R, K", [(1, 1, 16, 262144), (40, 1, 64, 262144), (300, 2, 200, 65536 + 8), (1000, 2, 16, 262144), (3000, 600, 8, 16384)])
 def test_adapters_long_inner_sums_of_one_sign(moe, T, n, R, K, dtype):
+    check_one_sign(moe, T, n, R, K, dtype)
+
+
+@pytest.mark.parametrize("based", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T, n, R, K, N", SUMS_TENSOR)
+def test_adapters_inner_sums_on_the_tensor_cores(moe, T, n, R, K, N, dtype, based):
+    check_sums(moe, T, n, R, K, N, dtype, based)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T, n, R, K", [(1000, 2, 64, 262144), (4100, 2, 64, 65536 + 8), (4100, 300, 40, 16384), (2048, 16, 128, 24576)])
+def test_adapters_long_inner_sums_of_one_sign_on_the_tensor_cores(moe, T, n, R, K, dtype):
     check_one_sign(moe, T, n, R, K, dtype)
