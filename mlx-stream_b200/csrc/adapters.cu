@@ -489,7 +489,7 @@ __device__ __forceinline__ void ad_fold(const AdaptersArgs& a, uint32_t C, uint3
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const uint32_t r = j * 64 + lane * 2;
-                v[n][j][0] *= scale;
+                v[n][j][0] = r < R ? v[n][j][0] * scale : 0.f;       // zeros behind the rank whatever the scale
                 v[n][j][1] = r + 1 < R ? v[n][j][1] * scale : 0.f;
                 most = fmaxf(most, fmaxf(fabsf(v[n][j][0]), fabsf(v[n][j][1])));
             }

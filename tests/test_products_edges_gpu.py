@@ -236,3 +236,23 @@ def test_adapters_inner_sums_on_the_tensor_cores(moe, T, n, R, K, N, dtype, base
 @pytest.mark.parametrize("T, n, R, K", [(1000, 2, 64, 262144), (4100, 2, 64, 65536 + 8), (4100, 300, 40, 16384), (2048, 16, 128, 24576)])
 def test_adapters_long_inner_sums_of_one_sign_on_the_tensor_cores(moe, T, n, R, K, dtype):
     check_one_sign(moe, T, n, R, K, dtype)
+
+
+@pytest.mark.parametrize("dtype, out", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("T, n, R", [(3, 2, 16), (50, 2, 32), (200, 2, 24), (1000, 8, 64)])
+def test_adapters_infinite_scale(moe, T, n, R, dtype, out):
+    """An infinite scale makes infinities of an adapter of rank one, of the product's sign, and stays in its tokens."""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randn(T, 128, device="cuda", generator=gen).to(DT[dtype])
+    a, b = torch.randn(n, R, 128, device="cuda", generator=gen).to(DT[dtype]), torch.randn(n, 72, R, device="cuda", generator=gen).to(DT[dtype])
+    b[b == 0] = 1
+    ids = (torch.arange(T, device="cuda") % n).to(torch.int32)
+    scales, ranks = torch.ones(n, device="cuda"), torch.ones(n, device="cuda", dtype=torch.int32)
+    finite = lora(moe, x, a, b, ids, DT[out], scales=scales, ranks=ranks)
+    assert torch.isfinite(finite).all()
+    scales[1] = float("inf")
+    y = lora(moe, x, a, b, ids, DT[out], scales=scales, ranks=ranks)
+    mine = ids == 1
+    u = (x[mine].double() @ a[1, 0].double())[:, None] * b[1, :, 0].double()
+    assert (u != 0).all() and torch.equal(y[mine].double(), u.sign() * float("inf"))
+    assert torch.equal(y[~mine], finite[~mine])
