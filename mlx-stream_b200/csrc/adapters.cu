@@ -1175,7 +1175,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
 
 template <class... Params, class... Args>
 static cudaError_t ad_launch(void (*kernel)(Params...), uint32_t C, uint32_t clusters, uint32_t threads, size_t smem, cudaStream_t st, const Args&... args) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_shared(kernel);
     return e == cudaSuccess ? launch_dependent_clusters(kernel, C, clusters, threads, smem, st, args...) : e;
 }
 // clusters of 1, 2, 4, 8 CTAs of the tensor-core kernel that the device holds at once
@@ -1183,7 +1183,7 @@ struct AbClusters { uint32_t n[9]; };
 static AbClusters ab_clusters(const void* kernel, uint32_t n_parts, int sm_count) {
     AbClusters c{};
     const AbSmem L = ab_smem(AB_MAX_R, n_parts);
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L.bytes);
+    if (allow_shared(kernel) != cudaSuccess) cudaGetLastError();
     for (uint32_t C = 1; C <= 8; C *= 2) {
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;

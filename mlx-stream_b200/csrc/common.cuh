@@ -87,6 +87,32 @@ __device__ __forceinline__ void bulk_g2s(void* dst_smem, const void* src_gmem, u
                  "l"(src_gmem), "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
 }
+// A kernel's limit of dynamic shared memory belongs to the function on its device, not to a launch.  Set to a call's own size it may be lowered by
+// another host thread's call, of another handle, before the first one's launch, which then fails.  So every call sets the same: all that a block may have beside the
+// kernel's static memory.
+static inline cudaError_t allow_shared(const void* kernel) {
+    struct Known { const void* kernel; int bytes; };
+    static thread_local Known known[32];               // what is set is kept, not that it was
+    Known* k = known;
+    while (k < known + 32 && k->kernel && k->kernel != kernel) ++k;
+    int bytes = 0;
+    if (k < known + 32 && k->kernel == kernel) {
+        bytes = k->bytes;
+    } else {
+        cudaFuncAttributes fa;
+        int device = 0, most = 0;
+        cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+        if (e == cudaSuccess) e = cudaGetDevice(&device);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+        if (e != cudaSuccess) return e;
+        bytes = most - (int)fa.sharedSizeBytes;
+        if (k < known + 32) *k = Known{kernel, bytes};
+    }
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+template <class... Params>
+static inline cudaError_t allow_shared(void (*kernel)(Params...)) { return allow_shared(reinterpret_cast<const void*>(kernel)); }
+
 // Programmatic dependent launch (the chain router -> dispatch -> staging -> gate/up -> down -> combine): a kernel lets the
 // next one of the stream start while it still runs; the next one does what needs nothing of it (its prologue, the down
 // kernel its first weight copies) and then waits for the whole grid before it and for its memory.  A kernel allows its

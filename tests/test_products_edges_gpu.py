@@ -7,6 +7,8 @@ Tolerances, from the arithmetic alone.
   * f32 outputs of products of random signs are held to what f32 sums give: 2^-20 of the result in the 2-norm (eight steps: 16 instructions' truncations over an
     accumulator that holds half of its last value on average), or one and a half times the error of the same product in 32 bits, where that is more.
 """
+import threading
+
 import pytest
 import torch
 
@@ -256,3 +258,49 @@ def test_adapters_infinite_scale(moe, T, n, R, dtype, out):
     u = (x[mine].double() @ a[1, 0].double())[:, None] * b[1, :, 0].double()
     assert (u != 0).all() and torch.equal(y[mine].double(), u.sign() * float("inf"))
     assert torch.equal(y[~mine], finite[~mine])
+
+
+# ------------------------------------------------------------------------------------------------------------
+# several host threads
+# ------------------------------------------------------------------------------------------------------------
+def in_threads(works):
+    """Each of `works` in a thread of its own, all at once; what they raised."""
+    raised, ready = [], threading.Barrier(len(works))
+
+    def run(work):
+        try:
+            torch.cuda.set_device(0)
+            ready.wait()
+            work()
+        except Exception as e:                           # noqa: BLE001
+            raised.append(e)
+    threads = [threading.Thread(target=run, args=(w,)) for w in works]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return raised
+
+
+@pytest.mark.parametrize("shapes", [((200, 2, 256), (200, 2, 8)), ((4000, 2, 64), (4000, 2, 128)), ((40, 2, 256), (40, 2, 16))])
+def test_adapters_of_two_handles_on_two_threads(shapes):
+    """The same kernel with another amount of shared memory from each thread."""
+    def calls(T, n, R):
+        m = pkg.MoE(pkg.make_config(128, 128, 4, 1, max_tokens=4))
+        gen = torch.Generator(device="cuda").manual_seed(R)
+        x = torch.randn(T, 64, device="cuda", generator=gen).to(torch.bfloat16)
+        a, b = torch.randn(n, R, 64, device="cuda", generator=gen).to(torch.bfloat16), torch.randn(n, 64, R, device="cuda", generator=gen).to(torch.bfloat16)
+        ids = (torch.arange(T, device="cuda") % n).to(torch.int32)
+        want = lora(m, x, a, b, ids, torch.bfloat16)
+        y = torch.empty_like(want)
+        st = torch.cuda.Stream()
+        torch.cuda.synchronize()
+
+        def work():
+            for i in range(20000):
+                m.adapters(x.data_ptr(), T, a.data_ptr(), b.data_ptr(), ids.data_ptr(), y.data_ptr(), 64, 64, R, n, stream=st.cuda_stream)
+                if i % 500 == 499:
+                    st.synchronize()
+            assert torch.equal(y, want)
+        return work
+    assert in_threads([calls(*s) for s in shapes]) == []
