@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(DTHREADS) dispatch_place_kernel(const int32_t*
 
 // above the 48 KB every kernel may use: more than 700 experts
 static cudaError_t dispatch_smem(const void* kernel, size_t bytes) {
-    return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
+    return bytes > 48 * 1024 ? allow_shared(kernel) : cudaSuccess;
 }
 
 cudaError_t launch_dispatch_large(const int32_t* ids, uint32_t A, uint32_t E, const uint8_t* loaded, DispatchTables t,

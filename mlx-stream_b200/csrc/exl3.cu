@@ -529,7 +529,7 @@ static cudaError_t launch_gemv(int nproj, int epi, int kbits, GemvParams& P, int
     P.max_parts = (uint32_t)k_parts;
 #define MLXS_LAUNCH(NP, EP, KBITS)                                                                                \
     do {                                                                                                         \
-        e = cudaFuncSetAttribute(exl3_gemv_kernel<NP, EP, KBITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+        e = allow_shared(exl3_gemv_kernel<NP, EP, KBITS>);                                                       \
         if (e != cudaSuccess) return e;                                                                          \
         e = launch_dependent(dependent, exl3_gemv_kernel<NP, EP, KBITS>, ctas, NP * 256 + 32, smem, st, P);      \
         if (e != cudaSuccess) return e;                                                                          \

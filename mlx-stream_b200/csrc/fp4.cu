@@ -518,7 +518,7 @@ cudaError_t launch_fp4_gemv(const Fp4GemvArgs& a, int down, cudaStream_t st) {
     const size_t smem = zs_bytes + (size_t)ns * P.stage_bytes;
     const int ctas = per_sm * a.sm_count;
     auto launch = [&](auto kernel) -> cudaError_t {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        const cudaError_t e = allow_shared(kernel);
         return e != cudaSuccess ? e : launch_dependent(!down || a.dependent, kernel, ctas, nproj * 256 + 32, smem, st, P);
     };
     const cudaError_t e = a.nv ? (down ? launch(fp4_gemv_kernel<1, true, false>) : launch(fp4_gemv_kernel<2, true, false>))

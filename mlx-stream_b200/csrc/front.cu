@@ -227,7 +227,7 @@ cudaError_t launch_front(const FrontArgs& a, cudaStream_t st) {
     P.rthreads = front_route_threads(a.E, a.K);
     P.by_warp = front_by_warp(a.E, a.K, a.T, a.H, a.w_router, a.smem_max) ? 1 : 0;
     const size_t smem = front_smem_bytes(a.E, a.K, a.T, a.H, a.w_router, P.by_warp);
-    cudaError_t e = cudaFuncSetAttribute(front_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_shared(front_kernel);
     if (e != cudaSuccess) return e;
     const bool barrier = a.w_router || !P.by_warp;
     // a warp per staging task (a row's 128-block; for the FP4 banks a sixteenth of a row, or a quarter where that would be more

@@ -54,7 +54,7 @@ cudaError_t launch_router_logits(const __nv_bfloat16* x, const __nv_bfloat16* w,
         return cudaGetLastError();
     }
     const size_t smem = logits_smem_bytes(H, RL_WARPS);
-    cudaError_t err = cudaFuncSetAttribute(router_logits_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t err = allow_shared(router_logits_kernel);
     if (err != cudaSuccess) return err;
     const uint32_t slots = RL_WARPS / LG_PARTS;
     router_logits_kernel<<<(E + slots - 1) / slots, RL_WARPS * 32, smem, st>>>(x, w, T, E, H, logits);

@@ -304,3 +304,35 @@ def test_adapters_of_two_handles_on_two_threads(shapes):
             assert torch.equal(y, want)
         return work
     assert in_threads([calls(*s) for s in shapes]) == []
+
+
+@pytest.mark.parametrize("T", [1, 20, 300])
+@pytest.mark.parametrize("bank", ["BANK_EXL3_K3_MUL1", "BANK_MXFP4"])
+def test_layers_of_two_handles_on_two_threads(bank, T):
+    """Handles of two geometries: the streaming kernels, the front, the router's logits and the dispatch take other amounts of shared memory."""
+    def calls(H, I, E):
+        m = pkg.MoE(pkg.make_config(H, I, E, 2, bank_kind=getattr(pkg, bank), max_tokens=T))
+        gen = torch.Generator(device="cuda").manual_seed(H)
+        logical, _ = m.record_bytes()
+        record = torch.zeros(logical, device="cuda", dtype=torch.uint8)
+        record[1::7] = 60
+        for e in range(E):
+            m.load_expert(0, e, record.data_ptr(), logical, True)
+        w = torch.randn(E, H, device="cuda", generator=gen).to(torch.bfloat16)
+        m.set_router_weight(0, w.data_ptr(), True)
+        x = torch.randn(T, H, device="cuda", generator=gen).to(torch.bfloat16)
+        y = torch.zeros(T, H, device="cuda", dtype=torch.bfloat16)
+        st = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        m.forward_x(0, x.data_ptr(), T, y.data_ptr(), st.cuda_stream)
+        torch.cuda.synchronize()
+        want = y.clone()
+
+        def work():
+            for i in range(30000 if T == 1 else 5000):
+                m.forward_x(0, x.data_ptr(), T, y.data_ptr(), st.cuda_stream)
+                if i % 100 == 99:
+                    st.synchronize()
+            assert torch.equal(y.view(torch.int16), want.view(torch.int16)) and m.stats().device_status == 0
+        return work
+    assert in_threads([calls(512, 256, 8), calls(5120, 512, 64)]) == []
