@@ -237,9 +237,9 @@ int mlxs_moe_sort_rows(mlxs_moe *h, const int32_t *slot_dev, uint32_t n, uint32_
                        uint32_t *offsets_dev, void *stream);
 /* Self-test of the bounded waits (no counterpart in the reference).  Every wait inside a kernel gives up after a
  * number of polls, records MLXS_E_DEVICE_STATUS's word and lets the CTA return; poll_limit sets that number for the
- * EXL3 streaming kernels (0 = the default, 2^20).  withhold_stage = n > 0 makes every gate/up producer leave out the
- * copies of its n-th ring stage, so the wait for that stage runs out: the call completes, the status word reads
- * "a bounded wait ran out", nothing faults and nothing is left in flight.  (0, 0) restores normal operation. */
+ * EXL3 streaming kernels and the tensor-core kernels of mlxs_moe_grouped and mlxs_moe_adapters (0 = the default, 2^20).  withhold_stage = n > 0 makes
+ * every gate/up producer, and every producer of those two, leave out the copies of its n-th ring stage, so the wait for that stage runs out: the call completes, the status word reads
+ * "a bounded wait ran out", nothing faults and nothing is left in flight; a product's rows that wait for it are not written.  (0, 0) restores normal operation. */
 int mlxs_moe_debug_wait(mlxs_moe *h, uint32_t poll_limit, uint32_t withhold_stage);
 
 /* per-stage device timing with CUDA events on the caller's stream, off by default (the reference's comptime profile

@@ -908,7 +908,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         // ---------------- a ring slot's warp: every L.slots-th stage ----------------
         const uint32_t slot = warp - AD_WARPS - 1, full = smem_u32(&full_bar[slot]), empty = smem_u32(&empty_bar[slot]), at = ring + slot * L.slot;
         const uint32_t chunk = lane & 7u, row0 = lane >> 3;
-        uint32_t ph = 0, base = 0;                                    // stages of the units before, modulo the ring
+        uint32_t ph = 0, base = 0, before = 0;                        // base: stages of the units before, modulo the ring
         bool ok = true;
         for (uint32_t u = cl % P.per_seg; u < n_units && ok; u += P.per_seg) {
             const AdUnit un = ad_find(so, n_places, AD_TT, u);
@@ -919,7 +919,8 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
 #pragma unroll
             for (uint32_t i = 0; i < AD_TT / 4; ++i) xr[i] = static_cast<const T*>(a.x) + (size_t)(t0 + so.order[un.at + min(row0 + i * 4, un.rows - 1)]) * a.ld_x;
             for (uint32_t st = (slot + L.slots - base) % L.slots; st < n_st; st += L.slots) {
-                if (!mbar_wait_warp_at(empty, ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
+                if (!mbar_wait_warp_at(empty, ph ^ 1u, &s_abort, a.poll_limit)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
+                if (a.withhold && before + st + 1 == a.withhold) { ph ^= 1u; continue; }
                 if (st < n_in) {
                     const uint32_t k = (ks0 + st) * 64;
                     if (lane == 0) {
@@ -948,8 +949,8 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
                 ph ^= 1u;
             }
             base = (base + n_st) % L.slots;
+            before += n_st;
         }
-        if (s_abort) for (int i = 0; i < 2000; ++i) __nanosleep(1000);   // copies in flight land before the memory goes
     } else if (warp == AD_WARPS) {
         // ---------------- issuer ----------------
         const uint32_t fmt = std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16, idesc = umma_idesc(fmt, 64);
@@ -957,7 +958,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
             if (!ok) return;
-            ok = mbar_wait_warp(bar, parity, &s_abort);
+            ok = mbar_wait_warp_at(smem_u32(bar), parity, &s_abort, a.poll_limit);
             if (!ok) give_up(code);
             tc_fence_after();
         };
@@ -1037,7 +1038,7 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         uint32_t n_done = 0, n_rounds = 0, n_blocks = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(bar), parity, &s_abort));
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(bar), parity, &s_abort, a.poll_limit));
             if (!ok) give_up(ST_WAIT_FULL);
             return ok;
         };
@@ -1166,9 +1167,11 @@ __global__ void __launch_bounds__((1 + AD_WARPS + AB_MOST_SLOTS) * 32, 1) adapte
         }
     }
     // every thread comes here, also after a give-up
+    if (s_abort) cluster_abort(&s_abort, C);
     tc_fence_before();
     __syncwarp();
     cluster_sync_all();
+    if (s_abort) abort_drain();                         // in every CTA of the cluster alike
     tc_fence_after();
     if (warp == AD_WARPS) tmem_free(tmem, 512);
 }

@@ -43,6 +43,13 @@ static int check_ptr(const char* who, const char* what, const void* p, uintptr_t
     return 0;
 }
 
+// the bounds of the kernels' waits (mlxs_moe_debug_wait)
+template <class Args>
+static void set_waits(Args& a, const mlxs_moe* h) {
+    if (h->dbg_poll_limit) a.poll_limit = h->dbg_poll_limit;
+    a.withhold = h->dbg_withhold;
+}
+
 extern "C" int mlxs_moe_grouped(mlxs_moe* h, const mlxs_grouped_desc* d, const void* x_dev, const void* w_dev, const uint32_t* offsets_dev,
                                 const uint32_t* order_dev, void* y_dev, void* stream) {
     const char* who = "grouped";
@@ -83,6 +90,7 @@ extern "C" int mlxs_moe_grouped(mlxs_moe* h, const mlxs_grouped_desc* d, const v
     if (!h) return mlxs_fail(MLXS_E_ARG, "grouped: null handle");
     a.x = x_dev; a.w = w_dev; a.y = y_dev; a.offsets = offsets_dev; a.order = order_dev;
     a.status = h->status; a.sm_count = h->sm_count;
+    set_waits(a, h);
     DeviceGuard dev;
     cudaError_t e = dev.enter(h->cfg.device);
     if (e == cudaSuccess) e = launch_grouped(a, (cudaStream_t)stream);
@@ -120,6 +128,7 @@ extern "C" int mlxs_moe_adapters(mlxs_moe* h, const mlxs_adapters_desc* d, const
     if (!h) return mlxs_fail(MLXS_E_ARG, "adapters: null handle");
     a.x = x_dev; a.a = a_dev; a.b = b_dev; a.base = base_dev; a.y = y_dev; a.ids = ids_dev; a.scales = scales_dev; a.ranks = ranks_dev;
     a.status = h->status; a.sm_count = h->sm_count;
+    set_waits(a, h);
     DeviceGuard dev;
     cudaError_t e = dev.enter(h->cfg.device);
     if (e == cudaSuccess) e = launch_adapters(a, (cudaStream_t)stream);
@@ -168,6 +177,7 @@ cudaError_t mlxs_run_shared_adapted(mlxs_moe* h, const LayerBank& L, const void*
         a.x = x; a.w = w; a.y = y; a.G = 1; a.K = K; a.N = N; a.rows = a.x_rows = a.y_rows = T; a.x_div = 1;
         a.dtype = DT_BF16; a.out_dtype = DT_F32; a.ld_x = a.ld_w = K; a.ld_y = ld_y; a.w_stride = (size_t)N * K;
         a.status = h->status; a.sm_count = h->sm_count;
+        set_waits(a, h);
         return launch_grouped(a, st);
     };
     auto adapt = [&](const void* x, const void* A, const void* B, uint32_t K, uint32_t N, float* y, size_t ld_y) {
@@ -177,6 +187,7 @@ cudaError_t mlxs_run_shared_adapted(mlxs_moe* h, const LayerBank& L, const void*
         a.K = K; a.N = N; a.R = d.rank; a.n_adapters = d.n_adapters; a.T = T; a.dtype = DT_BF16; a.out_dtype = DT_F32;
         a.ld_x = K; a.ld_base = a.ld_y = ld_y; a.a_stride = (size_t)d.rank * K; a.b_stride = (size_t)N * d.rank;
         a.status = h->status; a.sm_count = h->sm_count;
+        set_waits(a, h);
         return launch_adapters(a, st);
     };
     const float limit = h->cfg.act == MLXS_ACT_SWIGLU_CLAMPED ? h->cfg.act_limit : 0.f;

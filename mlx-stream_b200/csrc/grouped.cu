@@ -262,7 +262,7 @@ static cudaError_t few_launch(const GroupedArgs& a, cudaStream_t st) {
 // Sorted rows, 64 groups of 512, K 4096, gate and up of 2048: 0.86 - 0.94 ms = 1,170 - 1,280 TFLOP/s, the tensor pipe busy 81 - 84 % of the cycles at 1.57 GHz (power
 // cap); one product of 8192^3 0.73 - 0.83 ms where the library's took 0.68 - 0.70.  What is left: a 256-row item has no second accumulator buffer (512 columns are full),
 // so its epilogue (2 - 5 us of 60) stands alone, and 512 rows of a group are often three tiles of 192.
-// Every wait is bounded; on a give-up the CTA sets the status word and still meets the others at the end.
+// Every wait is bounded; on a give-up the CTA sets the status word, tells its cluster and still meets the others at the end; what the wait was for is not stored.
 constexpr uint32_t GT_KS = 64;                                   // inputs per stage: 128 bytes, one swizzle row
 constexpr uint32_t GT_STAGES = 4;
 constexpr uint32_t GT_A_HALF = 128 * GT_KS * 2;                  // 128 outputs of a stage
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
     if (warp == 0) {
         // ---------------- producer: this CTA's outputs' weights, and its half of the tile's rows where they lie in order ----------------
         const bool gather = a.gather;
-        uint32_t s = 0, ph = 0;
+        uint32_t s = 0, ph = 0, n_stage = 0;
         bool ok = true;
         for (uint32_t i = pair; i < n_items && ok; i += n_pairs) {
             const GtItem it = walk.at(i / P.n_ft);
@@ -432,8 +432,8 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
             const uint32_t hb = it.n / 2, b0 = it.p0 + rank * hb, bi = hb <= 16 ? 0 : hb <= 32 ? 1 : (hb + 31) / 32;
             const uint32_t bytes = 2 * (GT_A_BYTES + (gather ? 0 : gt_box_rows(bi) * GT_KS * 2));   // both CTAs' copies
             for (uint32_t ks = ks0; ks < ks1; ++ks) {
-                if (!mbar_wait_warp_at(smem_u32(&empty_bar[s]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
-                if (lane == 0) {
+                if (!mbar_wait_warp_at(smem_u32(&empty_bar[s]), ph ^ 1u, &s_abort, a.poll_limit)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
+                if (lane == 0 && (!a.withhold || ++n_stage != a.withhold)) {
                     const uint32_t full = map_to_rank(smem_u32(&full_bar[s]), leader), sa = ring + s * GT_A_BYTES;
                     const int32_t k = (int32_t)(ks * GT_KS);
                     if (rank == 0) mbar_expect_tx(&full_bar[s], bytes);
@@ -455,7 +455,6 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                 if (++s == GT_STAGES) { s = 0; ph ^= 1u; }
             }
         }
-        if (s_abort) for (int i = 0; i < 2000; ++i) __nanosleep(1000);   // copies in flight land before the memory goes
     } else if (warp == 1) {
         // ---------------- MMA issuer: the even CTA's, for both ----------------
         if (rank == 0) {
@@ -471,12 +470,12 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
                 for (uint32_t chain = 0; chain < n_chains && ok; ++chain) {
                     const uint32_t buf = n_done % n_buf, acc = tmem + buf * 2 * P.cap;
                     const uint32_t k0 = SUMS ? ks0 + chain * P.chain : ks0, k1 = SUMS ? min(k0 + P.chain, ks1) : ks1;
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_empty[buf]), (n_done / n_buf & 1u) ^ 1u, &s_abort));
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_empty[buf]), (n_done / n_buf & 1u) ^ 1u, &s_abort, a.poll_limit));
                     if (!ok) { give_up(ST_WAIT_EMPTY); break; }
                     tc_fence_after();
                     for (uint32_t ks = k0; ks < k1; ++ks) {
-                        ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&full_bar[s]), ph, &s_abort));
-                        if (ok && a.gather) ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&x_full[xs]), x_ph, &s_abort));
+                        ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&full_bar[s]), ph, &s_abort, a.poll_limit));
+                        if (ok && a.gather) ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&x_full[xs]), x_ph, &s_abort, a.poll_limit));
                         if (!ok) { give_up(ST_WAIT_FULL); break; }
                         tc_fence_after();
                         const uint32_t sa = ring + s * GT_A_BYTES, sb = ring + GT_X + (a.gather ? xs * x_slot : s * GT_B_BYTES);
@@ -514,7 +513,7 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
             for (uint32_t chain = 0; chain < n_chains; ++chain) {
             const uint32_t buf = n_done % n_buf, lanes = (q * 32u) << 16;
             const bool last = !SUMS || chain + 1 == n_chains;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_full[buf]), n_done / n_buf & 1u, &s_abort));
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait_cluster(smem_u32(&acc_full[buf]), n_done / n_buf & 1u, &s_abort, a.poll_limit));
             if (!ok) { give_up(ST_WAIT_FULL); break; }
             tc_fence_after();
             for (uint32_t c = half * 16; c < it.rows; c += 32) {
@@ -655,7 +654,7 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
             n_next = ask_rows(i + n_pairs);
             for (uint32_t ks = ks0 + (turn + GT_STAGES - base) % GT_STAGES; ks < ks1; ks += GT_STAGES) {
                 const uint32_t sb = ring + GT_X + slot * x_slot;
-                if (!mbar_wait_warp_at(smem_u32(&x_empty[slot]), ph ^ 1u, &s_abort)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
+                if (!mbar_wait_warp_at(smem_u32(&x_empty[slot]), ph ^ 1u, &s_abort, a.poll_limit)) { give_up(ST_WAIT_EMPTY); ok = false; break; }
                 const uint32_t k = ks * GT_KS + chunk * 8;
                 const bool there = k < a.K;                       // K is a multiple of 8
                 const uint16_t* x = static_cast<const uint16_t*>(a.x) + (there ? k : 0);
@@ -675,10 +674,13 @@ __global__ void __launch_bounds__(GT_THREADS, 1) grouped_tile_kernel(const __gri
         }
     }
     // every thread comes here, also after a give-up
+    if (s_abort) cluster_abort(&s_abort, 2 * P.parts);
     tc_fence_before();
     __syncwarp();
     cluster_sync_all();
-    if (P.parts > 1 && pair < n_items) {
+    const bool gave_up = s_abort != 0;                  // in every CTA of the cluster alike: a part of the sums may be missing
+    if (gave_up) abort_drain();
+    if (P.parts > 1 && pair < n_items && !gave_up) {
         // the parts of a share of the rows, in order, over distributed shared memory: a thread four outputs of a row, of both accumulators
         GtWalk w{s_off, s_tiles, a.G};
         const GtItem it = w.at(pair / P.n_ft);

@@ -302,6 +302,8 @@ struct GroupedArgs {
     size_t ld_x, ld_y, ld_w, w_stride;
     uint32_t* status;
     int sm_count;
+    uint32_t poll_limit = 1u << 20;    // polls after which a wait gives up
+    uint32_t withhold = 0;             // self-test: every producer leaves out its n-th ring stage (0: off)
     __host__ __device__ uint32_t n_w() const { return swiglu ? 2 * N : N; }
 };
 cudaError_t launch_grouped(const GroupedArgs& a, cudaStream_t st);
@@ -321,6 +323,8 @@ struct AdaptersArgs {
     size_t ld_x, ld_base, ld_y, a_stride, b_stride;
     uint32_t* status;
     int sm_count;
+    uint32_t poll_limit = 1u << 20;    // as for the grouped products
+    uint32_t withhold = 0;
 };
 cudaError_t launch_adapters(const AdaptersArgs& a, cudaStream_t st);
 

@@ -40,9 +40,9 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 // a bounded wait by all lanes of a warp: one answer for the warp
-__device__ __forceinline__ bool mbar_wait_warp_at(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool mbar_wait_warp_at(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit = (1u << 20)) {
     if (__all_sync(0xFFFFFFFFu, mbar_try_wait_at(bar, parity))) return true;
-    return __all_sync(0xFFFFFFFFu, mbar_wait_bounded_at(bar, parity, abort_flag));
+    return __all_sync(0xFFFFFFFFu, mbar_wait_bounded_at(bar, parity, abort_flag, 0, limit));
 }
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t sleep_ns = 0,
                                                uint32_t limit = (1u << 20)) {

@@ -39,12 +39,20 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
     return ok != 0;
 }
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t limit = (1u << 20)) {
-    for (uint32_t i = 0; i < limit; ++i) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    for (uint32_t i = 1; i < limit; ++i) {
         if (mbar_try_wait_cluster(bar, parity)) return true;
         if ((i & 63u) == 63u && *abort_flag) return false;
     }
     return false;
 }
+// A wait of this CTA has run out: before the CTAs meet for the last time every one of the cluster is told, so that none goes on with what is missing
+__device__ __forceinline__ void cluster_abort(volatile int* abort_flag, uint32_t n_ctas) {
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(const_cast<int*>(abort_flag));
+    for (uint32_t r = 0; r < n_ctas; ++r) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_rank(at, r)), "r"(1u) : "memory");
+}
+// after a give-up: copies and products in flight end before the memory goes
+__device__ __forceinline__ void abort_drain() { for (int i = 0; i < 2000; ++i) __nanosleep(1000); }
 // Tensor-map copies into this CTA's shared memory whose bytes count on a barrier of either CTA of the pair.  The innermost
 // coordinate is a multiple of 16 bytes; no multicast.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, int32_t c3, uint32_t bar) {

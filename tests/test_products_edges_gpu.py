@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from __graft_entry__ import load_package
-from test_products_gpu import CODE, DT, STEP, half_step
+from test_products_gpu import CODE, DT, SENTINEL, STEP, half_step
 
 pytestmark = pytest.mark.gpu
 pkg = load_package()
@@ -336,3 +336,65 @@ def test_layers_of_two_handles_on_two_threads(bank, T):
             assert torch.equal(y.view(torch.int16), want.view(torch.int16)) and m.stats().device_status == 0
         return work
     assert in_threads([calls(512, 256, 8), calls(5120, 512, 64)]) == []
+
+
+# ------------------------------------------------------------------------------------------------------------
+# waits that run out
+# ------------------------------------------------------------------------------------------------------------
+@pytest.fixture
+def waiting():
+    """A handle of the test's own, whose waits are short while a ring stage is left out of every producer's."""
+    m = pkg.MoE(pkg.make_config(128, 128, 4, 1, max_tokens=4))
+    yield m
+    m.debug_wait(0, 0)
+    m.close()
+
+
+def runs_out(m, call, y, stage, writes_nothing=True):
+    """`call` writes y: it returns, reports, stores nothing that waited, and the call after it is right."""
+    y.fill_(SENTINEL)
+    call()
+    torch.cuda.synchronize()
+    good = y.clone()
+    assert m.stats().device_status == 0 and not (good == SENTINEL).any()
+    y.fill_(SENTINEL)
+    m.debug_wait(poll_limit=300, withhold_stage=stage)
+    call()
+    torch.cuda.synchronize()
+    m.debug_wait(0, 0)
+    assert m.stats().device_status in (2, 3)
+    left = y == SENTINEL
+    assert left.all() if writes_nothing else torch.equal(y[~left], good[~left]) and left.any()
+    m.status_clear()
+    assert m.stats().device_status == 0
+    call()
+    torch.cuda.synchronize()
+    assert m.stats().device_status == 0 and torch.equal(y, good)
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("rows, K, N, stage", [(64, 5120, 2304, 1), (64, 5120, 2304, 5), (300, 5120, 2304, 2), (3000, 1024, 1024, 1)])
+def test_tiles_whose_wait_runs_out(waiting, rows, K, N, stage, out, gather):
+    """Parts of the reduction over a cluster (64 and 300 rows), and pairs that walk the tiles."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, K, device="cuda", generator=gen).to(torch.bfloat16)
+    w = (torch.randn(N, K, device="cuda", generator=gen) * K ** -0.5).to(torch.bfloat16)
+    y = torch.empty(rows, N, device="cuda", dtype=DT[out])
+    order = torch.arange(rows, device="cuda", dtype=torch.int32)
+    runs_out(waiting, lambda: waiting.grouped(x.data_ptr(), w.data_ptr(), None, y.data_ptr(), rows, 1, K, N, out_dtype=CODE[out],
+                                              order=order.data_ptr(), gather=gather, stream=stream()), y, stage)
+
+
+@pytest.mark.parametrize("T, n, R, stage", [(1000, 8, 64, 1), (1000, 8, 128, 7), (200, 1, 128, 1), (3000, 2, 64, 35)])
+@pytest.mark.parametrize("dtype, out", [("bf16", "f32"), ("f16", "f16")])
+def test_adapters_whose_wait_runs_out(waiting, T, n, R, stage, dtype, out):
+    """Stages of the inner product, and of the outer one (the last case: 46 units, clusters of two, 32 stages and then eight)."""
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randn(T, 4096, device="cuda", generator=gen).to(DT[dtype])
+    a = (torch.randn(n, R, 4096, device="cuda", generator=gen) / 64).to(DT[dtype])
+    b = torch.randn(n, 2048, R, device="cuda", generator=gen).to(DT[dtype])
+    ids = (torch.arange(T, device="cuda") % n).to(torch.int32)
+    y = torch.empty(T, 2048, device="cuda", dtype=DT[out])
+    runs_out(waiting, lambda: waiting.adapters(x.data_ptr(), T, a.data_ptr(), b.data_ptr(), ids.data_ptr(), y.data_ptr(), 4096, 2048, R, n,
+                                               dtype=CODE[dtype], out_dtype=CODE[out], stream=stream()), y, stage, writes_nothing=stage < 35)
