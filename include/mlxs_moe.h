@@ -223,7 +223,8 @@ int mlxs_moe_fp4_native_probe(int32_t device, uint32_t rate_mmas, mlxs_fp4_nativ
 int mlxs_moe_mma_rate(int32_t device, uint32_t n, int a_from_tmem, uint32_t mmas, double *ns_per_mma);
 
 int mlxs_moe_stats_get(mlxs_moe *h, mlxs_moe_stats *out);
-/* The device status word is sticky (a host must see a fault it did not poll for): once a kernel has recorded an error
+/* The device status word is sticky (a host must see a fault it did not poll for) and keeps the gravest of what was recorded: a run that failed, then
+ * expert ids out of range, then what a call answers as documented (rows skipped, offsets cut, adapter ids that count as none).  Once a kernel has recorded an error
  * every mlxs_moe_forward_host returns MLXS_E_DEVICE_STATUS until the host acknowledges it here.  Synchronises the
  * device, clears the word and the streaming kernels' arrival counters a call that gave up may have left behind.
  * No counterpart in the reference (its kernels have no device-side error word). */

@@ -901,8 +901,8 @@ static int read_status(mlxs_moe* h, cudaStream_t st) {
     uint32_t s = 0;
     CU(cudaMemcpyAsync(&s, h->status, 4, cudaMemcpyDeviceToHost, st));
     CU(cudaStreamSynchronize(st));
-    h->stats.device_status = s;
-    if (s) return fail(MLXS_E_DEVICE_STATUS, "device status %u (%s)", s,
+    h->stats.device_status = s & ST_CODE;
+    if (s) return fail(MLXS_E_DEVICE_STATUS, "device status %u (%s)", s & ST_CODE,
                        s == ST_BAD_EXPERT_ID ? "expert id out of range" : s == ST_NOT_LOADED ? "a routed expert is not resident"
                        : s == ST_WORKLIST_OVERFLOW ? "work list overflow"
                        : s == ST_EP_OVERFLOW ? "expert parallel: a rank received more rows than the workspace holds"
@@ -1003,7 +1003,7 @@ extern "C" int mlxs_moe_stats_get(mlxs_moe* h, mlxs_moe_stats* out) {
     CU(cudaDeviceSynchronize());
     CU(cudaMemcpy(hdr, h->tabs.header, sizeof hdr, cudaMemcpyDeviceToHost));
     CU(cudaMemcpy(&s, h->status, 4, cudaMemcpyDeviceToHost));
-    h->stats.device_status = s;
+    h->stats.device_status = s & ST_CODE;
     h->stats.distinct_experts_last = hdr[HDR_DISTINCT];
     h->stats.weight_bytes_last = (uint64_t)hdr[HDR_DISTINCT] * (h->last_logical ? h->last_logical : h->logical_bytes);
     h->stats.resident_bytes = h->resident;

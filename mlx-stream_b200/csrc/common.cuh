@@ -8,18 +8,21 @@
 namespace mlxs {
 
 // Error words kernels may write into the handle's status word (never trap, never spin without a bound).
+// What a kernel records in the handle's status word, by atomicMax: a code in the low byte, which is what the host reports, under a rank.  A run that failed hides
+// the ids that another call took for others, and those hide what a call answers as documented (rows skipped, offsets cut, ids that count as none).
+constexpr uint32_t ST_MISTAKEN = 1u << 8, ST_FAILED = 2u << 8, ST_CODE = 0xFFu;
 enum : uint32_t {
     ST_OK = 0,
-    ST_BAD_EXPERT_ID = 1,    // a routed id outside [0, n_experts)
-    ST_WAIT_FULL = 2,        // a consumer's bounded wait for a staged copy ran out
-    ST_WAIT_EMPTY = 3,       // the producer's bounded wait for a free stage ran out
-    ST_WORKLIST_OVERFLOW = 4,
-    ST_NOT_LOADED = 5,       // a routed expert has no resident record
-    ST_EP_OVERFLOW = 6,      // expert parallel: a rank received more rows than its workspace holds
-    ST_EP_TIMEOUT = 7,       // expert parallel: a peer's epoch word did not arrive within the bound
-    ST_BAD_ROW = 8,          // grouped product: a gathered or scattered row outside its buffer
-    ST_BAD_OFFSETS = 9,      // grouped product: group offsets that descend or pass the call's rows
-    ST_BAD_ADAPTER = 10      // adapters: an id outside [.., n_adapters)
+    ST_BAD_EXPERT_ID = ST_MISTAKEN | 1,      // a routed id outside [0, n_experts)
+    ST_WAIT_FULL = ST_FAILED | 2,            // a consumer's bounded wait for a staged copy ran out
+    ST_WAIT_EMPTY = ST_FAILED | 3,           // the producer's bounded wait for a free stage ran out
+    ST_WORKLIST_OVERFLOW = ST_FAILED | 4,
+    ST_NOT_LOADED = ST_FAILED | 5,           // a routed expert has no resident record
+    ST_EP_OVERFLOW = ST_FAILED | 6,          // expert parallel: a rank received more rows than its workspace holds
+    ST_EP_TIMEOUT = ST_FAILED | 7,           // expert parallel: a peer's epoch word did not arrive within the bound
+    ST_BAD_ROW = 8,                          // grouped product: a gathered or scattered row outside its buffer
+    ST_BAD_OFFSETS = 9,                      // grouped product: group offsets that descend or pass the call's rows
+    ST_BAD_ADAPTER = 10                      // adapters: an id outside [.., n_adapters)
 };
 
 constexpr uint32_t SCALE_BITS = 0x3DB504F3u;  // 128^-0.5 (src/arch/deepseek_v41/experts.zig:428-429)

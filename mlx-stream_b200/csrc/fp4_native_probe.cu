@@ -298,7 +298,7 @@ extern "C" int mlxs_moe_fp4_native_probe(int32_t device, uint32_t rate_mmas, mlx
     if (e == cudaSuccess) cudaMemcpy(&st, d_status, 4, cudaMemcpyDeviceToHost);
     cudaFree(dbuf);
     if (e != cudaSuccess) return mlxs_fail(MLXS_E_CUDA, "fp4_native_probe: %s", cudaGetErrorString(e));
-    if (st) return mlxs_fail(MLXS_E_DEVICE_STATUS, "fp4_native_probe: a bounded wait ran out (status %u)", st);
+    if (st) return mlxs_fail(MLXS_E_DEVICE_STATUS, "fp4_native_probe: a bounded wait ran out (status %u)", st & ST_CODE);
     out->rel_l2_hi_lo = errs[1];
     out->rel_l2_hi_only = errs[0];
     out->tflops_f16 = tf[0];
@@ -337,7 +337,7 @@ extern "C" int mlxs_moe_mma_rate(int32_t device, uint32_t n, int a_from_tmem, ui
     cudaEventDestroy(b);
     cudaFree(d_status);
     if (e != cudaSuccess) return mlxs_fail(MLXS_E_CUDA, "mma_rate: %s", cudaGetErrorString(e));
-    if (st) return mlxs_fail(MLXS_E_DEVICE_STATUS, "mma_rate: a bounded wait ran out (status %u)", st);
+    if (st) return mlxs_fail(MLXS_E_DEVICE_STATUS, "mma_rate: a bounded wait ran out (status %u)", st & ST_CODE);
     *ns_per_mma = (double)ms * 1e6 / (double)mmas;
     return MLXS_OK;
 }

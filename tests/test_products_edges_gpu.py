@@ -398,3 +398,36 @@ def test_adapters_whose_wait_runs_out(waiting, T, n, R, stage, dtype, out):
     y = torch.empty(T, 2048, device="cuda", dtype=DT[out])
     runs_out(waiting, lambda: waiting.adapters(x.data_ptr(), T, a.data_ptr(), b.data_ptr(), ids.data_ptr(), y.data_ptr(), 4096, 2048, R, n,
                                                dtype=CODE[dtype], out_dtype=CODE[out], stream=stream()), y, stage, writes_nothing=stage < 35)
+
+
+def test_a_failed_run_is_not_hidden_by_what_a_call_answers_as_documented(waiting):
+    """The status word is sticky: an adapter id that counts as none before, or after, a wait that ran out; a slot id taken for another."""
+    x, w = torch.randn(64, 1024, device="cuda").to(torch.bfloat16), torch.randn(512, 1024, device="cuda").to(torch.bfloat16)
+    a, b = torch.randn(1, 8, 1024, device="cuda").to(torch.bfloat16), torch.randn(1, 512, 8, device="cuda").to(torch.bfloat16)
+    y = torch.zeros(64, 512, device="cuda", dtype=torch.bfloat16)
+    ids = torch.ones(64, device="cuda", dtype=torch.int32)
+    slots = torch.tensor([0, 99, 1], device="cuda", dtype=torch.int32)
+    order, offsets = torch.zeros(3, device="cuda", dtype=torch.int32), torch.zeros(5, device="cuda", dtype=torch.int32)
+
+    def bad_id():
+        waiting.adapters(x.data_ptr(), 64, a.data_ptr(), b.data_ptr(), ids.data_ptr(), y.data_ptr(), 1024, 512, 8, 1, stream=stream())
+
+    def bad_slot():
+        waiting.sort_rows(slots.data_ptr(), 3, 4, order.data_ptr(), offsets.data_ptr(), stream())
+
+    def lost_wait():
+        waiting.debug_wait(poll_limit=300, withhold_stage=1)
+        waiting.grouped(x.data_ptr(), w.data_ptr(), None, y.data_ptr(), 64, 1, 1024, 512, stream=stream())
+        waiting.debug_wait(0, 0)
+
+    def status_after(*calls):
+        waiting.status_clear()
+        for c in calls:
+            c()
+        torch.cuda.synchronize()
+        return waiting.stats().device_status
+    assert status_after(bad_id) == 10 and status_after(bad_slot) == 1 and status_after(lost_wait) in (2, 3)
+    assert status_after(bad_id, lost_wait) in (2, 3) and status_after(lost_wait, bad_id) in (2, 3)
+    assert status_after(bad_slot, lost_wait) in (2, 3) and status_after(lost_wait, bad_slot) in (2, 3)
+    assert status_after(bad_id, bad_slot) == 1 and status_after(bad_slot, bad_id) == 1
+    waiting.status_clear()
