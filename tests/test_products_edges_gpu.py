@@ -7,13 +7,16 @@ Tolerances, from the arithmetic alone.
   * f32 outputs of products of random signs are held to what f32 sums give: 2^-20 of the result in the 2-norm (eight steps: 16 instructions' truncations over an
     accumulator that holds half of its last value on average), or one and a half times the error of the same product in 32 bits, where that is more.
 """
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
 
 from __graft_entry__ import load_package
-from test_products_gpu import CODE, DT, SENTINEL, STEP, half_step
+from test_products_gpu import CODE, DT, FIRST_CALLS, SENTINEL, SIZES, STEP, Adapters, Grouped, half_step, some_ids
 
 pytestmark = pytest.mark.gpu
 pkg = load_package()
@@ -431,3 +434,115 @@ def test_a_failed_run_is_not_hidden_by_what_a_call_answers_as_documented(waiting
     assert status_after(bad_slot, lost_wait) in (2, 3) and status_after(lost_wait, bad_slot) in (2, 3)
     assert status_after(bad_id, bad_slot) == 1 and status_after(bad_slot, bad_id) == 1
     waiting.status_clear()
+
+
+# ------------------------------------------------------------------------------------------------------------
+# kernels that the other file's sizes and types do not take
+# ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("layout", ["out_in", "in_out"])
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+@pytest.mark.parametrize("sizes", ["one", "decode", "all_in_last", "sixteens", "big"])
+def test_grouped_f16_with_f32_outputs(moe, sizes, act, layout):
+    c = Grouped(SIZES[sizes], 264, 136, "f16", "f32", layout, act, 1.0 if act == "swiglu" else 0.0, gather=sizes == "decode", scatter=True, x_div=2, pad=8, spare_rows=3)
+    c.call(moe)
+    c.check()
+
+
+@pytest.mark.parametrize("dtype, out", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("sizes", ["sixteens", "big"])
+def test_grouped_of_more_inputs_than_a_chain(moe, sizes, dtype, out):
+    """Odd lengths of the last chain and stage, with running sums for 16-bit outputs (f16)."""
+    for K, layout, act in ((8200, "out_in", "none"), (8648, "in_out", "swiglu"), (9216, "out_in", "swiglu")):
+        c = Grouped(SIZES[sizes], K, 72, dtype, out, layout, act, gather=K == 8648, scatter=True, pad=8, spare_rows=2)
+        c.call(moe)
+        first = c.y_all.clone()
+        c.check(K)
+        c.call(moe)
+        torch.cuda.synchronize()
+        assert torch.equal(c.y_all, first)
+
+
+@pytest.mark.parametrize("R", [40, 64, 72, 120, 128])
+@pytest.mark.parametrize("K, N", [(8, 8), (72, 264), (1032, 1400), (2304, 512)])
+@pytest.mark.parametrize("T, n", [(500, 7), (5000, 5)])
+def test_adapters_on_the_tensor_cores_of_the_layer_calls_types(moe, T, n, R, K, N):
+    for dtype, out, in_place in (("bf16", "f32", True), ("f16", "f16", False)):
+        ranks = [max(1, R - 3 * i) for i in range(n)] if in_place else None
+        c = Adapters(some_ids(T, n, "mixed" if in_place else "runs"), n, R, K, N, dtype, out, ranks=ranks, pad=8, in_place=in_place)
+        c.call(moe)
+        first = c.y_all.clone()
+        c.check((dtype, out))
+        if not in_place:
+            c.call(moe)
+            torch.cuda.synchronize()
+            assert torch.equal(c.y_all, first)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T, n, R, K", [(5, 2, 16, 20008), (50, 1, 64, 33000), (300, 2, 256, 20480), (700, 600, 24, 16392), (1000, 8, 64, 24584)])
+def test_adapters_of_long_inputs_with_16_bit_outputs(moe, T, n, R, K, dtype):
+    c = Adapters(some_ids(T, n, "mixed"), n, R, K, 72, dtype, pad=8)
+    c.call(moe)
+    c.check()
+
+
+def test_adapters_of_two_ranks_in_one_graph(moe):
+    """One kernel with two amounts of shared memory, captured side by side and replayed; eager calls of other ranks in between."""
+    calls = [Adapters(some_ids(T, n, "mixed", T), n, R, 520, 264, "bf16", out, ranks=[R, 1, R - 4], seed=R)
+             for T, n, R, out in ((1000, 3, 64, "f32"), (1000, 3, 128, "f32"), (40, 3, 256, "bf16"), (40, 3, 8, "bf16"), (500, 3, 16, "bf16"), (500, 3, 256, "bf16"))]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for c in calls:
+            c.call(moe, stream())
+    for c in calls:
+        c.y_all.fill_(SENTINEL)
+    for _ in range(2):
+        g.replay()
+        Adapters(some_ids(300, 3, "mixed"), 3, 72, 520, 264, "bf16", "f32").call(moe)
+        torch.cuda.synchronize()
+        for c in calls:
+            c.check()
+
+
+@pytest.mark.parametrize("rows, T", [(400, 400), (1000, 900)])
+def test_a_process_whose_first_calls_of_the_tensor_core_kernels_are_captured(rows, T):
+    """400 tokens of two adapters, rank 64: the adapters' tensor map and its query of the clusters that fit happen inside the capture."""
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(rows), str(T)], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("T, R", [(400, 64), (900, 128), (300, 200)])
+def test_shared_expert_with_adapters_of_many_tokens(T, R):
+    """The layer call where its adapters take the tensor cores (bf16 inputs, f32 rows in place): what the routed rows, weighted by zero, leave."""
+    H, I, E, k, n = 512, 384, 4, 2, 3
+    m = pkg.MoE(pkg.make_config(H, I, E, k, bank_kind=pkg.BANK_MXFP4, act_limit=1.5, shared_expert=True, max_tokens=T))
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    logical, _ = m.record_bytes()
+    record = torch.zeros(logical, device="cuda", dtype=torch.uint8)
+    for e in range(E):
+        m.load_expert(0, e, record.data_ptr(), logical, True)
+
+    def rnd(*shape, std=1.0):
+        return (torch.randn(*shape, device="cuda", generator=gen) * std).to(torch.bfloat16)
+    w1, w3, w2 = rnd(I, H, std=H ** -0.5), rnd(I, H, std=H ** -0.5), rnd(H, I, std=I ** -0.5)
+    m.set_shared(0, w1.data_ptr(), w3.data_ptr(), w2.data_ptr(), True)
+    m.reserve_adapters()
+    ad = {"a1": rnd(n, R, H, std=H ** -0.5), "b1": rnd(n, I, R, std=0.1), "a3": rnd(n, R, H, std=H ** -0.5), "b3": rnd(n, I, R, std=0.1),
+          "a2": rnd(n, R, I, std=I ** -0.5), "b2": rnd(n, H, R, std=0.1)}
+    x, y = rnd(T, H), torch.empty(T, H, device="cuda", dtype=torch.bfloat16)
+    ids = torch.zeros(T, k, device="cuda", dtype=torch.int32)
+    ids[:, 1] = 1
+    weights, aid = torch.zeros(T, k, device="cuda"), torch.tensor(some_ids(T, n, "mixed", T), device="cuda", dtype=torch.int32)
+    full = pkg.make_shared_adapters(R, n, **{c: v.data_ptr() for c, v in ad.items()})
+    m.experts_adapted(0, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), T, full, aid.data_ptr(), y.data_ptr(), stream())
+    torch.cuda.synchronize()
+    assert m.stats().device_status == 0
+
+    def linear(v, w, a, b):
+        return lora_plain(v, a, b, aid, v @ w.double().T, None, torch.float64)
+    gate, up = linear(x.double(), w1, ad["a1"], ad["b1"]).clamp(max=1.5), linear(x.double(), w3, ad["a3"], ad["b3"]).clamp(-1.5, 1.5)
+    h = (gate * torch.sigmoid(gate) * up).to(torch.bfloat16).double()
+    # half a step of the output, and of those values of h whose f32 sums lie next to a rounding border (one in a hundred at most)
+    assert norm_off(y, linear(h, w2, ad["a2"], ad["b2"])) <= 2.0 ** -8 * 1.1
+    m.close()
