@@ -546,3 +546,80 @@ def test_shared_expert_with_adapters_of_many_tokens(T, R):
     # half a step of the output, and of those values of h whose f32 sums lie next to a rounding border (one in a hundred at most)
     assert norm_off(y, linear(h, w2, ad["a2"], ad["b2"])) <= 2.0 ** -8 * 1.1
     m.close()
+
+
+# ------------------------------------------------------------------------------------------------------------
+# the largest calls, and calls behind copies
+# ------------------------------------------------------------------------------------------------------------
+def test_grouped_most_rows_and_groups(moe):
+    """2^22 sorted positions of 1024 groups, gathered and scattered."""
+    gen = torch.Generator().manual_seed(1)
+    cuts = torch.sort(torch.randint(0, 2 ** 22 + 1, (1023,), generator=gen)).values.tolist()
+    sizes = [b - a for a, b in zip([0] + cuts, cuts + [2 ** 22])]
+    c = Grouped(sizes, 16, 8, "bf16", "f32", gather=True, scatter=True, x_div=8)
+    c.call(moe)
+    c.check()
+    assert moe.stats().device_status == 0
+
+
+@pytest.mark.parametrize("n", [3, 511, 2047, 5000])
+def test_adapters_most_tokens(moe, n):
+    T = 2 ** 22
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(T, 8, device="cuda", generator=gen).to(torch.bfloat16)
+    a, b = torch.randn(n, 8, 8, device="cuda", generator=gen).to(torch.bfloat16), torch.randn(n, 8, 8, device="cuda", generator=gen).to(torch.bfloat16)
+    ids = torch.randint(-1, n, (T,), device="cuda", generator=gen).to(torch.int32)
+    y = lora(moe, x, a, b, ids, torch.float32)
+    at = torch.randint(0, T, (20000,), device="cuda", generator=gen)
+    at[:3] = torch.tensor([0, T - 1, T - 2], device="cuda")
+    i = ids[at].long().clamp(min=0)
+    u = torch.einsum("tk,trk->tr", x[at].double(), a[i].double())
+    want = torch.einsum("tr,tor->to", u, b[i].double()) * (ids[at] >= 0)[:, None]
+    assert norm_off(y[at], want) <= 2.0 ** -20 and (y[ids < 0] == 0).all()
+    assert moe.stats().device_status == 0
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("layout", ["out_in", "in_out"])
+@pytest.mark.parametrize("K, N", [(262144, 8), (8, 262144)])
+def test_grouped_longest_and_widest(moe, K, N, layout, rows):
+    for act in ("none", "swiglu"):
+        c = Grouped([rows], K, N, "bf16", "f32", layout, act)
+        c.call(moe)
+        c.check(act)
+
+
+@pytest.mark.parametrize("T", [3, 40, 300])
+@pytest.mark.parametrize("K, N", [(262144, 8), (8, 262144)])
+def test_adapters_longest_and_widest(moe, K, N, T):
+    for R in (16, 64, 256):
+        c = Adapters([0] * T, 1, R, K, N, "bf16", "f32")
+        c.call(moe)
+        c.check(R)
+
+
+def test_products_behind_copies_in_a_graph(moe):
+    """A call's launch begins under the one before it; behind a copy or a memset of a graph it waits as any other."""
+    g40, g9 = Grouped([20, 0, 20], 264, 136, gather=True), Grouped([4, 5], 264, 136)
+    ad = Adapters(some_ids(500, 3, "mixed"), 3, 64, 264, 136, "bf16", "f32", in_place=True)
+    few = Adapters(some_ids(9, 3, "mixed"), 3, 16, 264, 136)
+    calls = (g40, g9, ad, few)
+    sources = [c.x_all.clone() for c in calls]
+    base = ad.y_all.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for c, s in zip(calls, sources):
+            c.x_all.copy_(s)
+            if c is ad:
+                c.y_all.copy_(base)
+            c.call(moe, stream())
+    for k in range(3):
+        for c, s in zip(calls, sources):
+            s.mul_(-1.0)                                 # the rows of this replay
+            c.x_all.zero_()
+            if c is not ad:
+                c.y_all.fill_(SENTINEL)
+        graph.replay()
+        torch.cuda.synchronize()
+        for c in calls:
+            c.check(k)
