@@ -12,8 +12,9 @@
 //     factors is far inside an output's rounding; three of bf16, 24 bits, where outputs are f32 (rank 64, 5120 inputs, no base: two parts 2.5e-6 off 64 bits,
 //     f32 2.3e-7).  f16 parts are scaled by the row's largest power of two, since A x may pass f16's range where y does not.
 //   * base is added in f32, one rounding.
-// Measured (GPU time, other inputs every call): one token of rank 16, 5120 -> 2304: 6.7 us, a chain of two cluster barriers and three cold loads; 64 tokens of 48
-// adapters, rank 32: 13 us (floor 2.6); 4000 of eight, rank 32: 38 us (floor 12.5); 8192 tokens of six, rank 64, 4096 -> 2048: 55 us (floor 21); 999 of 24, rank 128, f32: 36 us (floor 14).
+// Measured (GPU time, other inputs every call): one token of rank 16, 5120 -> 2304: 7.3 us, a chain of two cluster barriers and three cold loads; 64 tokens of 48
+// adapters, rank 32: 10.3 us (floor 1.7), f32 outputs 11.2; 4000 of eight, rank 32: 38.5 us (floor 12.5), f32 outputs 44; 8192 tokens of six, rank 64, 4096 -> 2048: 56.5 us (floor
+// 19.7), f32 outputs 68; 999 of 24, rank 128, f16, f32 outputs: 37 us (floor 10.3); 8192 of six, rank 256 (mma.sync): 290 us (floor 23), f32 outputs 382.
 // The mma.sync kernels take operands straight from global memory as fragments, 16 bytes per lane: a lane's eight consecutive inputs stand for the k
 // positions 2t, 2t+1, 2t+8, 2t+9 of two products, the same for both operands.
 #include <type_traits>
@@ -801,9 +802,9 @@ __global__ void __launch_bounds__(AD_WARPS * 32, 2) adapters_sorted_kernel(const
 // the adapter's rank).  A warp to a ring slot, one that issues the products, eight that read accumulators: inner sums -> shared memory -> the cluster's fold ->
 // parts of u as operand rows; outputs -> turned through shared memory -> + base -> y.  The fold's steps are joined by mbarriers between the CTAs, so the
 // ring runs on underneath.  Every wait is bounded: a give-up sets the status word, and everybody still meets at the end.
-// 8192 tokens of six adapters, rank 64, 4096 -> 2048, in cycles: sort 8,500, start 3,500, inner 35,000 (the issuer: 400 for a stage's four small MMAs), fold
-// 7,000, outer 40,000 (16 blocks of 128 outputs; each a chain of tensor-memory read, turn, base and store over eight warps): 55 us against 71 with
-// mma.sync.  Measured and not kept: base through the ring (52 -> 51 us, rank 128 with f32 outputs 36 -> 51), prefetches of x and base into L2 (their issue
+// 8192 tokens of six adapters, rank 64, 4096 -> 2048, in cycles (with one buffer of accumulators; with two the call takes 1 us more): sort 8,500, start 3,500,
+// inner 35,000 (the issuer: 400 for a stage's four small MMAs), fold 7,000, outer 40,000 (16 blocks of 128 outputs; each a chain of tensor-memory read, turn, base
+// and store over eight warps): 56.5 us against 71 with mma.sync.  Measured and not kept: base through the ring (52 -> 51 us, rank 128 with f32 outputs 36 -> 51), prefetches of x and base into L2 (their issue
 // takes what they save), 64-byte pieces of base one block further ahead.
 // The accumulators truncate (see the grouped products).  The inner product's stages go in order to accumulators of a few stages each, three to a buffer of two;
 // the epilogue warps add a buffer's, rounding, to sums in shared memory while the next one fills, so an inner product of any length has chains of

@@ -3,7 +3,7 @@
 // the call's rows alone (the groups' sizes are on the device):
 //   * up to 16 rows: grouped_few_kernel streams the weights through mma.sync (bound: HBM);
 //   * more: grouped_tile_kernel, tcgen05 tiles over CTA pairs.  Many rows per group are bound by the tensor pipe under the power cap, few by HBM:
-//     512 rows over 256 groups (K 2304, N 5120, f32) 0.75 ms = 6.7 TB/s, 1.02 of the measured copy rate, with the same tiles.
+//     512 rows over 256 groups (K 2304, N 5120, f32) 0.76 ms = 6.6 TB/s, 1.01 of the measured copy rate, with the same tiles.
 // 17 rows over 64 groups (K 5120, 2 x 2304 outputs): 121 us with the tiles (5.9 TB/s); 16 rows: 105 us streamed (6.3 TB/s) against 126 with the tiles.
 #include "common.cuh"
 #include "kernels.h"
@@ -257,7 +257,7 @@ static cudaError_t few_launch(const GroupedArgs& a, cudaStream_t st) {
 //   * gate and up are one accumulator each, so a thread has both of an output; the weights' box is gate rows behind up rows (a four-dimensional map);
 //   * weights with the inputs first are M-major operands: boxes of 64 outputs x 64 inputs, the same stage;
 //   * gathered rows come by cp.async into a ring of their own, two warps to a stage.  Tensor-map gathers (four rows to a copy) take 97 cycles each: 32768 rows 3.0 ms against
-//     1.05 now; one arrival per copying thread on the slot's barrier took longer than the stage (2400 rows 720 us against 390);
+//     1.29 to 1.32 now (gate and up of 2048, groups as routed; in sorted order and groups of 512 each 0.86 to 0.94); one arrival per copying thread on the slot's barrier took longer than the stage (2400 rows 720 us against 390);
 //   * the epilogue packs two rows to a word and turns 16 x 32 outputs through shared memory: 8-byte stores, 64 bytes of a row per warp.
 // Sorted rows, 64 groups of 512, K 4096, gate and up of 2048: 0.86 - 0.94 ms = 1,170 - 1,280 TFLOP/s, the tensor pipe busy 81 - 84 % of the cycles at 1.57 GHz (power
 // cap); one product of 8192^3 0.73 - 0.83 ms where the library's took 0.68 - 0.70.  What is left: a 256-row item has no second accumulator buffer (512 columns are full),
