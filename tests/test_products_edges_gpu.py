@@ -623,3 +623,14 @@ def test_products_behind_copies_in_a_graph(moe):
         torch.cuda.synchronize()
         for c in calls:
             c.check(k)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("T, n, R", [(700, 600, 256), (3000, 2047, 136), (200, 3, 136), (64, 2, 248), (9, 2, 136)])
+def test_adapters_of_ranks_above_128_with_f32_outputs(moe, T, n, R, dtype):
+    """The most shared memory (three parts, tables of many adapters), the first rank whose outer products are rounded, ranks of their own."""
+    c = Adapters(some_ids(T, n, "mixed"), n, R, 328, 136, dtype, "f32", ranks=[R - 8 * (i % 9) for i in range(n)], pad=8)
+    c.call(moe)
+    c.check()
+    off, off32 = adapters_off(moe, T, min(n, 20), R, 1032, 136, dtype, False)
+    assert as_f32(off, off32), (off, off32)
